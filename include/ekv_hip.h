@@ -482,6 +482,101 @@ int ekv_compact_slots(int32_t *indptr, void *slots, int32_t slot_bytes, const ui
                       void *out, int64_t *counts, int32_t write_back, void *stream);
 
 /*
+ * The arguments of ekv_prefix_attention.  Strides count elements; `tokens` query tokens in all, row r's
+ * at [q_start[r], q_start[r + 1]) (q_start NULL: one a row), never more than max_query.
+ */
+typedef struct ekv_attention {
+  const void *query;            /* [tokens, q_heads, head_dim] */
+  int64_t q_stride_token, q_stride_head;
+  const void *keys, *values;    /* element (block, pos, head, dim), both with the strides below */
+  int64_t kv_stride_block, kv_stride_pos, kv_stride_head;
+  int64_t blocks;               /* pages of the cache */
+  const int32_t *table;         /* [rows, width]: the rows' own pages */
+  int64_t table_stride;
+  const int32_t *lens;          /* [rows]: their tokens, the query tokens included */
+  const int32_t *q_start;       /* [rows + 1] or NULL */
+  const int32_t *prefix_table;  /* [prefix_groups, prefix_width]: the shared pages */
+  int64_t prefix_stride;
+  const int32_t *prefix_lens;   /* [prefix_groups] */
+  const int32_t *prefix_rows;   /* [prefix_groups + 1], ascending: group g's rows (NULL: one group of every row) */
+  float *scores;                /* [rows, kv_heads, >= width * block_size] or NULL */
+  int64_t scores_stride_row, scores_stride_head;
+  void *out;                    /* [tokens, q_heads, head_dim], the queries' type */
+  int64_t out_stride_token, out_stride_head;
+  float *lse;                   /* [tokens, q_heads], contiguous */
+  int32_t q_dtype, kv_dtype;
+  int32_t rows, width, prefix_groups, prefix_width, tokens, max_query;
+  int32_t q_heads, kv_heads, head_dim, block_size;
+  float scale, k_scale, v_scale, decay;
+} ekv_attention_t;
+
+/*
+ * One layer's attention over the paged cache, for a batch whose rows share prefixes.  No counterpart in
+ * the reference, which leaves attention to the serving engine.
+ *
+ * Query token i (of t) of row r sees every token of its group's prefix and the row's own slots
+ * j <= lens[r] - t + i.  With s = scale * k_scale * <q, k>, head hq reading KV head hq / (q_heads / kv_heads):
+ *     lse = log sum exp(s)        out = v_scale * sum exp(s - lse) v
+ * and a query that sees nothing has out 0 and lse -inf.  A table entry that is no page of the cache
+ * (negative, or blocks and more) is as if its tokens were not there.  What the cache holds in slots that
+ * no query of the row sees is never used, whatever it is.  A prefix's pages are read for all the queries
+ * of its group together.  Tokens of no row, and of a row past its max_query-th, get out 0 and lse -inf.
+ * With `scores`, each own slot j < lens[r] also accumulates the weight its key received:
+ *     scores[r, h, j] = decay * scores[r, h, j] + sum over the row's queries of head h of exp(s - lse)
+ * (other slots are left alone).  Sums, maxima and weights are float32; no atomics, so equal calls give
+ * equal bits.
+ * Types: fp32, f16 and bf16 with keys and values of the same type, or fp8 e4m3 keys and values with bf16
+ * queries.  head_dim 32, 64, 128 or 256; any block size and any number of query heads per KV head; rows of
+ * the query, keys and values start at multiples of 16 bytes; width * block_size below 2^31.
+ * workspace: ekv_prefix_attention_workspace(a) bytes of device memory (0: the arguments are refused or
+ * empty), 16-byte aligned, which the call may overwrite.
+ */
+size_t ekv_prefix_attention_workspace(const ekv_attention_t *a);
+int ekv_prefix_attention(const ekv_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The arguments of ekv_evict_tokens.  Strides count elements; the slots of a (row, head) are contiguous. */
+typedef struct ekv_eviction {
+  void *keys, *values;          /* element (block, pos, head, dim), both with the strides below */
+  int64_t kv_stride_block, kv_stride_pos, kv_stride_head;
+  int64_t blocks;               /* pages of the cache */
+  const int32_t *table;         /* [rows, width]: pages that no other row uses */
+  int64_t table_stride;
+  const int32_t *lens;          /* [rows] */
+  const int32_t *budget;        /* [rows], or NULL: fixed_budget for every row */
+  const int32_t *seen;          /* [rows]: the position the row's next token will have */
+  const float *scores;          /* [rows, kv_heads, width * block_size] */
+  int64_t scores_stride_row, scores_stride_head;
+  const int32_t *positions;     /* [rows, kv_heads, width * block_size] */
+  int64_t positions_stride_row, positions_stride_head;
+  float *new_scores;            /* scores itself, or a buffer that does not overlap it */
+  int64_t new_scores_stride_row, new_scores_stride_head;
+  int32_t *new_positions;       /* positions itself, or a buffer that does not overlap it */
+  int64_t new_positions_stride_row, new_positions_stride_head;
+  int32_t *new_lens;            /* [rows], not lens */
+  int32_t kv_dtype, rows, kv_heads, head_dim, width, block_size, fixed_budget, recent, sinks;
+  int32_t pad;
+} ekv_eviction_t;
+
+/*
+ * Evicts the cached tokens that accumulated least attention weight, per row and KV head.  No counterpart
+ * in the reference, whose budget works on whole blocks.
+ *
+ * Of the n = lens[r] tokens of (r, h) the b = min(n, max(budget, 0)) that come first in the order
+ * (protected first, then the higher score, then the lower slot) stay; a token is protected when
+ * positions[r, h, j] < sinks or >= seen[r] - recent.  A NaN score ranks with -inf.  The k-th token kept
+ * in a slot >= b moves into the k-th freed slot < b (its key and value in the cache, in place, its score
+ * and position in the new buffers); every other kept token stays in its slot.  From b to
+ * width * block_size the new scores are 0 and the new positions -1.  new_lens[r] = b, the same for every
+ * head.  A slot whose table entry is no page of the cache is neither read nor written.
+ * Keys and values fp32, f16, bf16 or fp8 e4m3; head_dim 32, 64, 128 or 256; rows at multiples of 16 bytes;
+ * width * block_size below 2^31, rows * kv_heads below 2^23.
+ * workspace: ekv_evict_tokens_workspace(rows, kv_heads, width * block_size) bytes, 16-byte aligned, which
+ * the call may overwrite.
+ */
+size_t ekv_evict_tokens_workspace(int32_t rows, int32_t kv_heads, int32_t capacity);
+int ekv_evict_tokens(const ekv_eviction_t *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Device memory, copies and IPC for the statistic planes.  They replace the ctypes calls
  * into libcudart of runtime/audit.py:17-23, :55-60, runtime/audit_kernel.py:146-158 and
  * observe/cuda.py:12-58.  These are not for hot loops.

@@ -22,6 +22,19 @@ int check_hip(hipError_t err, const char *what);
 // Number of compute units of the current device (cached per device).
 int cu_count();
 
+// pos / block_size by a multiplication, umulhi(2 * pos, mul) >> shift, exact for 0 <= pos < 2^31: with
+// L = ceil(log2(block_size)) and m = ceil(2^(31 + L) / block_size), m fits 32 bits and
+// floor(pos * m / 2^(31 + L)) is the quotient.
+struct PageDivisor {
+  uint32_t mul;
+  int shift;
+};
+inline PageDivisor page_divisor(int32_t block_size) {
+  int bits = 0;
+  while ((1ll << bits) < block_size) ++bits;
+  return {(uint32_t)((((uint64_t)1 << (31 + bits)) + block_size - 1) / block_size), bits};
+}
+
 // ---------------------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------------------

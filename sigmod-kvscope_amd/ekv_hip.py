@@ -44,6 +44,39 @@ class AuditLayer(ctypes.Structure):
     ]
 
 
+class Attention(ctypes.Structure):
+    """``ekv_attention_t``: the arguments of ``ekv_prefix_attention``."""
+
+    _fields_ = [
+        ("query", _p), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("keys", _p), ("values", _p), ("kv_stride_block", _i64), ("kv_stride_pos", _i64), ("kv_stride_head", _i64),
+        ("blocks", _i64), ("table", _p), ("table_stride", _i64), ("lens", _p), ("q_start", _p),
+        ("prefix_table", _p), ("prefix_stride", _i64), ("prefix_lens", _p), ("prefix_rows", _p),
+        ("scores", _p), ("scores_stride_row", _i64), ("scores_stride_head", _i64),
+        ("out", _p), ("out_stride_token", _i64), ("out_stride_head", _i64), ("lse", _p),
+        ("q_dtype", _i32), ("kv_dtype", _i32), ("rows", _i32), ("width", _i32), ("prefix_groups", _i32),
+        ("prefix_width", _i32), ("tokens", _i32), ("max_query", _i32), ("q_heads", _i32), ("kv_heads", _i32),
+        ("head_dim", _i32), ("block_size", _i32),
+        ("scale", _f32), ("k_scale", _f32), ("v_scale", _f32), ("decay", _f32),
+    ]
+
+
+class Eviction(ctypes.Structure):
+    """``ekv_eviction_t``: the arguments of ``ekv_evict_tokens``."""
+
+    _fields_ = [
+        ("keys", _p), ("values", _p), ("kv_stride_block", _i64), ("kv_stride_pos", _i64), ("kv_stride_head", _i64),
+        ("blocks", _i64), ("table", _p), ("table_stride", _i64), ("lens", _p), ("budget", _p), ("seen", _p),
+        ("scores", _p), ("scores_stride_row", _i64), ("scores_stride_head", _i64),
+        ("positions", _p), ("positions_stride_row", _i64), ("positions_stride_head", _i64),
+        ("new_scores", _p), ("new_scores_stride_row", _i64), ("new_scores_stride_head", _i64),
+        ("new_positions", _p), ("new_positions_stride_row", _i64), ("new_positions_stride_head", _i64),
+        ("new_lens", _p), ("kv_dtype", _i32), ("rows", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+        ("width", _i32), ("block_size", _i32), ("fixed_budget", _i32), ("recent", _i32), ("sinks", _i32),
+        ("pad", _i32),
+    ]
+
+
 _SIGNATURES: dict[str, list] = {
     "ekv_last_error": [],
     "ekv_abi_version": [],
@@ -134,6 +167,10 @@ _SIGNATURES: dict[str, list] = {
     "ekv_compact_slots": [
         _p, _p, _i32, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i64, _p, _p, _p, _i64, _p, _p, _i32, _p,
     ],
+    "ekv_prefix_attention_workspace": [_p],  # ctypes.addressof an Attention
+    "ekv_prefix_attention": [_p, _p, _sz, _p],
+    "ekv_evict_tokens_workspace": [_i32, _i32, _i32],
+    "ekv_evict_tokens": [_p, _p, _sz, _p],  # ctypes.addressof an Eviction
     "ekv_malloc": [ctypes.POINTER(ctypes.c_void_p), _sz],
     "ekv_free": [_p],
     "ekv_memset": [_p, ctypes.c_int, _sz],
