@@ -56,7 +56,7 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, int64_t item, Se
   item /= p.kv_heads;
   const int chunk = (int)(item % p.s_pre);
   int g, tile;
-  if (!find_tile<TILE>(p, (int)(item / p.s_pre), g, tile)) return false;
+  if (!find_tile(p, (int)(item / p.s_pre), TILE, g, tile)) return false;
   const RowQueries t = group_queries(p, g);
   s.table = p.ptable + (int64_t)g * p.ptable_stride;
   s.first = t.first;
@@ -251,12 +251,13 @@ template <class T, int D, bool WHOLE>
 __global__ __launch_bounds__(kThreads, D *T::kBytes <= 512 ? 2 : 1) void narrow_kernel(const Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t item = (int64_t)blockIdx.x * (kThreads / kWave) + wave;
+  const int64_t shared = p.wide_pre ? 0 : p.items_pre;  // items of the prefixes come first
   Segment s;
-  if (item < p.items_pre) {
+  if (item < shared) {
     if (!prefix_segment<kRowsPerTile>(p, item, s)) return;
   } else {
-    if (item - p.items_pre >= p.items_own) return;
-    if (!own_segment<kRowsPerTile>(p, item - p.items_pre, s)) return;
+    if (item - shared >= p.items_own) return;
+    if (!own_segment<kRowsPerTile>(p, item - shared, s)) return;
   }
   attend<T, D, WHOLE, kTiles<T, D>>(p, s);
 }
@@ -274,19 +275,6 @@ __device__ __forceinline__ int row_of(const Params &p, int token) {
   }
   return lo;
 }
-__device__ __forceinline__ int group_of(const Params &p, int row) {
-  if (p.groups == 0) return -1;
-  if (p.prows == nullptr) return 0;
-  if (row < p.prows[0] || row >= p.prows[p.groups]) return -1;
-  int lo = 0, hi = p.groups;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.prows[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 __device__ __forceinline__ void store(float *dst, float v) { *dst = v; }
 __device__ __forceinline__ void store(__bf16 *dst, float v) { *dst = (__bf16)v; }
 __device__ __forceinline__ void store(_Float16 *dst, float v) { *dst = (_Float16)v; }
@@ -306,10 +294,13 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
   if (i_q >= 0 && i_q < min(t.count, p.max_query)) {
     const int len = row_length(p, row);
     const int seen = min(len, len - t.count + 1 + i_q);
-    own = seen > 0 ? (seen - 1) / p.chunk_own + 1 : 0;
     const int g = group_of(p, row);
-    if (g >= 0) {
-      const int n = group_length(p, g);
+    const int n = g >= 0 ? group_length(p, g) : 0;
+    if (p.wide_own) {
+      const int64_t all = (int64_t)n + max(seen, 0);
+      own = all > 0 ? (int)((all - 1) / p.chunk_own) + 1 : 0;
+    } else {
+      own = seen > 0 ? (seen - 1) / p.chunk_own + 1 : 0;
       pre = n > 0 ? (n - 1) / p.chunk_pre + 1 : 0;
     }
   }
@@ -450,24 +441,54 @@ void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim,
   if (slots < 1) slots = 1;
 }
 
-void plan(Params &p, int head_dim) {
+// The wide kernel's: a few workgroups for each that the chip holds, no chunk shorter than 512 keys (its
+// partial outputs, written and read again, are as much traffic as 64 keys and values).
+void split_wide(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim, int &chunk, int &slots) {
+  int64_t n = ceil_div(4 * (int64_t)cu_count(), items_per_chunk > 0 ? items_per_chunk : 1);
+  const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
+  n = n > fit ? fit : n;
+  n = n > kMaxSlots ? kMaxSlots : n < 1 ? 1 : n;
+  const int64_t each = ceil_div(ceil_div(keys, n), 64) * 64;
+  chunk = (int)(each < 512 ? 512 : each > (1 << 30) ? INT32_MAX : each);
+  slots = (int)ceil_div(keys, chunk);
+  if (slots < 1) slots = 1;
+}
+
+void plan(Params &p, int head_dim, int kv_dtype) {
   const int64_t queries = (int64_t)p.tokens * p.q_heads;
-  p.tiles_own = (int)ceil_div((int64_t)p.max_query * p.group, kRowsPerTile);
-  split((int64_t)p.width * p.block_size, (int64_t)p.rows * p.kv_heads * p.tiles_own, queries, head_dim, p.chunk_own,
-        p.s_own);
-  p.items_own = (int64_t)p.rows * p.kv_heads * p.tiles_own * p.s_own;
+  const int64_t own_rows = (int64_t)p.max_query * p.group;
+  const bool half = kv_dtype != EKV_F32;
+  const int64_t axis = (int64_t)(p.width + (p.groups > 0 ? p.pwidth : 0)) * p.block_size;
+  p.wide_own = half && own_rows >= kWideRows && axis < (1 << 30);
+  p.wide_pre = half && !p.wide_own && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= kWideRows;
+  p.tile_own = p.wide_own ? wide_tile_rows() : kRowsPerTile;
+  p.tile_pre = p.wide_pre ? wide_tile_rows() : kRowsPerTile;
+  p.tiles_own = (int)ceil_div(own_rows, p.tile_own);
+  const int64_t own_keys = (int64_t)p.width * p.block_size, prefix_keys = p.groups > 0 ? (int64_t)p.pwidth * p.block_size : 0;
+  const int64_t own_items = (int64_t)p.rows * p.kv_heads * p.tiles_own;
   p.items_pre = 0;
   p.s_pre = 0;
   p.chunk_pre = 64;
-  if (p.groups > 0) {
-    p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, kRowsPerTile) + p.groups);
-    split((int64_t)p.pwidth * p.block_size, (int64_t)p.kv_heads * p.tiles_pre, queries, head_dim, p.chunk_pre,
-          p.s_pre);
-    p.items_pre = (int64_t)p.kv_heads * p.tiles_pre * p.s_pre;
+  if (p.wide_own) {
+    split_wide(own_keys + prefix_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
+  } else {
+    split(own_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
+    if (p.groups > 0) {
+      p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
+      const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
+      if (p.wide_pre) split_wide(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
+      else split(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
+      p.items_pre = items * p.s_pre;
+    }
   }
+  p.items_own = own_items * p.s_own;
+  p.direct = p.wide_own && p.s_own == 1;
 }
 
+int64_t narrow_items(const Params &p) { return p.wide_own ? 0 : p.items_own + (p.wide_pre ? 0 : p.items_pre); }
+
 size_t workspace_bytes(const Params &p, int head_dim) {
+  if (p.direct) return 16;
   return (size_t)(p.s_own + p.s_pre) * p.tokens * p.q_heads * ((size_t)head_dim * 4 + 8);
 }
 
@@ -476,14 +497,18 @@ int launch(const Params &p, hipStream_t stream) {
   const bool whole = p.block_size % 16 == 0;
   int rc = EKV_OK;
   if (p.tokens > 0) {
-    const unsigned grid = (unsigned)ceil_div(p.items_pre + p.items_own, kThreads / kWave);
-    if (whole) hipLaunchKernelGGL((narrow_kernel<T, D, true>), dim3(grid), dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((narrow_kernel<T, D, false>), dim3(grid), dim3(kThreads), 0, stream, p);
-    rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
-    if (rc != EKV_OK) return rc;
-    const unsigned joins = (unsigned)ceil_div((int64_t)p.tokens * p.q_heads, kThreads / kWave);
-    hipLaunchKernelGGL((combine_kernel<typename T::Query, D>), dim3(joins), dim3(kThreads), 0, stream, p);
-    rc = check_hip(hipGetLastError(), "ekv_prefix_attention combine launch");
+    if (p.wide_own || p.wide_pre) rc = wide_attention(p, T::kType, D, p.wide_own, stream);
+    const unsigned grid = (unsigned)ceil_div(narrow_items(p), kThreads / kWave);
+    if (rc == EKV_OK && grid > 0) {
+      if (whole) hipLaunchKernelGGL((narrow_kernel<T, D, true>), dim3(grid), dim3(kThreads), 0, stream, p);
+      else hipLaunchKernelGGL((narrow_kernel<T, D, false>), dim3(grid), dim3(kThreads), 0, stream, p);
+      rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
+    }
+    if (rc == EKV_OK && !p.direct) {
+      const unsigned joins = (unsigned)ceil_div((int64_t)p.tokens * p.q_heads, kThreads / kWave);
+      hipLaunchKernelGGL((combine_kernel<typename T::Query, D>), dim3(joins), dim3(kThreads), 0, stream, p);
+      rc = check_hip(hipGetLastError(), "ekv_prefix_attention combine launch");
+    }
   }
   if (rc != EKV_OK || p.scores == nullptr) return rc;
   if (p.width == 0) return rc;
@@ -570,8 +595,9 @@ int fill(const ekv_attention_t *a, Params &p) {
   p.scale2 = a->scale * a->k_scale * kLog2e;
   p.v_scale = a->v_scale;
   p.decay = a->decay;
-  plan(p, a->head_dim);
-  if (p.items_own + p.items_pre >= (1ll << 26) - 64 ||
+  plan(p, a->head_dim, a->kv_dtype);
+  // a launch has fewer than 2^32 threads: 64 an item of the narrow kernel, 256 of the wide one
+  if (narrow_items(p) >= (1ll << 26) - 64 || (p.wide_own ? p.items_own : p.wide_pre ? p.items_pre : 0) >= (1ll << 24) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
       (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >= (1ll << 26) - 64))
     return fail(EKV_EINVAL, "%s: %d rows of %d blocks and %d tokens of %d heads pass the threads of a launch", who,
@@ -598,7 +624,7 @@ extern "C" int ekv_prefix_attention(const ekv_attention_t *a, void *workspace, s
   if (rc != EKV_OK) return rc;
   if (p.tokens == 0 && (p.scores == nullptr || p.rows == 0)) return EKV_OK;
   if (p.rows == 0) return fail(EKV_EINVAL, "ekv_prefix_attention: %d tokens of no row", p.tokens);
-  if (p.k == nullptr || p.v == nullptr || p.lens == nullptr ||
+  if (((p.k == nullptr || p.v == nullptr) && (p.width > 0 || p.groups > 0)) || p.lens == nullptr ||
       (p.tokens > 0 && (p.q == nullptr || p.out == nullptr || p.lse == nullptr)) ||
       (p.table == nullptr && p.width > 0) || (p.groups > 0 && (p.ptable == nullptr || p.plens == nullptr)))
     return fail(EKV_EINVAL, "ekv_prefix_attention: null pointer");

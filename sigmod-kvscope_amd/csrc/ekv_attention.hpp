@@ -20,6 +20,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRowsPerTile = 16;  // query rows of one narrow tile (the matrix instruction's columns)
+constexpr int kWideRows = 64;     // from so many query rows a set of keys on, the wide kernel
 constexpr int kMaxSlots = 64;     // partial results a query row can have from its own pages, and from its prefix
 
 struct Params {
@@ -47,7 +48,12 @@ struct Params {
   float scale2, v_scale, decay;  // scale2: scale * k_scale * log2(e)
   // the split: own pages in s_own chunks of chunk_own keys, prefixes in s_pre chunks of chunk_pre
   int chunk_own, s_own, tiles_own, chunk_pre, s_pre, tiles_pre;
+  int tile_own, tile_pre;  // query rows of a tile
   int64_t items_own, items_pre;
+  // wide_own: the own keys of a row go through the wide kernel, behind its prefix's on one axis (no items of
+  // the prefix's own); wide_pre: the prefixes do.  direct: one chunk holds everything a query sees, so the
+  // wide kernel writes the result.
+  bool wide_own, wide_pre, direct;
 };
 
 __device__ __forceinline__ int page_of(const Params &p, int pos) {
@@ -63,21 +69,25 @@ __device__ __forceinline__ int page_of(const Params &p, int pos) {
 // they are summed in.
 
 struct F32 {
+  static constexpr int kType = EKV_F32;
   static constexpr int kBytes = 4;
   static constexpr int kStepDims = 4;  // dims of one matrix instruction
   typedef float Query;
 };
 struct F16 {
+  static constexpr int kType = EKV_F16;
   static constexpr int kBytes = 2;
   static constexpr int kStepDims = 32;
   typedef _Float16 Query;
 };
 struct BF16 {
+  static constexpr int kType = EKV_BF16;
   static constexpr int kBytes = 2;
   static constexpr int kStepDims = 32;
   typedef __bf16 Query;
 };
 struct FP8 {  // keys and values e4m3, queries bf16
+  static constexpr int kType = EKV_FP8_E4M3;
   static constexpr int kBytes = 1;
   static constexpr int kStepDims = 32;
   typedef __bf16 Query;
@@ -227,17 +237,30 @@ __device__ __forceinline__ int group_length(const Params &p, int g) {
   return min(max(p.plens[g], 0), p.pwidth * p.block_size);
 }
 
-// Group and tile of tile number `index` when every group's queries are cut into tiles of TILE query
+// The group of a row, or -1.
+__device__ __forceinline__ int group_of(const Params &p, int row) {
+  if (p.groups == 0) return -1;
+  if (p.prows == nullptr) return 0;
+  if (row < p.prows[0] || row >= p.prows[p.groups]) return -1;
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.prows[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Group and tile of tile number `index` when every group's queries are cut into tiles of `rows` query
 // rows; false past the last.  All 64 lanes call it with one index and receive one answer.
-template <int TILE>
-__device__ __forceinline__ bool find_tile(const Params &p, int index, int &g, int &tile) {
+__device__ __forceinline__ bool find_tile(const Params &p, int index, int rows, int &g, int &tile) {
   int before = 0;
   for (int base = 0; base < p.groups; base += kWave) {
     const int mine = base + lane_id();
     int n = 0;
     if (mine < p.groups) {
       const RowQueries t = group_queries(p, mine);
-      n = (int)(((int64_t)t.count * p.group + TILE - 1) / TILE);
+      n = (int)(((int64_t)t.count * p.group + rows - 1) / rows);
     }
     const int inc = wave_inclusive_scan(n);
     const uint64_t past = __ballot(before + inc > index);
@@ -251,6 +274,10 @@ __device__ __forceinline__ bool find_tile(const Params &p, int index, int &g, in
   }
   return false;
 }
+
+// The wide kernel (16-bit and fp8 keys): query rows of its tiles, and the launch over the own keys or the prefixes.
+int wide_tile_rows();
+int wide_attention(const Params &p, int kv_dtype, int head_dim, bool own, hipStream_t stream);
 
 }  // namespace attn
 }  // namespace ekv

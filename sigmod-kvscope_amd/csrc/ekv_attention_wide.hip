@@ -1,0 +1,421 @@
+// Attention of many query rows against one set of keys: prompt chunks over a prefix and their own keys, and
+// the queries of a whole group over its shared prefix.  The arithmetic bounds it, so the keys and values of
+// a step are staged through LDS once for all the waves of a workgroup, and both products run on the 16-bit
+// matrix instruction of 32 x 32 x 16.
+//
+// A wave has 32 query rows.  S^T = K Q^T leaves a lane one query's logits (keys 8a + 4h + b of each 32, in
+// lane half h), so the softmax of a row is in-lane work and one exchange between the halves.  The product
+// over keys is a sum, so its order is free as long as both operands agree: O^T = V^T P^T takes a lane's
+// weights where they lie, rounded to 16 bits, and the values through the transposing LDS read, four keys
+// of one dim a lane.  The weights' rounding (half a step of the type, relative) is of the size of the
+// output's own; their sum, the maxima and the outputs are float32.
+//
+// Measured, head dim 128: 3200 f16 query rows a KV head against prefixes of 32768 tokens 639 us (630 TFLOP/s, with
+// the own tokens and the join); bf16 prompt chunks of up to 4096 rows 293 us (630 TFLOP/s).  The narrow form of the
+// same calls, one wave for 16 query rows, took 2456 and 1247 us.
+#include "ekv_attention.hpp"
+
+namespace ekv {
+namespace attn {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Half {  // the type of the operands in LDS: fp8 widens to bf16 exactly
+  typedef __bf16 type;
+};
+template <>
+struct Half<F16> {
+  typedef _Float16 type;
+};
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __bf16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, _Float16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+
+// The shapes of one instance.  K and V of a step lie in LDS row by row, their 16-byte pieces (K) and
+// 64-byte pieces (V) permuted within the row by the row's number, so that the reads (K: 32 rows of one
+// piece; V: 4 rows of 64 bytes) meet every bank once.
+template <class T, int D>
+struct Wide {
+  static constexpr int kWaves = 4;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kKeys = D == 256 ? 32 : 64;  // of a step
+  static constexpr int kRow = D * 2;                // bytes of a row in LDS
+  static constexpr int kPieces = D * T::kBytes / 16;  // 16-byte pieces of a row in memory
+  static constexpr int kLoads = (kKeys * kPieces + kThreads - 1) / kThreads;  // of a thread, for K and for V
+  static constexpr int kLine = kRow < 256 ? 256 / kRow : 1;                   // rows in 256 bytes
+  static constexpr int kTile = kKeys * kRow;
+  __device__ static __forceinline__ int key_at(int row, int piece) {
+    return row * kRow + (piece ^ (row / kLine & (D / 8 - 1) & 15)) * 16;
+  }
+  __device__ static __forceinline__ int value_chunk(int row, int chunk) {
+    return row * kRow + (chunk ^ (row / kLine & (D / 32 - 1) & 3)) * 64;
+  }
+};
+
+// What a workgroup works on.  The keys are numbered along one axis, the prefix's first: [begin, end).
+struct Item {
+  const int32_t *ptable, *table;
+  int plen, begin, end;
+  int first, rows, m0;  // first token, query rows, the tile's first one
+  int head, slot;
+  int see;              // query token i sees keys below plen + see + i
+};
+
+// Out 0 and lse -inf for the tokens [from, to) of KV head `head`.
+template <class Q, int D>
+__device__ __forceinline__ void clear_tokens(const Params &p, int from, int to, int head, int threads) {
+  const int64_t n = (int64_t)max(to - from, 0) * p.group;
+  for (int64_t i = threadIdx.x; i < n * D; i += threads) {
+    const int64_t m = i / D;
+    const int token = from + (int)(m / p.group), q_head = head * p.group + (int)(m % p.group);
+    ((Q *)p.out)[token * p.o_st + q_head * p.o_sh + i % D] = (Q)0.f;
+    if (i % D == 0) p.lse[(int64_t)token * p.q_heads + q_head] = -INFINITY;
+  }
+}
+
+template <class T, int D>
+__device__ __forceinline__ bool own_item(const Params &p, int64_t index, Item &s) {
+  using W = Wide<T, D>;
+  s.head = (int)(index % p.kv_heads);
+  index /= p.kv_heads;
+  s.slot = (int)(index % p.s_own);
+  index /= p.s_own;
+  // the last tiles of a row see the most keys: they start first
+  const int row = (int)(index % p.rows), tile = p.tiles_own - 1 - (int)(index / p.rows);
+  const int len = row_length(p, row);
+  const RowQueries t = row_queries(p, row);
+  const int count = min(t.count, p.max_query);
+  if (p.direct && tile == 0) {  // tokens that no tile writes
+    typedef typename T::Query Q;
+    clear_tokens<Q, D>(p, t.first + count, t.first + t.count, s.head, W::kThreads);
+    if (row == 0) clear_tokens<Q, D>(p, 0, t.first, s.head, W::kThreads);
+    if (row == p.rows - 1) clear_tokens<Q, D>(p, t.first + t.count, p.tokens, s.head, W::kThreads);
+  }
+  s.first = t.first;
+  s.rows = count * p.group;
+  s.m0 = tile * p.tile_own;
+  if (s.m0 >= s.rows) return false;
+  s.table = p.table + (int64_t)row * p.table_stride;
+  s.ptable = nullptr;
+  s.plen = 0;
+  const int g = group_of(p, row);
+  if (g >= 0) {
+    s.ptable = p.ptable + (int64_t)g * p.ptable_stride;
+    s.plen = group_length(p, g);
+  }
+  s.see = len - t.count + 1;
+  const int last = (min(s.m0 + p.tile_own, s.rows) - 1) / p.group;
+  const int64_t begin = (int64_t)s.slot * p.chunk_own;
+  s.end = (int)min(begin + p.chunk_own, (int64_t)s.plen + max(0, min(len, s.see + last)));
+  s.begin = (int)min(begin, (int64_t)INT32_MAX);
+  return s.begin < s.end || p.direct;
+}
+
+template <class T, int D>
+__device__ __forceinline__ bool prefix_item(const Params &p, int64_t index, Item &s) {
+  s.head = (int)(index % p.kv_heads);
+  index /= p.kv_heads;
+  const int chunk = (int)(index % p.s_pre);
+  int g, tile;
+  if (!find_tile(p, (int)(index / p.s_pre), p.tile_pre, g, tile)) return false;
+  const RowQueries t = group_queries(p, g);
+  s.ptable = p.ptable + (int64_t)g * p.ptable_stride;
+  s.table = nullptr;
+  s.plen = group_length(p, g);
+  s.first = t.first;
+  s.rows = t.count * p.group;
+  s.m0 = tile * p.tile_pre;
+  s.see = 0;
+  s.slot = p.s_own + chunk;
+  const int64_t begin = (int64_t)chunk * p.chunk_pre;
+  s.end = (int)min(begin + p.chunk_pre, (int64_t)s.plen);
+  s.begin = (int)min(begin, (int64_t)INT32_MAX);
+  return s.begin < s.end;
+}
+
+// One step's keys and values on their way from memory to LDS.
+template <class T, int D>
+struct Stage {
+  using W = Wide<T, D>;
+  int page;        // of this lane's key of the step after the next load
+  u32x4 k[W::kLoads], v[W::kLoads];
+  uint64_t ok;     // the keys of the loaded step that are there
+
+  // the page of key `base + lane` (one load a lane, a step ahead of the rows')
+  __device__ __forceinline__ void look(const Params &p, const Item &s, int base) {
+    const int at = base + lane_id() % W::kKeys;
+    page = -1;
+    if (at < s.end) {
+      const bool shared = at < s.plen;
+      page = (shared ? s.ptable : s.table)[page_of(p, shared ? at : at - s.plen)];
+    }
+  }
+  __device__ __forceinline__ void load(const Params &p, const Item &s, int base) {
+    const int at = base + lane_id() % W::kKeys;
+    const int pos = at < s.plen ? at : at - s.plen;
+    const bool good = at < s.end && (uint32_t)page < (uint64_t)p.blocks;
+    ok = __ballot(good);
+    const int in_page = good ? pos - page_of(p, pos) * p.block_size : 0;
+    const int64_t off = ((int64_t)(good ? page : 0) * p.st_block + (int64_t)in_page * p.st_pos +
+                         (int64_t)s.head * p.st_head) * T::kBytes;
+    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
+#pragma unroll
+    for (int i = 0; i < W::kLoads; ++i) {
+      const int piece = threadIdx.x + i * W::kThreads;
+      if (W::kKeys * W::kPieces % W::kThreads != 0 && piece >= W::kKeys * W::kPieces) break;
+      const int row = piece / W::kPieces, col = piece % W::kPieces;
+      const int64_t at_row = (int64_t)(((uint64_t)(uint32_t)__shfl(hi, row) << 32) | (uint32_t)__shfl(lo, row)) + col * 16;
+      k[i] = *as_global((const u32x4 *)(p.k + at_row));
+      v[i] = *as_global((const u32x4 *)(p.v + at_row));
+    }
+  }
+  // K at `keys`, V behind it; the values of keys that are not there as 0 (0 * NaN is no zero)
+  __device__ __forceinline__ void store(char *keys) {
+    char *values = keys + W::kTile;
+#pragma unroll
+    for (int i = 0; i < W::kLoads; ++i) {
+      const int piece = threadIdx.x + i * W::kThreads;
+      if (W::kKeys * W::kPieces % W::kThreads != 0 && piece >= W::kKeys * W::kPieces) break;
+      const int row = piece / W::kPieces, col = piece % W::kPieces;
+      u32x4 x = v[i];
+      if (~ok != 0 && !(ok >> row & 1)) x = u32x4{0, 0, 0, 0};
+      if constexpr (T::kBytes == 1) {
+        *(u32x4 *)(keys + W::key_at(row, 2 * col)) = __builtin_bit_cast(u32x4, widen(k[i][0], k[i][1]));
+        *(u32x4 *)(keys + W::key_at(row, 2 * col + 1)) = __builtin_bit_cast(u32x4, widen(k[i][2], k[i][3]));
+        char *to = values + W::value_chunk(row, col / 2) + col % 2 * 32;
+        *(u32x4 *)to = __builtin_bit_cast(u32x4, widen(x[0], x[1]));
+        *(u32x4 *)(to + 16) = __builtin_bit_cast(u32x4, widen(x[2], x[3]));
+      } else {
+        *(u32x4 *)(keys + W::key_at(row, col)) = k[i];
+        *(u32x4 *)(values + W::value_chunk(row, col / 4) + col % 4 * 16) = x;
+      }
+    }
+  }
+};
+
+// The other lane half's value.
+__device__ __forceinline__ float other_half_max(float v) {
+  float a, b;
+  row_swap32(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  float a, b;
+  row_swap32(v, a, b);
+  return a + b;
+}
+
+// A running maximum is kept while no row of the wave passes it by more than this (powers of two): weights
+// then reach 2^8, well inside either type, and most steps leave the outputs unscaled.
+constexpr float kSlack = 8.f;
+
+template <class T, int D>
+__device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char *lds) {
+  using W = Wide<T, D>;
+  typedef typename Half<T>::type H;
+  constexpr int KT = W::kKeys / 32, DT = D / 32;
+  const int lane = lane_id(), half = lane / 32, n = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int w0 = s.m0 + wave * 32;  // the wave's first query row
+  const int m = w0 + n;
+  const bool live = m < s.rows;
+  const int i_q = live ? m / p.group : 0;
+  const int token = s.first + i_q, q_head = s.head * p.group + (live ? m - i_q * p.group : 0);
+  const bool any = w0 < s.rows;
+  const int limit = live ? min(s.end, s.plen + max(0, s.see + i_q)) : 0;  // this lane's query sees keys below it
+  const int every = min(s.end, s.plen + max(0, s.see + w0 / p.group));    // and every query of the wave keys below this
+  const int last_row = min(w0 + 31, s.rows - 1);
+  const int most = any ? min(s.end, s.plen + max(0, s.see + last_row / p.group)) : 0;  // none sees keys from here on
+
+  // a negative scale turns the query's sign; the smallest one keeps a masked logit at -inf where scale is 0
+  const float scale2 = fmaxf(fabsf(p.scale2), 0x1p-126f);
+  const uint32_t flip = p.scale2 < 0.f ? 0x80008000u : 0u;
+  u32x4 q[D / 16];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    q[c] = u32x4{0, 0, 0, 0};
+    if (live) {
+      q[c] = *as_global((const u32x4 *)(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh + c * 16 + half * 8) * 2));
+      q[c] ^= flip;
+    }
+  }
+
+  // LDS offsets of this lane's reads
+  int key_off[D / 16], value_off[DT];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) key_off[c] = W::key_at(n, 2 * c + half);
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+    value_off[d] = W::kTile + W::value_chunk(4 * half + lane % 16 / 4, d) + lane / 16 % 2 * 32 + lane % 4 * 8;
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  float top = -INFINITY, sum = 0.f;
+
+  Stage<T, D> stage;
+  uint64_t ok = 0;
+  if (s.begin < s.end) {
+    stage.look(p, s, s.begin);
+    stage.load(p, s, s.begin);
+    stage.look(p, s, s.begin + W::kKeys);
+    ok = stage.ok;
+    stage.store(lds);
+  }
+
+  auto step = [&](int base, char *buffer, char *next) {
+    lds_barrier();
+    const bool more = base + W::kKeys < s.end;
+    if (more) {
+      stage.load(p, s, base + W::kKeys);
+      stage.look(p, s, base + 2 * W::kKeys);
+    }
+    if (base < most) {
+      f32x16 x[KT];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) x[k] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          x[k] = mfma32(*(const u32x4 *)(buffer + key_off[c] + k * 32 * W::kRow), q[c], x[k], H{});
+      if (base + W::kKeys > every || ~ok != 0) {
+        const uint64_t mine = ok >> (4 * half);
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * k + 8 * (i / 4) + i % 4;
+            if (!(mine >> at & 1) || base + at + 4 * half >= limit) x[k][i] = -INFINITY;
+          }
+      }
+      float high = x[0][0];
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) high = fmaxf(high, x[k][i]);
+      high = other_half_max(high) * scale2;
+      if (!__all(high <= top + kSlack)) {
+        const float peak = fmaxf(top, high);
+        const float shrink = __builtin_amdgcn_exp2f(top - (peak == -INFINITY ? 0.f : peak));
+        sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= shrink;
+        top = peak;
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], scale2, -ref));
+          sum += x[k][i];
+        }
+#pragma unroll
+      for (int t = 0; t < W::kKeys / 16; ++t) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack2(x[t / 2][8 * (t % 2) + 2 * i], x[t / 2][8 * (t % 2) + 2 * i + 1], H{});
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          typedef __attribute__((address_space(3))) s16x4 *Lds;
+          const char *from = buffer + value_off[d] + t * 16 * W::kRow;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 8 * W::kRow));
+          const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+          acc[d] = mfma32(u32x4{a[0], a[1], b[0], b[1]}, w, acc[d], H{});
+        }
+      }
+    }
+    if (more) {
+      ok = stage.ok;
+      stage.store(next);
+    }
+  };
+  char *other = lds + 2 * W::kTile;
+  for (int base = s.begin; base < s.end;) {
+    step(base, lds, other);
+    base += W::kKeys;
+    if (base >= s.end) break;
+    step(base, other, lds);
+    base += W::kKeys;
+  }
+
+  sum = other_half_sum(sum);
+  if (!live) return;
+  if (p.direct) {
+    typedef typename T::Query Q;
+    const bool none = sum == 0.f;
+    const float inv = none ? 0.f : p.v_scale / sum;
+    char *o = p.out + ((int64_t)token * p.o_st + (int64_t)q_head * p.o_sh + 4 * half) * 2;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        Q *dst = (Q *)(o + (d * 32 + a * 8) * 2);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) dst[b] = (Q)(none ? 0.f : acc[d][4 * a + b] * inv);
+      }
+    if (half == 0) p.lse[(int64_t)token * p.q_heads + q_head] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    return;
+  }
+  const int64_t at = ((int64_t)s.slot * p.tokens + token) * p.q_heads + q_head;
+  if (half == 0) p.part_ml[at] = make_float2(top, sum);
+  float *o = p.part_o + at * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      *(f32x4 *)(o + d * 32 + a * 8) = f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+}
+
+template <class T, int D, bool OWN>
+__global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wide_kernel(const Params p) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * Wide<T, D>::kTile];
+  Item s;
+  if (!(OWN ? own_item<T, D>(p, blockIdx.x, s) : prefix_item<T, D>(p, blockIdx.x, s))) return;
+  attend_wide<T, D>(p, s, lds);
+}
+
+template <class T, int D>
+int launch_wide(const Params &p, bool own, hipStream_t stream) {
+  const unsigned grid = (unsigned)(own ? p.items_own : p.items_pre);
+  if (grid == 0) return EKV_OK;
+  if (own) hipLaunchKernelGGL((wide_kernel<T, D, true>), dim3(grid), dim3(Wide<T, D>::kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((wide_kernel<T, D, false>), dim3(grid), dim3(Wide<T, D>::kThreads), 0, stream, p);
+  return check_hip(hipGetLastError(), "ekv_prefix_attention wide launch");
+}
+
+template <class T>
+int wide_dim(const Params &p, int head_dim, bool own, hipStream_t stream) {
+  switch (head_dim) {
+    case 32: return launch_wide<T, 32>(p, own, stream);
+    case 64: return launch_wide<T, 64>(p, own, stream);
+    case 128: return launch_wide<T, 128>(p, own, stream);
+    default: return launch_wide<T, 256>(p, own, stream);
+  }
+}
+
+int wide_tile_rows() { return Wide<BF16, 128>::kWaves * 32; }
+
+int wide_attention(const Params &p, int kv_dtype, int head_dim, bool own, hipStream_t stream) {
+  switch (kv_dtype) {
+    case EKV_F16: return wide_dim<F16>(p, head_dim, own, stream);
+    case EKV_BF16: return wide_dim<BF16>(p, head_dim, own, stream);
+    default: return wide_dim<FP8>(p, head_dim, own, stream);
+  }
+}
+
+}  // namespace attn
+}  // namespace ekv
