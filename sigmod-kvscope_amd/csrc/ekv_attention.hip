@@ -12,22 +12,21 @@
 // A prefix is one set of items for all the queries of its group: its keys and values are read once per
 // tile of them and not once per row.
 #include "ekv_attention.hpp"
+#include <stdlib.h>
 
 namespace ekv {
 namespace attn {
 
-// What one wave works on: keys [begin, end) behind `table`, query rows [m0, M) of the tokens from `first`.
-struct Segment {
-  const int32_t *table;
-  int begin, end;
+// What one wave works on.
+struct Segment : Range {
   int first, rows;  // first token, query rows (tokens * group)
-  int m0;
-  int head, slot;
-  int see;  // query token i sees keys below see + i (own pages), or INT_MAX / 2 (a prefix)
+  int m0;           // the tile's first query row
+  int row, slot;    // the batch row (own keys), the slot of the partial results
+  int see;          // query token i sees keys below see + i (own pages), or INT_MAX / 2 (a prefix)
 };
 
 template <int TILE>
-__device__ __forceinline__ bool own_segment(const Params &p, int64_t item, Segment &s) {
+__device__ __forceinline__ bool own_segment(const Params &p, uint32_t item, Segment &s) {
   s.head = (int)(item % p.kv_heads);
   item /= p.kv_heads;
   const int tile = (int)(item % p.tiles_own);
@@ -37,6 +36,9 @@ __device__ __forceinline__ bool own_segment(const Params &p, int64_t item, Segme
   const int len = row_length(p, row);
   const RowQueries t = row_queries(p, row);
   s.table = p.table + (int64_t)row * p.table_stride;
+  s.ptable = nullptr;
+  s.plen = 0;
+  s.row = row;
   s.first = t.first;
   s.rows = min(t.count, p.max_query) * p.group;
   s.m0 = tile * TILE;
@@ -51,7 +53,7 @@ __device__ __forceinline__ bool own_segment(const Params &p, int64_t item, Segme
 }
 
 template <int TILE>
-__device__ __forceinline__ bool prefix_segment(const Params &p, int64_t item, Segment &s) {
+__device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, Segment &s) {
   s.head = (int)(item % p.kv_heads);
   item /= p.kv_heads;
   const int chunk = (int)(item % p.s_pre);
@@ -59,6 +61,9 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, int64_t item, Se
   if (!find_tile(p, (int)(item / p.s_pre), TILE, g, tile)) return false;
   const RowQueries t = group_queries(p, g);
   s.table = p.ptable + (int64_t)g * p.ptable_stride;
+  s.ptable = nullptr;
+  s.plen = 0;
+  s.row = -1;
   s.first = t.first;
   s.rows = t.count * p.group;
   s.m0 = tile * TILE;
@@ -70,159 +75,141 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, int64_t item, Se
   return s.begin < s.end;
 }
 
-// The keys and values of 16 consecutive slots, one lane's part: key l % 16, and the values of the four
-// keys 4 * (l / 16) + i, whose dims the 16 lanes of a lane group share out.
+// The shapes of one instance: one wave's step of about 8 KB (fp8) or 16 KB of keys and values on their way while
+// the step before is worked on, so that the 8 waves of a compute unit have 64 to 128 KB in flight.
 template <class T, int D>
-struct Tile {
-  static constexpr int kLaneDims = D / 16;  // of one value row
-  static constexpr int kPieceDims = kLaneDims * T::kBytes > 16 ? 16 / T::kBytes : kLaneDims;
-  static constexpr int kValuePieces = kLaneDims / kPieceDims;
-  static constexpr int kPieceBytes = kPieceDims * T::kBytes;
-  static constexpr int kPieceWords = kPieceBytes < 4 ? 1 : kPieceBytes / 4;
-  KeyRow<T, D> key;
-  uint32_t value[4][kValuePieces * kPieceWords];
-  uint32_t ok;  // bit i: key 4 * (l / 16) + i has a page in the cache
-
-  // WHOLE: the 16 slots lie in one page (block sizes that are multiples of 16), so its id is uniform.
-  template <bool WHOLE>
-  __device__ __forceinline__ void load(const Params &p, const Segment &s, int base, bool values) {
-    const int lane = lane_id(), g = lane / 16, n = lane % 16;
-    const int64_t head = (int64_t)s.head * p.st_head;
-    if constexpr (WHOLE) {
-      const int index = page_of(p, base);
-      int page = s.table[index];
-      const bool good = (uint32_t)page < (uint64_t)p.blocks;
-      ok = good ? 15u : 0u;
-      if (!good) page = 0;
-      const int at = base - index * p.block_size;
-      const int64_t origin = ((int64_t)page * p.st_block + (int64_t)at * p.st_pos + head) * T::kBytes;
-      key.load(p.k + origin + (int64_t)n * p.st_pos * T::kBytes, g);
-      if (values) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          load_value(p.v + origin + (int64_t)(4 * g + i) * p.st_pos * T::kBytes, n, i);
-      }
-    } else {
-      ok = 0;
-      {
-        const int pos = min(base + n, s.end - 1), index = page_of(p, pos);
-        int page = s.table[index];
-        if ((uint32_t)page >= (uint64_t)p.blocks) page = 0;
-        key.load(p.k + ((int64_t)page * p.st_block + (int64_t)(pos - index * p.block_size) * p.st_pos + head) *
-                           T::kBytes, g);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pos = min(base + 4 * g + i, s.end - 1), index = page_of(p, pos);
-        int page = s.table[index];
-        const bool good = (uint32_t)page < (uint64_t)p.blocks;
-        ok |= good ? 1u << i : 0u;
-        if (!good) page = 0;
-        if (values)
-          load_value(p.v + ((int64_t)page * p.st_block + (int64_t)(pos - index * p.block_size) * p.st_pos + head) *
-                               T::kBytes, n, i);
-      }
-    }
-  }
-  __device__ __forceinline__ void load_value(const char *row, int n, int i) {
-#pragma unroll
-    for (int c = 0; c < kValuePieces; ++c)
-      load_bytes<kPieceBytes>(row + (c * 16 + n) * kPieceBytes, value[i] + c * kPieceWords);
-  }
+struct Narrow {
+  static constexpr int kRow = Lds<T, D>::kRow;
+  static constexpr int kKeys = std::is_same<T, F32>::value ? (D <= 64 ? 32 : 16) : (D <= 64 ? 64 : 32);
+  typedef Stage<T, D, kKeys, kWave> Step;
+  static constexpr int kBytes = 2 * Step::kTile;  // LDS of a wave
+  static constexpr int kWaves = kBytes > 16384 ? 2 : 4;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kPieceDims = D >= 64 ? 4 : 2;  // float32: dims of a value row that a lane reads at once
 };
 
-// One wave per item.  S^T = K Q^T on the matrix cores leaves each lane the logits of four keys of one query
-// row.  O^T = V^T P^T is summed by the float32 matrix instruction of four keys: its P operand is what the
-// lane already holds (key 4g + i for step i, the weights never rounded), and its V operand one element of
-// the lane's own 16 bytes of a value row, so neither product moves data between lanes or through LDS.  The
-// float32 instruction has a sixteenth of the 16-bit one's rate, which for 16 query rows still outruns HBM.
-// Loads run one step (KT tiles) ahead in registers.
-template <class T, int D, bool WHOLE, int KT>
-__device__ __forceinline__ void attend(const Params &p, const Segment &s) {
-  using Tl = Tile<T, D>;
-  constexpr int E = sizeof(typename T::Query);
+// One wave per item.  S^T = K Q^T on the matrix cores leaves each lane the logits of four keys (4g + i of each 16,
+// in lane group g) of one query row.  O^T = V^T P^T takes as its P operand what the lane already holds, its weights
+// rounded to 16 bits (half a step of the type, relative: the size of the output's own rounding; float32 caches keep
+// float32 weights), and as its V operand the same keys' values by the transposing LDS read, so no weight moves
+// between lanes.  The LDS is the wave's own: nothing waits for another wave.
+template <class T, int D>
+__device__ __forceinline__ void attend(const Params &p, const Segment &s, char *lds) {
+  using N = Narrow<T, D>;
+  using L = Lds<T, D>;
+  constexpr int E = sizeof(typename T::Query), KT = N::kKeys / 16, QP = N::kRow / 64;
   const int lane = lane_id(), g = lane / 16, n = lane % 16;
   const int m = s.m0 + n;
   const bool live = m < s.rows;
   const int i_q = live ? m / p.group : 0;
   const int token = s.first + i_q, q_head = s.head * p.group + (live ? m - i_q * p.group : 0);
-  QueryRow<T, D> q;
-  q.load(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E, g, live);
-  const int limit = live ? min(s.end, s.see + i_q) : 0;   // this lane's query sees keys below it
-  const int every = min(s.end, s.see + s.m0 / p.group);    // and every query of the tile keys below this
-  const int last = s.begin + ((s.end - 1 - s.begin) & ~15);  // the last tile that starts before the end
+  const int limit = live ? min(s.end, s.see + i_q) : 0;  // this lane's query sees keys below it
+  const int every = min(s.end, s.see + s.m0 / p.group);  // and every query of the tile keys below this
+
+  typename N::Step stage;
+  stage.look(p, s, s.begin);
+  u32x4 q[QP];
+#pragma unroll
+  for (int c = 0; c < QP; ++c) {
+    q[c] = u32x4{0, 0, 0, 0};
+    if (live)
+      q[c] = *as_global((const u32x4 *)(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E + (4 * c + g) * 16));
+  }
+  stage.load(p, s, s.begin);
+  stage.look(p, s, s.begin + N::kKeys);
+
+  int key_off[QP];
+#pragma unroll
+  for (int c = 0; c < QP; ++c) key_off[c] = L::key_at(n, 4 * c + g);
+  const char *values = lds + N::Step::kTile;
+  float *logits = nullptr;  // of this lane's query row
+  if (p.logits != nullptr && s.row >= 0 && live)
+    logits = p.logits + (((int64_t)s.row * p.kv_heads + s.head) * p.logit_rows + m) * p.logit_stride;
 
   f32x4 acc[D / 16];
 #pragma unroll
-  for (int a = 0; a < D / 16; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < D / 16; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, sum = 0.f;
 
-  auto step = [&](Tl *t, int base) {
-    float x[KT][4];
-    float high = -INFINITY;
+  for (int base = s.begin; base < s.end; base += N::kKeys) {
+    const uint64_t ok = stage.ok;
+    stage.store(lds);
+    asm volatile("" ::: "memory");  // the lanes of the wave read what others wrote, in order
+    if (base + N::kKeys < s.end) {
+      stage.load(p, s, base + N::kKeys);
+      stage.look(p, s, base + 2 * N::kKeys);
+    }
+    f32x4 x[KT];
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
-      const f32x4 c = dot_tile<T, D>(t[k].key, q);
+      x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[k][i] = c[i] * p.scale2;
-      const int tile = base + 16 * k;
-      if (!__all(tile + 16 <= every && t[k].ok == 15u)) {
+      for (int c = 0; c < QP; ++c) x[k] = dot_piece<T>(*(const u32x4 *)(lds + key_off[c] + k * 16 * N::kRow), q[c], x[k]);
+      x[k] *= p.scale2;
+    }
+    if (base + N::kKeys > every || ~ok != 0) {
+      const uint64_t mine = ok >> (4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pos = tile + 4 * g + i;
-          const bool there = (t[k].ok >> i & 1u) != 0;
-          x[k][i] = there && pos < limit ? x[k][i] : -INFINITY;
-          if (!there || pos >= s.end) {  // what lies there may be anything: 0 * NaN is no zero
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-            for (int w = 0; w < Tl::kValuePieces * Tl::kPieceWords; ++w) t[k].value[i][w] = 0;
-          }
-        }
-      }
+        for (int i = 0; i < 4; ++i)
+          if (!(mine >> (16 * k + i) & 1) || base + 16 * k + 4 * g + i >= limit) x[k][i] = -INFINITY;
+    }
+    if (logits != nullptr) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        if (base + 16 * k + 4 * g < s.end) *(f32x4 *)(logits + base + 16 * k + 4 * g) = x[k];
+    }
+    float high = x[0][0];
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) high = fmaxf(high, x[k][i]);
-    }
     const float peak = fmaxf(top, rows_max(high));
     const float ref = peak == -INFINITY ? 0.f : peak;
-    const float shrink = __builtin_amdgcn_exp2f(top - ref);
     if (!__all(top == peak)) {
+      const float shrink = __builtin_amdgcn_exp2f(top - ref);
       sum *= shrink;
 #pragma unroll
-      for (int a = 0; a < D / 16; ++a) acc[a] *= shrink;
+      for (int d = 0; d < D / 16; ++d) acc[d] *= shrink;
     }
     top = peak;
 #pragma unroll
-    for (int k = 0; k < KT; ++k) {
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float w = __builtin_amdgcn_exp2f(x[k][i] - ref);
-        sum += w;
+        x[k][i] = __builtin_amdgcn_exp2f(x[k][i] - ref);
+        sum += x[k][i];
+      }
+    if constexpr (std::is_same<T, F32>::value) {
+      constexpr int PD = N::kPieceDims;
+      typedef float Piece __attribute__((ext_vector_type(PD)));
 #pragma unroll
-        for (int c = 0; c < Tl::kValuePieces; ++c) {
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int j = 0; j < Tl::kPieceDims; ++j)
-            acc[c * Tl::kPieceDims + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                element<T>(t[k].value[i] + c * Tl::kPieceWords, j), w, acc[c * Tl::kPieceDims + j], 0, 0, 0);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < D / 16 / PD; ++c) {
+            const Piece v = *(const Piece *)(values + L::value_at(16 * k + 4 * g + i, (c * 16 + n) * PD * 4));
+#pragma unroll
+            for (int j = 0; j < PD; ++j)
+              acc[c * PD + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], x[k][i], acc[c * PD + j], 0, 0, 0);
+          }
+    } else {
+      typedef typename T::Half H;
+#pragma unroll
+      for (int k = 0; k < KT; k += 2) {
+        const u32x4 w = {pack2(x[k][0], x[k][1], H{}), pack2(x[k][2], x[k][3], H{}), pack2(x[k + 1][0], x[k + 1][1], H{}),
+                         pack2(x[k + 1][2], x[k + 1][3], H{})};
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          const char *from = values + L::value_at(4 * g + n / 4, d * 32 + n % 4 * 8) + k * 16 * N::kRow;
+          const u32x2 v = read_transposed(from), u = read_transposed(from + 16 * N::kRow);
+          acc[d] = mfma16(u32x4{v[0], v[1], u[0], u[1]}, w, acc[d], H{});
         }
       }
     }
-  };
-  auto fetch = [&](Tl *t, int base) {
-#pragma unroll
-    for (int k = 0; k < KT; ++k) t[k].template load<WHOLE>(p, s, min(base + 16 * k, last), true);
-  };
-
-  Tl a[KT], b[KT];
-  constexpr int kStep = 16 * KT;
-  fetch(a, s.begin);
-  for (int base = s.begin;;) {
-    fetch(b, base + kStep);
-    step(a, base);
-    base += kStep;
-    if (base >= s.end) break;
-    fetch(a, base + kStep);
-    step(b, base);
-    base += kStep;
-    if (base >= s.end) break;
+    asm volatile("" ::: "memory");  // the next step overwrites what this one read
   }
 
   sum = rows_sum(sum);
@@ -230,27 +217,28 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s) {
   const int64_t at = ((int64_t)s.slot * p.tokens + token) * p.q_heads + q_head;
   if (g == 0) p.part_ml[at] = make_float2(top, sum);
   float *o = p.part_o + at * D;
+  if constexpr (std::is_same<T, F32>::value) {
+    constexpr int PD = N::kPieceDims;
 #pragma unroll
-  for (int c = 0; c < Tl::kValuePieces; ++c) {
+    for (int c = 0; c < D / 16 / PD; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float *dst = o + c * 16 * Tl::kPieceDims + (4 * g + e) * Tl::kPieceDims;
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int j = 0; j < Tl::kPieceDims; ++j) dst[j] = acc[c * Tl::kPieceDims + j][e];
-    }
+        for (int j = 0; j < PD; ++j) o[c * 16 * PD + (4 * g + e) * PD + j] = acc[c * PD + j][e];
+  } else {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) *(f32x4 *)(o + 16 * d + 4 * g) = acc[d];
   }
 }
 
 constexpr int kThreads = 256;
 
-// tiles of a step: about 8 KB of keys and values in flight per wave
 template <class T, int D>
-constexpr int kTiles = D * T::kBytes <= 128 ? 4 : D * T::kBytes <= 256 ? 2 : 1;
-
-template <class T, int D, bool WHOLE>
-__global__ __launch_bounds__(kThreads, D *T::kBytes <= 512 ? 2 : 1) void narrow_kernel(const Params p) {
+__global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void narrow_kernel(const Params p) {
+  using N = Narrow<T, D>;
+  __shared__ __attribute__((aligned(16))) char lds[N::kWaves * N::kBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / kWave) + wave;
+  const int64_t item = (int64_t)blockIdx.x * N::kWaves + wave;
   const int64_t shared = p.wide_pre ? 0 : p.items_pre;  // items of the prefixes come first
   Segment s;
   if (item < shared) {
@@ -259,7 +247,7 @@ __global__ __launch_bounds__(kThreads, D *T::kBytes <= 512 ? 2 : 1) void narrow_
     if (item - shared >= p.items_own) return;
     if (!own_segment<kRowsPerTile>(p, item - shared, s)) return;
   }
-  attend<T, D, WHOLE, kTiles<T, D>>(p, s);
+  attend<T, D>(p, s, lds + wave * N::kBytes);
 }
 
 // -- joining the chunks ---------------------------------------------------------------------------------
@@ -353,61 +341,108 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
 
 // -- the running weights ------------------------------------------------------------------------------
 
-constexpr int kWeighKeys = 64;  // keys of one wave
+// The logits were kept: a thread per four keys of a (row, KV head).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void fold_kernel(const Params p, int pieces) {
+  const uint32_t block = blockIdx.x;
+  const int head = (int)(block % p.kv_heads), row = (int)(block / p.kv_heads / pieces);
+  const int key = ((int)(block / p.kv_heads % pieces) * THREADS + threadIdx.x) * 4;
+  const int len = row_length(p, row);
+  if (key >= len) return;
+  const RowQueries t = row_queries(p, row);
+  const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
+  const float *logits = p.logits + ((int64_t)row * p.kv_heads + head) * p.logit_rows * p.logit_stride + key;
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int m = 0; m < rows; ++m) {
+    const int i_q = m / p.group;
+    const float lse = p.lse[(int64_t)(t.first + i_q) * p.q_heads + head * p.group + (m - i_q * p.group)];
+    if (lse == -INFINITY || key >= see + i_q) continue;  // it sees none of them (nor wrote their logits)
+    const f32x4 x = *(const f32x4 *)(logits + (int64_t)m * p.logit_stride);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total[i] += __builtin_amdgcn_exp2f(x[i] - lse * kLog2e);  // unseen ones are -inf
+  }
+  float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (key + i < len) out[key + i] = p.decay * out[key + i] + total[i];
+}
 
-// One wave per (row, KV head, 64 keys): the logits of every query row against them again, their weights
+// The logits again: one wave per (row, KV head, 64 keys), the logits of every query row against them, their weights
 // exp(s - lse) summed over the query rows in one order, and one addition to each key's running score.
-template <class T, int D, bool WHOLE>
+constexpr int kWeighKeys = 64;
+
+template <class T, int D>
 __global__ __launch_bounds__(kThreads) void weigh_kernel(const Params p, int pieces) {
-  constexpr int E = sizeof(typename T::Query);
-  constexpr int KT = kWeighKeys / 16;
+  constexpr int E = sizeof(typename T::Query), KT = kWeighKeys / 16, QP = Lds<T, D>::kRow / 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int64_t item = (int64_t)blockIdx.x * (kThreads / kWave) + wave;
   if (item >= (int64_t)p.rows * pieces * p.kv_heads) return;
-  Segment s;
-  s.head = (int)(item % p.kv_heads);
+  const int head = (int)(item % p.kv_heads);
   item /= p.kv_heads;
-  const int row = (int)(item / pieces);
-  s.begin = (int)(item % pieces) * kWeighKeys;
-  const int len = row_length(p, row);
-  s.end = min(s.begin + kWeighKeys, len);
-  if (s.begin >= s.end) return;
-  s.table = p.table + (int64_t)row * p.table_stride;
+  const int row = (int)(item / pieces), begin = (int)(item % pieces) * kWeighKeys;
+  const int len = row_length(p, row), end = min(begin + kWeighKeys, len);
+  if (begin >= end) return;
+  const int32_t *table = p.table + (int64_t)row * p.table_stride;
   const RowQueries t = row_queries(p, row);
   const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
   const int lane = lane_id(), g = lane / 16, n = lane % 16;
-  const int last = s.begin + ((s.end - 1 - s.begin) & ~15);
-  Tile<T, D> tile[KT];
+  const int mine = min(begin + lane, end - 1);
+  const int page_mine = table[page_of(p, mine)];
+  const uint64_t ok = __ballot((uint32_t)page_mine < (uint64_t)p.blocks) >> (4 * g);
+  // the key rows' pieces 4c + g, read where they lie: 64 bytes of 16 rows a load
+  u32x4 key[KT][QP];
 #pragma unroll
-  for (int k = 0; k < KT; ++k) tile[k].template load<WHOLE>(p, s, min(s.begin + 16 * k, last), false);
+  for (int k = 0; k < KT; ++k) {
+    const int pos = min(begin + 16 * k + n, end - 1);
+    int page = __shfl(page_mine, 16 * k + n);
+    if ((uint32_t)page >= (uint64_t)p.blocks) page = 0;
+    const char *from = p.k + ((int64_t)page * p.st_block + (int64_t)(pos - page_of(p, pos) * p.block_size) * p.st_pos +
+                              (int64_t)head * p.st_head) * T::kBytes;
+#pragma unroll
+    for (int c = 0; c < QP; ++c) {
+      if constexpr (T::kBytes == 1) {
+        const u32x2 x = *as_global((const u32x2 *)(from + (4 * c + g) * 8));
+        key[k][c] = widen(x[0], x[1]);
+      } else {
+        key[k][c] = *as_global((const u32x4 *)(from + (4 * c + g) * 16));
+      }
+    }
+  }
   float total[KT][4];
 #pragma unroll
   for (int k = 0; k < KT; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) total[k][i] = 0.f;
   // queries before the first key see none of them
-  const int m_first = max(0, (s.begin - see + 1)) * p.group / kRowsPerTile * kRowsPerTile;
-  for (int m0 = m_first; m0 < rows; m0 += kRowsPerTile) {
+  const int64_t before = (int64_t)max(0, begin - see + 1) * p.group;
+  for (int m0 = (int)min(before, (int64_t)rows) / kRowsPerTile * kRowsPerTile; m0 < rows; m0 += kRowsPerTile) {
     const int m = m0 + n;
     const bool live = m < rows;
     const int i_q = live ? m / p.group : 0;
-    const int token = t.first + i_q, q_head = s.head * p.group + (live ? m - i_q * p.group : 0);
-    QueryRow<T, D> q;
-    q.load(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E, g, live);
+    const int token = t.first + i_q, q_head = head * p.group + (live ? m - i_q * p.group : 0);
+    u32x4 q[QP];
+#pragma unroll
+    for (int c = 0; c < QP; ++c) {
+      q[c] = u32x4{0, 0, 0, 0};
+      if (live)
+        q[c] = *as_global((const u32x4 *)(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E + (4 * c + g) * 16));
+    }
     const float lse = live ? p.lse[(int64_t)token * p.q_heads + q_head] : -INFINITY;
     const float lse2 = lse * kLog2e;
-    const int limit = lse == -INFINITY ? 0 : min(s.end, see + i_q);
+    const int limit = lse == -INFINITY ? 0 : min(end, see + i_q);
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
-      const f32x4 c = dot_tile<T, D>(tile[k].key, q);
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < QP; ++c) x = dot_piece<T>(key[k][c], q[c], x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool sees = (tile[k].ok >> i & 1u) != 0 && s.begin + 16 * k + 4 * g + i < limit;
-        total[k][i] += sees ? __builtin_amdgcn_exp2f(c[i] * p.scale2 - lse2) : 0.f;
+        const bool sees = (ok >> (16 * k + i) & 1) != 0 && begin + 16 * k + 4 * g + i < limit;
+        total[k][i] += sees ? __builtin_amdgcn_exp2f(x[i] * p.scale2 - lse2) : 0.f;
       }
     }
   }
-  float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)s.head * p.sc_head;
+  float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
 #pragma unroll
@@ -415,8 +450,8 @@ __global__ __launch_bounds__(kThreads) void weigh_kernel(const Params p, int pie
       float v = total[k][i];
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) v += shfl_xor(v, d);
-      const int pos = s.begin + 16 * k + 4 * g + i;
-      if (n == i && pos < s.end) out[pos] = p.decay * out[pos] + v;
+      const int pos = begin + 16 * k + 4 * g + i;
+      if (n == i && pos < end) out[pos] = p.decay * out[pos] + v;
     }
   }
 }
@@ -437,6 +472,7 @@ void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim,
   n = n > kMaxSlots ? kMaxSlots : n < 1 ? 1 : n;
   chunk = (int)(ceil_div(ceil_div(keys, n), 64) * 64);
   if (chunk < 64) chunk = 64;
+  if (getenv("EKV_CHUNK")) chunk = atoi(getenv("EKV_CHUNK"));
   slots = (int)ceil_div(keys, chunk);
   if (slots < 1) slots = 1;
 }
@@ -482,26 +518,37 @@ void plan(Params &p, int head_dim, int kv_dtype) {
     }
   }
   p.items_own = own_items * p.s_own;
+  // The logits of a decode step's few query rows are kept (4 bytes each, written and read, against the key read
+  // again) where they stay below a gigabyte.
+  p.logit_rows = p.logit_stride = 0;
+  if (p.scores != nullptr && own_rows <= kRowsPerTile && p.tokens > 0) {
+    const int64_t stride = ceil_div(own_keys, 4) * 4;
+    if (stride * p.rows * p.kv_heads * own_rows <= (256ll << 20)) {
+      p.logit_rows = (int)own_rows;
+      p.logit_stride = stride;
+    }
+  }
   p.direct = p.wide_own && p.s_own == 1;
 }
 
 int64_t narrow_items(const Params &p) { return p.wide_own ? 0 : p.items_own + (p.wide_pre ? 0 : p.items_pre); }
 
+size_t partial_bytes(const Params &p, int head_dim) {
+  return p.direct ? 0 : (size_t)(p.s_own + p.s_pre) * p.tokens * p.q_heads * ((size_t)head_dim * 4 + 8);
+}
 size_t workspace_bytes(const Params &p, int head_dim) {
-  if (p.direct) return 16;
-  return (size_t)(p.s_own + p.s_pre) * p.tokens * p.q_heads * ((size_t)head_dim * 4 + 8);
+  return (partial_bytes(p, head_dim) + 15) / 16 * 16 + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4 + 16;
 }
 
 template <class T, int D>
 int launch(const Params &p, hipStream_t stream) {
-  const bool whole = p.block_size % 16 == 0;
   int rc = EKV_OK;
   if (p.tokens > 0) {
     if (p.wide_own || p.wide_pre) rc = wide_attention(p, T::kType, D, p.wide_own, stream);
-    const unsigned grid = (unsigned)ceil_div(narrow_items(p), kThreads / kWave);
+    using N = Narrow<T, D>;
+    const unsigned grid = (unsigned)ceil_div(narrow_items(p), N::kWaves);
     if (rc == EKV_OK && grid > 0) {
-      if (whole) hipLaunchKernelGGL((narrow_kernel<T, D, true>), dim3(grid), dim3(kThreads), 0, stream, p);
-      else hipLaunchKernelGGL((narrow_kernel<T, D, false>), dim3(grid), dim3(kThreads), 0, stream, p);
+      hipLaunchKernelGGL((narrow_kernel<T, D>), dim3(grid), dim3(N::kThreads), 0, stream, p);
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
     }
     if (rc == EKV_OK && !p.direct) {
@@ -510,12 +557,16 @@ int launch(const Params &p, hipStream_t stream) {
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention combine launch");
     }
   }
-  if (rc != EKV_OK || p.scores == nullptr) return rc;
-  if (p.width == 0) return rc;
-  const int pieces = (int)ceil_div((int64_t)p.width * p.block_size, kWeighKeys);
-  const unsigned weigh = (unsigned)ceil_div((int64_t)p.rows * pieces * p.kv_heads, kThreads / kWave);
-  if (whole) hipLaunchKernelGGL((weigh_kernel<T, D, true>), dim3(weigh), dim3(kThreads), 0, stream, p, pieces);
-  else hipLaunchKernelGGL((weigh_kernel<T, D, false>), dim3(weigh), dim3(kThreads), 0, stream, p, pieces);
+  if (rc != EKV_OK || p.scores == nullptr || p.width == 0) return rc;
+  const int64_t capacity = (int64_t)p.width * p.block_size, segments = (int64_t)p.rows * p.kv_heads;
+  if (p.logits != nullptr) {
+    const int pieces = (int)ceil_div(capacity, 4 * kThreads);
+    hipLaunchKernelGGL((fold_kernel<kThreads>), dim3((unsigned)(segments * pieces)), dim3(kThreads), 0, stream, p, pieces);
+  } else {
+    const int pieces = (int)ceil_div(capacity, kWeighKeys);
+    const unsigned weigh = (unsigned)ceil_div(segments * pieces, kThreads / kWave);
+    hipLaunchKernelGGL((weigh_kernel<T, D>), dim3(weigh), dim3(kThreads), 0, stream, p, pieces);
+  }
   return check_hip(hipGetLastError(), "ekv_prefix_attention weights launch");
 }
 
@@ -644,6 +695,7 @@ extern "C" int ekv_prefix_attention(const ekv_attention_t *a, void *workspace, s
   const int64_t queries = (int64_t)p.tokens * p.q_heads;
   p.part_o = (float *)workspace;
   p.part_ml = (float2 *)(p.part_o + (int64_t)(p.s_own + p.s_pre) * queries * a->head_dim);
+  if (p.logit_rows > 0) p.logits = (float *)((char *)workspace + (attn::partial_bytes(p, a->head_dim) + 15) / 16 * 16);
   hipStream_t s = (hipStream_t)stream;
   switch (a->kv_dtype) {
     case EKV_F32: return attn::launch_dim<attn::F32>(p, a->head_dim, s);

@@ -15,6 +15,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -42,6 +43,9 @@ struct Params {
   float *lse;
   float *part_o;   // [slots][tokens][q_heads][head_dim], unnormalised
   float2 *part_ml;  // [slots][tokens][q_heads]: maximum (in powers of two) and sum
+  float *logits;   // [rows][kv_heads][logit_rows][logit_stride], in powers of two, or null
+  int64_t logit_stride;
+  int logit_rows;
   int rows, width, groups, pwidth, tokens, max_query, q_heads, kv_heads, group, block_size;
   uint32_t bs_mul;  // page_divisor(block_size)
   int bs_shift;
@@ -62,148 +66,179 @@ __device__ __forceinline__ int page_of(const Params &p, int pos) {
 
 // -- element types --------------------------------------------------------------------------------
 //
-// A key row is the A operand of the matrix product S^T = K Q^T: lane l holds key l % 16 and, of its
-// head_dim elements, those of its lane group g = l / 16.  The contraction runs over all of them, so
-// which dims a lane group holds is free as long as the query operand agrees: each takes whole 16-byte
-// pieces.  Products of 16-bit (and fp8, converted exactly to bf16) elements are exact in the float32
+// Keys and values meet the matrix instructions out of LDS: fp8 ones are widened to bf16 on the way there,
+// which holds them exactly, the others keep their type.  Products of 16-bit elements are exact in the float32
 // they are summed in.
 
 struct F32 {
   static constexpr int kType = EKV_F32;
-  static constexpr int kBytes = 4;
-  static constexpr int kStepDims = 4;  // dims of one matrix instruction
+  static constexpr int kBytes = 4;  // of an element in the cache
+  static constexpr int kLds = 4;    // and in LDS
   typedef float Query;
+  typedef float Half;
 };
 struct F16 {
   static constexpr int kType = EKV_F16;
   static constexpr int kBytes = 2;
-  static constexpr int kStepDims = 32;
+  static constexpr int kLds = 2;
   typedef _Float16 Query;
+  typedef _Float16 Half;  // the 16-bit type that keys, values and weights meet in
 };
 struct BF16 {
   static constexpr int kType = EKV_BF16;
   static constexpr int kBytes = 2;
-  static constexpr int kStepDims = 32;
+  static constexpr int kLds = 2;
   typedef __bf16 Query;
+  typedef __bf16 Half;
 };
 struct FP8 {  // keys and values e4m3, queries bf16
   static constexpr int kType = EKV_FP8_E4M3;
   static constexpr int kBytes = 1;
-  static constexpr int kStepDims = 32;
+  static constexpr int kLds = 2;
   typedef __bf16 Query;
+  typedef __bf16 Half;
 };
 
 // 8 consecutive e4m3 values as bf16: both formats hold them exactly
-__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+__device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, true)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true))};
 }
 
-// element j of the dwords at w, as float32
+// two weights as 16-bit ones
+__device__ __forceinline__ uint32_t pack2(float a, float b, __bf16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, _Float16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+
+// products of 16 or 32 rows and columns over 32 or 16 of the contracted index
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// 16 x 16 over the 16 (float32) or 32 elements that one 16-byte piece a lane holds
 template <class T>
-__device__ __forceinline__ float element(const uint32_t *w, int j) {
+__device__ __forceinline__ f32x4 dot_piece(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (std::is_same<T, F32>::value) {
-    return __builtin_bit_cast(float, w[j]);
-  } else if constexpr (std::is_same<T, BF16>::value) {
-    return __builtin_bit_cast(float, (j & 1) ? (w[j / 2] & 0xffff0000u) : (w[j / 2] << 16));
-  } else if constexpr (std::is_same<T, F16>::value) {
-    const f16x2 h = __builtin_bit_cast(f16x2, w[j / 2]);
-    return (float)h[j & 1];
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
   } else {
-    const f32x2 f = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j / 4], true)
-                            : __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j / 4], false);
-    return f[j & 1];
+    return mfma16(a, b, c, typename T::Half{});
   }
 }
 
-// BYTES (2, 4, 8 or a multiple of 16) from global memory into dwords
-template <int BYTES>
-__device__ __forceinline__ void load_bytes(const char *src, uint32_t *dst) {
-  if constexpr (BYTES == 2) {
-    dst[0] = *as_global((const uint16_t *)src);
-  } else if constexpr (BYTES == 4) {
-    dst[0] = *as_global((const uint32_t *)src);
-  } else if constexpr (BYTES == 8) {
-    const u32x2 x = *as_global((const u32x2 *)src);
-    dst[0] = x[0];
-    dst[1] = x[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i) {
-      const u32x4 x = *as_global((const u32x4 *)(src + 16 * i));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[4 * i + e] = x[e];
-    }
+// Keys and values of a step in LDS, row by row.  The 16-byte pieces of a key row are permuted by the row's number
+// so that the reads of one piece of 16 (32) rows meet every bank; the 32-byte pieces of a 16-bit value row so that
+// the transposing reads, 4 (8) rows of 64 (32) bytes for half a wave, do.
+template <class T, int D>
+struct Lds {
+  static constexpr int kRow = D * T::kLds;
+  static constexpr int kLine = kRow < 256 ? 256 / kRow : 1;  // rows in 256 bytes
+  __device__ static __forceinline__ int key_at(int row, int piece) {
+    return row * kRow + (piece ^ (row / kLine & (kRow / 16 - 1) & 15)) * 16;
   }
-}
-
-// The first dim of the 8 (16-bit, fp8) or 4 (float32) that lane group g supplies in piece c of a row.
-template <class T, int D>
-__device__ __forceinline__ int piece_dim(int c, int g) {
-  if constexpr (std::is_same<T, F32>::value) return c * 16 + g * 4;
-  else if constexpr (std::is_same<T, FP8>::value && D >= 64) return (c / 2) * 64 + g * 16 + (c & 1) * 8;
-  else return c * 32 + g * 8;
-}
-template <class T, int D>
-constexpr int kPieces = std::is_same<T, F32>::value ? D / 16 : D / 32;
-
-// The lane's part of one key row: D / 4 elements.
-template <class T, int D>
-struct KeyRow {
-  static constexpr int kLoad = (std::is_same<T, FP8>::value && D == 32) ? 8 : 16;  // bytes of a load
-  static constexpr int kLoads = D * T::kBytes / 4 / kLoad;
-  uint32_t w[D * T::kBytes / 16];
-  __device__ __forceinline__ void load(const char *row, int g) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_bytes<kLoad>(row + (i * 4 + g) * kLoad, w + i * kLoad / 4);
+  // the byte of a value row; the 16 from a multiple of 16 on are together
+  __device__ static __forceinline__ int value_at(int row, int byte) {
+    if constexpr (T::kLds == 4) return row * kRow + byte;
+    const int chunk = byte / 64 ^ (row / kLine & (kRow / 64 - 1) & 3);
+    return row * kRow + chunk * 64 + ((byte & 32) ^ (row & 4) * 8) + byte % 32;
   }
 };
 
-// The lane's part of one query row, in the order of the key rows' pieces.
-template <class T, int D>
-struct QueryRow {
-  static constexpr int kDwords = std::is_same<T, F32>::value ? D / 4 : D / 8;
-  uint32_t w[kDwords];
-  __device__ __forceinline__ void load(const char *row, int g, bool live) {
-    constexpr int E = sizeof(typename T::Query);
+// The keys that a wave or workgroup reads: numbered along one axis, a prefix's first, of it [begin, end).
+struct Range {
+  const int32_t *ptable, *table;
+  int plen, begin, end, head;
+};
+
+// One step of KEYS keys and values on its way from memory through registers to LDS.  Loads take whole rows, 16
+// bytes a lane, the form that memory serves fastest.  The pages come one step ahead of the rows, a lookup a lane:
+// loads return in order, so a lookup right before its rows would wait for every row ahead of it.
+template <class T, int D, int KEYS, int THREADS>
+struct Stage {
+  static constexpr int kPieces = D * T::kBytes / 16;  // 16-byte pieces of a row in memory
+  static constexpr int kAll = KEYS * kPieces;
+  static constexpr int kLoads = (kAll + THREADS - 1) / THREADS;  // of a thread, for K and for V
+  static constexpr int kTile = KEYS * Lds<T, D>::kRow;           // LDS bytes of K, and of V behind it
+  int page;     // of this lane's key of the step after the next load
+  uint64_t ok;  // the keys of the loaded step that are there (KEYS = 32: twice)
+  u32x4 k[kLoads], v[kLoads];
+
+  // the thread's i-th piece, and whether there is one (KEYS * pieces is a multiple of 64, so a wave agrees)
+  __device__ __forceinline__ bool piece(int i, int &row, int &col) const {
+    const int at = (THREADS == kWave ? lane_id() : (int)threadIdx.x) + i * THREADS;
+    row = at / kPieces;
+    col = at % kPieces;
+    return kAll % THREADS == 0 || at < kAll;
+  }
+  __device__ __forceinline__ void look(const Params &p, const Range &s, int base) {
+    const int at = base + lane_id() % KEYS;
+    page = -1;
+    if (at < s.end) {
+      const bool shared = at < s.plen;
+      page = (shared ? s.ptable : s.table)[page_of(p, shared ? at : at - s.plen)];
+    }
+  }
+  __device__ __forceinline__ void load(const Params &p, const Range &s, int base) {
+    const int at = base + lane_id() % KEYS;
+    const int pos = at < s.plen ? at : at - s.plen;
+    const bool good = at < s.end && (uint32_t)page < (uint64_t)p.blocks;
+    ok = __ballot(good);
+    const int in_page = good ? pos - page_of(p, pos) * p.block_size : 0;
+    const int64_t off = ((int64_t)(good ? page : 0) * p.st_block + (int64_t)in_page * p.st_pos +
+                         (int64_t)s.head * p.st_head) * T::kBytes;
+    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
 #pragma unroll
-    for (int c = 0; c < kPieces<T, D>; ++c) {
-      if (live) load_bytes<16>(row + piece_dim<T, D>(c, g) * E, w + 4 * c);
-      else w[4 * c] = w[4 * c + 1] = w[4 * c + 2] = w[4 * c + 3] = 0;
+    for (int i = 0; i < kLoads; ++i) {
+      int row, col;
+      if (!piece(i, row, col)) break;
+      const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl(hi, row) << 32) | (uint32_t)__shfl(lo, row)) + col * 16;
+      k[i] = *as_global((const u32x4 *)(p.k + from));
+      v[i] = *as_global((const u32x4 *)(p.v + from));
+    }
+  }
+  // the values of keys that are not there as 0 (0 * NaN is no zero)
+  __device__ __forceinline__ void store(char *keys) const {
+    using L = Lds<T, D>;
+    char *values = keys + kTile;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      int row, col;
+      if (!piece(i, row, col)) break;
+      u32x4 x = v[i];
+      if (~ok != 0 && !(ok >> row & 1)) x = u32x4{0, 0, 0, 0};
+      if constexpr (T::kBytes == 1) {
+        *(u32x4 *)(keys + L::key_at(row, 2 * col)) = widen(k[i][0], k[i][1]);
+        *(u32x4 *)(keys + L::key_at(row, 2 * col + 1)) = widen(k[i][2], k[i][3]);
+        *(u32x4 *)(values + L::value_at(row, 32 * col)) = widen(x[0], x[1]);
+        *(u32x4 *)(values + L::value_at(row, 32 * col + 16)) = widen(x[2], x[3]);
+      } else {
+        *(u32x4 *)(keys + L::key_at(row, col)) = k[i];
+        *(u32x4 *)(values + L::value_at(row, 16 * col)) = x;
+      }
     }
   }
 };
 
-// S^T of 16 keys and 16 query rows: lane l receives keys 4 * (l / 16) + i of query row l % 16.
-template <class T, int D>
-__device__ __forceinline__ f32x4 dot_tile(const KeyRow<T, D> &k, const QueryRow<T, D> &q) {
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < kPieces<T, D>; ++c) {
-    if constexpr (std::is_same<T, F32>::value) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k.w[4 * c + e]),
-                                                   __builtin_bit_cast(float, q.w[4 * c + e]), acc, 0, 0, 0);
-    } else if constexpr (std::is_same<T, FP8>::value) {
-      const bf16x8 a = widen(k.w[2 * c], k.w[2 * c + 1]);
-      const bf16x8 b = __builtin_bit_cast(bf16x8, u32x4{q.w[4 * c], q.w[4 * c + 1], q.w[4 * c + 2], q.w[4 * c + 3]});
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
-    } else {
-      const u32x4 ka = {k.w[4 * c], k.w[4 * c + 1], k.w[4 * c + 2], k.w[4 * c + 3]};
-      const u32x4 qb = {q.w[4 * c], q.w[4 * c + 1], q.w[4 * c + 2], q.w[4 * c + 3]};
-      if constexpr (std::is_same<T, BF16>::value)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ka), __builtin_bit_cast(bf16x8, qb),
-                                                      acc, 0, 0, 0);
-      else
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, ka), __builtin_bit_cast(f16x8, qb), acc,
-                                                     0, 0, 0);
-    }
-  }
-  return acc;
+// Four values of one dim a lane out of LDS: in a group of 16 lanes, lane 4j + c gives the place of dims 4c .. 4c + 3
+// of key j, and lane n receives dim n of the four keys.
+__device__ __forceinline__ u32x2 read_transposed(const char *from) {
+  typedef __attribute__((address_space(3))) s16x4 *Ptr;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(from)));
 }
 
 // -- segments of work -------------------------------------------------------------------------------

@@ -18,57 +18,20 @@
 namespace ekv {
 namespace attn {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-template <class T>
-struct Half {  // the type of the operands in LDS: fp8 widens to bf16 exactly
-  typedef __bf16 type;
-};
-template <>
-struct Half<F16> {
-  typedef _Float16 type;
-};
-
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, __bf16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, _Float16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __bf16) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, _Float16) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
-}
-
-// The shapes of one instance.  K and V of a step lie in LDS row by row, their 16-byte pieces (K) and
-// 64-byte pieces (V) permuted within the row by the row's number, so that the reads (K: 32 rows of one
-// piece; V: 4 rows of 64 bytes) meet every bank once.
 template <class T, int D>
 struct Wide {
   static constexpr int kWaves = 4;
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kKeys = D == 256 ? 32 : 64;  // of a step
-  static constexpr int kRow = D * 2;                // bytes of a row in LDS
-  static constexpr int kPieces = D * T::kBytes / 16;  // 16-byte pieces of a row in memory
-  static constexpr int kLoads = (kKeys * kPieces + kThreads - 1) / kThreads;  // of a thread, for K and for V
-  static constexpr int kLine = kRow < 256 ? 256 / kRow : 1;                   // rows in 256 bytes
-  static constexpr int kTile = kKeys * kRow;
-  __device__ static __forceinline__ int key_at(int row, int piece) {
-    return row * kRow + (piece ^ (row / kLine & (D / 8 - 1) & 15)) * 16;
-  }
-  __device__ static __forceinline__ int value_chunk(int row, int chunk) {
-    return row * kRow + (chunk ^ (row / kLine & (D / 32 - 1) & 3)) * 64;
-  }
+  static constexpr int kRow = Lds<T, D>::kRow;
+  typedef Stage<T, D, kKeys, kThreads> Step;
+  static constexpr int kTile = Step::kTile;
 };
 
-// What a workgroup works on.  The keys are numbered along one axis, the prefix's first: [begin, end).
-struct Item {
-  const int32_t *ptable, *table;
-  int plen, begin, end;
+// What a workgroup works on.
+struct Item : Range {
   int first, rows, m0;  // first token, query rows, the tile's first one
-  int head, slot;
+  int slot;
   int see;              // query token i sees keys below plen + see + i
 };
 
@@ -85,7 +48,7 @@ __device__ __forceinline__ void clear_tokens(const Params &p, int from, int to, 
 }
 
 template <class T, int D>
-__device__ __forceinline__ bool own_item(const Params &p, int64_t index, Item &s) {
+__device__ __forceinline__ bool own_item(const Params &p, uint32_t index, Item &s) {
   using W = Wide<T, D>;
   s.head = (int)(index % p.kv_heads);
   index /= p.kv_heads;
@@ -123,7 +86,7 @@ __device__ __forceinline__ bool own_item(const Params &p, int64_t index, Item &s
 }
 
 template <class T, int D>
-__device__ __forceinline__ bool prefix_item(const Params &p, int64_t index, Item &s) {
+__device__ __forceinline__ bool prefix_item(const Params &p, uint32_t index, Item &s) {
   s.head = (int)(index % p.kv_heads);
   index /= p.kv_heads;
   const int chunk = (int)(index % p.s_pre);
@@ -144,66 +107,6 @@ __device__ __forceinline__ bool prefix_item(const Params &p, int64_t index, Item
   return s.begin < s.end;
 }
 
-// One step's keys and values on their way from memory to LDS.
-template <class T, int D>
-struct Stage {
-  using W = Wide<T, D>;
-  int page;        // of this lane's key of the step after the next load
-  u32x4 k[W::kLoads], v[W::kLoads];
-  uint64_t ok;     // the keys of the loaded step that are there
-
-  // the page of key `base + lane` (one load a lane, a step ahead of the rows')
-  __device__ __forceinline__ void look(const Params &p, const Item &s, int base) {
-    const int at = base + lane_id() % W::kKeys;
-    page = -1;
-    if (at < s.end) {
-      const bool shared = at < s.plen;
-      page = (shared ? s.ptable : s.table)[page_of(p, shared ? at : at - s.plen)];
-    }
-  }
-  __device__ __forceinline__ void load(const Params &p, const Item &s, int base) {
-    const int at = base + lane_id() % W::kKeys;
-    const int pos = at < s.plen ? at : at - s.plen;
-    const bool good = at < s.end && (uint32_t)page < (uint64_t)p.blocks;
-    ok = __ballot(good);
-    const int in_page = good ? pos - page_of(p, pos) * p.block_size : 0;
-    const int64_t off = ((int64_t)(good ? page : 0) * p.st_block + (int64_t)in_page * p.st_pos +
-                         (int64_t)s.head * p.st_head) * T::kBytes;
-    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
-#pragma unroll
-    for (int i = 0; i < W::kLoads; ++i) {
-      const int piece = threadIdx.x + i * W::kThreads;
-      if (W::kKeys * W::kPieces % W::kThreads != 0 && piece >= W::kKeys * W::kPieces) break;
-      const int row = piece / W::kPieces, col = piece % W::kPieces;
-      const int64_t at_row = (int64_t)(((uint64_t)(uint32_t)__shfl(hi, row) << 32) | (uint32_t)__shfl(lo, row)) + col * 16;
-      k[i] = *as_global((const u32x4 *)(p.k + at_row));
-      v[i] = *as_global((const u32x4 *)(p.v + at_row));
-    }
-  }
-  // K at `keys`, V behind it; the values of keys that are not there as 0 (0 * NaN is no zero)
-  __device__ __forceinline__ void store(char *keys) {
-    char *values = keys + W::kTile;
-#pragma unroll
-    for (int i = 0; i < W::kLoads; ++i) {
-      const int piece = threadIdx.x + i * W::kThreads;
-      if (W::kKeys * W::kPieces % W::kThreads != 0 && piece >= W::kKeys * W::kPieces) break;
-      const int row = piece / W::kPieces, col = piece % W::kPieces;
-      u32x4 x = v[i];
-      if (~ok != 0 && !(ok >> row & 1)) x = u32x4{0, 0, 0, 0};
-      if constexpr (T::kBytes == 1) {
-        *(u32x4 *)(keys + W::key_at(row, 2 * col)) = __builtin_bit_cast(u32x4, widen(k[i][0], k[i][1]));
-        *(u32x4 *)(keys + W::key_at(row, 2 * col + 1)) = __builtin_bit_cast(u32x4, widen(k[i][2], k[i][3]));
-        char *to = values + W::value_chunk(row, col / 2) + col % 2 * 32;
-        *(u32x4 *)to = __builtin_bit_cast(u32x4, widen(x[0], x[1]));
-        *(u32x4 *)(to + 16) = __builtin_bit_cast(u32x4, widen(x[2], x[3]));
-      } else {
-        *(u32x4 *)(keys + W::key_at(row, col)) = k[i];
-        *(u32x4 *)(values + W::value_chunk(row, col / 4) + col % 4 * 16) = x;
-      }
-    }
-  }
-};
-
 // The other lane half's value.
 __device__ __forceinline__ float other_half_max(float v) {
   float a, b;
@@ -223,7 +126,7 @@ constexpr float kSlack = 8.f;
 template <class T, int D>
 __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char *lds) {
   using W = Wide<T, D>;
-  typedef typename Half<T>::type H;
+  typedef typename T::Half H;
   constexpr int KT = W::kKeys / 32, DT = D / 32;
   const int lane = lane_id(), half = lane / 32, n = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -254,17 +157,17 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
   // LDS offsets of this lane's reads
   int key_off[D / 16], value_off[DT];
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) key_off[c] = W::key_at(n, 2 * c + half);
+  for (int c = 0; c < D / 16; ++c) key_off[c] = Lds<T, D>::key_at(n, 2 * c + half);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
-    value_off[d] = W::kTile + W::value_chunk(4 * half + lane % 16 / 4, d) + lane / 16 % 2 * 32 + lane % 4 * 8;
+    value_off[d] = W::kTile + Lds<T, D>::value_at(4 * half + lane % 16 / 4, d * 64 + lane / 16 % 2 * 32 + lane % 4 * 8);
 
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float top = -INFINITY, sum = 0.f;
 
-  Stage<T, D> stage;
+  typename W::Step stage;
   uint64_t ok = 0;
   if (s.begin < s.end) {
     stage.look(p, s, s.begin);
@@ -329,11 +232,8 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
         for (int i = 0; i < 4; ++i) w[i] = pack2(x[t / 2][8 * (t % 2) + 2 * i], x[t / 2][8 * (t % 2) + 2 * i + 1], H{});
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          typedef __attribute__((address_space(3))) s16x4 *Lds;
           const char *from = buffer + value_off[d] + t * 16 * W::kRow;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 8 * W::kRow));
-          const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+          const u32x2 a = read_transposed(from), b = read_transposed(from + 8 * W::kRow);
           acc[d] = mfma32(u32x4{a[0], a[1], b[0], b[1]}, w, acc[d], H{});
         }
       }
