@@ -527,7 +527,7 @@ typedef struct ekv_attention {
  * equal bits.
  * Types: fp32, f16 and bf16 with keys and values of the same type, or fp8 e4m3 keys and values with bf16
  * queries.  head_dim 32, 64, 128 or 256; any block size and any number of query heads per KV head; rows of
- * the query, keys and values start at multiples of 16 bytes; width * block_size below 2^31.
+ * the query, keys and values start at multiples of 16 bytes; width * block_size below 2^31 - 4096.
  * workspace: ekv_prefix_attention_workspace(a) bytes of device memory (0: the arguments are refused or
  * empty), 16-byte aligned, which the call may overwrite.
  */

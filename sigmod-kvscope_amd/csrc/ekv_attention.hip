@@ -6,59 +6,31 @@
 //   scores[row, head, j] = decay * scores[row, head, j] + sum_{q of the row and head} exp(s_qj - lse_q)
 //
 // A query sees the whole prefix of its row's group and its row's own keys up to itself.  The keys are cut
-// into chunks, every (chunk, KV head, tile of query rows) is one item of work, and an item leaves its
-// maximum, sum and unnormalised output, which combine_kernel joins:
+// into pieces; a piece leaves its maximum, sum and unnormalised output for each of its query rows, which
+// combine_kernel joins:
 //   m = max_c m_c,  l = sum_c l_c 2^(m_c - m),  out = sum_c o_c 2^(m_c - m) / l.
-// A prefix is one set of items for all the queries of its group: its keys and values are read once per
-// tile of them and not once per row.
+// A prefix is read once per tile of its group's query rows and not once per row.
 #include "ekv_attention.hpp"
-#include <stdlib.h>
 
 namespace ekv {
 namespace attn {
+
+__host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // What one wave works on.
 struct Segment : Range {
   int first, rows;  // first token, query rows (tokens * group)
   int m0;           // the tile's first query row
-  int row, slot;    // the batch row (own keys), the slot of the partial results
+  int row, slot;    // the batch row (own keys; -1: a prefix), the slot of the partial results
   int see;          // query token i sees keys below see + i (own pages), or INT_MAX / 2 (a prefix)
 };
 
-template <int TILE>
-__device__ __forceinline__ bool own_segment(const Params &p, uint32_t item, Segment &s) {
-  s.head = (int)(item % p.kv_heads);
-  item /= p.kv_heads;
-  const int tile = (int)(item % p.tiles_own);
-  item /= p.tiles_own;
-  const int chunk = (int)(item % p.s_own);
-  const int row = (int)(item / p.s_own);
-  const int len = row_length(p, row);
-  const RowQueries t = row_queries(p, row);
-  s.table = p.table + (int64_t)row * p.table_stride;
-  s.ptable = nullptr;
-  s.plen = 0;
-  s.row = row;
-  s.first = t.first;
-  s.rows = min(t.count, p.max_query) * p.group;
-  s.m0 = tile * TILE;
-  s.see = len - t.count + 1;
-  s.slot = chunk;
-  if (s.m0 >= s.rows) return false;
-  const int last = (min(s.m0 + TILE, s.rows) - 1) / p.group;
-  const int64_t begin = (int64_t)chunk * p.chunk_own;
-  s.end = (int)min(begin + p.chunk_own, (int64_t)min(len, s.see + last));
-  s.begin = (int)min(begin, (int64_t)INT32_MAX);
-  return s.begin < s.end;
-}
-
-template <int TILE>
 __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, Segment &s) {
   s.head = (int)(item % p.kv_heads);
   item /= p.kv_heads;
   const int chunk = (int)(item % p.s_pre);
   int g, tile;
-  if (!find_tile(p, (int)(item / p.s_pre), TILE, g, tile)) return false;
+  if (!find_tile(p, (int)(item / p.s_pre), kRowsPerTile, g, tile)) return false;
   const RowQueries t = group_queries(p, g);
   s.table = p.ptable + (int64_t)g * p.ptable_stride;
   s.ptable = nullptr;
@@ -66,7 +38,7 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, S
   s.row = -1;
   s.first = t.first;
   s.rows = t.count * p.group;
-  s.m0 = tile * TILE;
+  s.m0 = tile * kRowsPerTile;
   s.see = INT32_MAX / 2;
   s.slot = p.s_own + chunk;
   const int64_t begin = (int64_t)chunk * p.chunk_pre;
@@ -85,6 +57,9 @@ struct Narrow {
   static constexpr int kBytes = 2 * Step::kTile;  // LDS of a wave
   static constexpr int kWaves = kBytes > 16384 ? 2 : 4;
   static constexpr int kThreads = kWaves * kWave;
+  // waves of a compute unit: as many as LDS has room for, 2 a SIMD (1 at head dim 256) at most for their registers
+  static constexpr int kFit = 163840 / (kWaves * kBytes + 1024) * kWaves;
+  static constexpr int kResident = kFit < (D == 256 ? 4 : 8) ? kFit : (D == 256 ? 4 : 8);
   static constexpr int kPieceDims = D >= 64 ? 4 : 2;  // float32: dims of a value row that a lane reads at once
 };
 
@@ -107,7 +82,7 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
   const int every = min(s.end, s.see + s.m0 / p.group);  // and every query of the tile keys below this
 
   typename N::Step stage;
-  stage.look(p, s, s.begin);
+  if (s.begin < s.end) stage.look(p, s, s.begin);
   u32x4 q[QP];
 #pragma unroll
   for (int c = 0; c < QP; ++c) {
@@ -115,8 +90,10 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
     if (live)
       q[c] = *as_global((const u32x4 *)(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E + (4 * c + g) * 16));
   }
-  stage.load(p, s, s.begin);
-  stage.look(p, s, s.begin + N::kKeys);
+  if (s.begin < s.end) {
+    stage.load(p, s, s.begin);
+    stage.look(p, s, s.begin + N::kKeys);
+  }
 
   int key_off[QP];
 #pragma unroll
@@ -233,21 +210,134 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
 
 constexpr int kThreads = 256;
 
+// The own keys of a decode step stream at the rate that memory has only if every wave has the same share of them to
+// the end: rows have lengths that the host does not know, and items of a fixed length left the last ones running
+// alone (128 rows of 512 to 8192 tokens: 427 us in chunks of 256 or 1024 keys against 358 us, 6.4 TB/s).  So the units of 64 keys of
+// all rows, one row after the other, are one list; each (KV head, query tile) has `share` waves, and wave j of them
+// takes units j T / share to (j + 1) T / share of the T, in at most kMaxSlots pieces a row.
+constexpr int kUnit = 64;
+
+struct Share {
+  int64_t total;  // units of all rows
+  int share;      // waves that have some
+  // the wave that unit x is in
+  __device__ __forceinline__ int wave_of(int64_t x) const { return (int)(((x + 1) * share - 1) / total); }
+};
+
+__device__ __forceinline__ int row_units(const Params &p, int row) { return (row_length(p, row) + kUnit - 1) / kUnit; }
+
+// Every thread of the workgroup: the list's size, the waves that share it, and for wave w of the workgroup, number
+// w of `first` on of its head and tile, the row that its first unit is in and the units before that row.
+template <int WAVES>
+__device__ __forceinline__ Share share_out(const Params &p, int64_t first, int *start_row, int64_t *start_at) {
+  constexpr int kN = WAVES * kWave;
+  __shared__ int64_t s_sum[WAVES];
+  __shared__ int s_max[WAVES];
+  const int wave = threadIdx.x / kWave, per = (p.rows + kN - 1) / kN;
+  const int r0 = min((int)threadIdx.x * per, p.rows), r1 = min(r0 + per, p.rows);
+  int64_t mine = 0;
+  int longest = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int n = row_units(p, r);
+    mine += n;
+    longest = max(longest, n);
+  }
+  int64_t inclusive = mine;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t other = __shfl_up(inclusive, d);
+    if (lane_id() >= d) inclusive += other;
+    longest = max(longest, __shfl_xor(longest, d));
+  }
+  if (lane_id() == kWave - 1) s_sum[wave] = inclusive;
+  if (lane_id() == 0) s_max[wave] = longest;
+  __syncthreads();
+  int64_t before = inclusive - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    before += w < wave ? s_sum[w] : 0;
+    total += s_sum[w];
+    longest = max(longest, s_max[w]);
+  }
+  Share s;
+  s.total = total;
+  int64_t share = min((int64_t)p.share, total);
+  // a row of u units meets at most u share / total + 2 waves
+  if (longest > 0) share = min(share, max((int64_t)1, total * (p.s_own - 2) / longest));
+  s.share = (int)share;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int64_t j = (first + w) / ((int64_t)p.kv_heads * p.tiles_own);
+    if (j >= share) continue;
+    const int64_t x = j * total / share;
+    if (x < before || x >= before + mine) continue;
+    int64_t at = before;
+    for (int r = r0; r < r1; ++r) {
+      const int n = row_units(p, r);
+      if (x < at + n) {
+        start_row[w] = r;
+        start_at[w] = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  return s;
+}
+
 template <class T, int D>
 __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void narrow_kernel(const Params p) {
   using N = Narrow<T, D>;
   __shared__ __attribute__((aligned(16))) char lds[N::kWaves * N::kBytes];
+  __shared__ int s_row[N::kWaves];
+  __shared__ int64_t s_at[N::kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t item = (int64_t)blockIdx.x * N::kWaves + wave;
-  const int64_t shared = p.wide_pre ? 0 : p.items_pre;  // items of the prefixes come first
+  char *mine = lds + wave * N::kBytes;
+  const int64_t shared = p.wide_pre ? 0 : ceil_div(p.items_pre, N::kWaves);  // the prefixes' items come first
   Segment s;
-  if (item < shared) {
-    if (!prefix_segment<kRowsPerTile>(p, item, s)) return;
-  } else {
-    if (item - shared >= p.items_own) return;
-    if (!own_segment<kRowsPerTile>(p, item - shared, s)) return;
+  if (blockIdx.x < shared) {
+    const int64_t item = (int64_t)blockIdx.x * N::kWaves + wave;
+    if (item < p.items_pre && prefix_segment(p, (uint32_t)item, s)) attend<T, D>(p, s, mine);
+    return;
   }
-  attend<T, D>(p, s, lds + wave * N::kBytes);
+  const int64_t first = (blockIdx.x - shared) * N::kWaves;
+  const Share share = share_out<N::kWaves>(p, first, s_row, s_at);
+  const int each = p.kv_heads * p.tiles_own;
+  const int j = (int)((first + wave) / each), part = (int)((first + wave) % each);
+  if (j >= share.share) return;
+  s.head = part % p.kv_heads;
+  s.m0 = part / p.kv_heads * kRowsPerTile;
+  s.ptable = nullptr;
+  s.plen = 0;
+  int64_t at = (int64_t)j * share.total / share.share;
+  const int64_t stop = (int64_t)(j + 1) * share.total / share.share;
+  s.row = __builtin_amdgcn_readfirstlane(s_row[wave]);
+  int64_t row_at = s_at[wave];  // the units before the row
+  while (true) {
+    const int len = row_length(p, s.row), units = (len + kUnit - 1) / kUnit;
+    if (units > 0) {
+      const int j0 = share.wave_of(row_at), j1 = share.wave_of(row_at + units - 1);
+      if (part == 0 && j == j0 && lane_id() == 0) p.row_slots[s.row] = j1 - j0 + 1;
+      const RowQueries t = row_queries(p, s.row);
+      s.table = p.table + (int64_t)s.row * p.table_stride;
+      s.first = t.first;
+      s.rows = min(t.count, p.max_query) * p.group;
+      s.see = len - t.count + 1;
+      s.slot = j - j0;
+      const int u0 = (int)(at - row_at), u1 = (int)(min(stop, row_at + units) - row_at);
+      s.begin = u0 * kUnit;
+      if (s.m0 < s.rows) {
+        const int last = (min(s.m0 + kRowsPerTile, s.rows) - 1) / p.group;
+        s.end = (int)min((int64_t)u1 * kUnit, (int64_t)min(len, s.see + last));  // may be before s.begin: the partial result is empty
+        attend<T, D>(p, s, mine);
+      }
+      at = row_at + u1;
+      row_at += units;
+    }
+    if (at >= stop) break;
+    ++s.row;
+  }
 }
 
 // -- joining the chunks ---------------------------------------------------------------------------------
@@ -288,7 +378,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
       const int64_t all = (int64_t)n + max(seen, 0);
       own = all > 0 ? (int)((all - 1) / p.chunk_own) + 1 : 0;
     } else {
-      own = seen > 0 ? (seen - 1) / p.chunk_own + 1 : 0;
+      own = seen > 0 ? p.row_slots[row] : 0;
       pre = n > 0 ? (n - 1) / p.chunk_pre + 1 : 0;
     }
   }
@@ -458,11 +548,8 @@ __global__ __launch_bounds__(kThreads) void weigh_kernel(const Params p, int pie
 
 // -- the launches ---------------------------------------------------------------------------------------
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// How the keys are cut.  A long table is cut so that the items fill the chip several times over (rows have
-// different lengths and the host knows only the widest), but no chunk is shorter than 64 keys, and the
-// partial outputs stay below 256 MB.
+// How a prefix's keys are cut where the narrow kernel reads them: so that the items fill the chip several times
+// over, but no chunk is shorter than 64 keys, and the partial outputs stay below 256 MB.
 void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim, int &chunk, int &slots) {
   const int64_t target = 32 * (int64_t)cu_count();
   int64_t n = ceil_div(target, items_per_chunk > 0 ? items_per_chunk : 1);
@@ -472,7 +559,6 @@ void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim,
   n = n > kMaxSlots ? kMaxSlots : n < 1 ? 1 : n;
   chunk = (int)(ceil_div(ceil_div(keys, n), 64) * 64);
   if (chunk < 64) chunk = 64;
-  if (getenv("EKV_CHUNK")) chunk = atoi(getenv("EKV_CHUNK"));
   slots = (int)ceil_div(keys, chunk);
   if (slots < 1) slots = 1;
 }
@@ -488,6 +574,16 @@ void split_wide(int64_t keys, int64_t items_per_chunk, int64_t queries, int head
   chunk = (int)(each < 512 ? 512 : each > (1 << 30) ? INT32_MAX : each);
   slots = (int)ceil_div(keys, chunk);
   if (slots < 1) slots = 1;
+}
+
+template <class T>
+int narrow_waves(int head_dim) {
+  return head_dim == 32 ? Narrow<T, 32>::kResident : head_dim == 64 ? Narrow<T, 64>::kResident
+         : head_dim == 128 ? Narrow<T, 128>::kResident : Narrow<T, 256>::kResident;
+}
+int narrow_waves(int kv_dtype, int head_dim) {
+  return kv_dtype == EKV_F32 ? narrow_waves<F32>(head_dim) : kv_dtype == EKV_FP8_E4M3 ? narrow_waves<FP8>(head_dim)
+                                                                                     : narrow_waves<BF16>(head_dim);
 }
 
 void plan(Params &p, int head_dim, int kv_dtype) {
@@ -508,7 +604,16 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   if (p.wide_own) {
     split_wide(own_keys + prefix_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
   } else {
-    split(own_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
+    // waves that a (KV head, tile) has: all together those that the chip holds, and no more than there are units
+    const int64_t each = (int64_t)p.kv_heads * p.tiles_own, units = p.rows * ceil_div(own_keys, kUnit);
+    int64_t share = (int64_t)cu_count() * narrow_waves(kv_dtype, head_dim) / each;
+    share = share > units ? units : share;
+    p.share = (int)(share < 1 ? 1 : share);
+    int64_t slots = ceil_div(own_keys, kUnit);
+    const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
+    slots = slots > fit ? fit : slots;
+    p.s_own = (int)(slots > kMaxSlots ? kMaxSlots : slots < 3 ? 3 : slots);
+    p.waves_own = each * p.share;
     if (p.groups > 0) {
       p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
       const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
@@ -517,7 +622,7 @@ void plan(Params &p, int head_dim, int kv_dtype) {
       p.items_pre = items * p.s_pre;
     }
   }
-  p.items_own = own_items * p.s_own;
+  p.items_own = p.wide_own ? own_items * p.s_own : 0;
   // The logits of a decode step's few query rows are kept (4 bytes each, written and read, against the key read
   // again) where they stay below a gigabyte.
   p.logit_rows = p.logit_stride = 0;
@@ -531,13 +636,12 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   p.direct = p.wide_own && p.s_own == 1;
 }
 
-int64_t narrow_items(const Params &p) { return p.wide_own ? 0 : p.items_own + (p.wide_pre ? 0 : p.items_pre); }
-
 size_t partial_bytes(const Params &p, int head_dim) {
   return p.direct ? 0 : (size_t)(p.s_own + p.s_pre) * p.tokens * p.q_heads * ((size_t)head_dim * 4 + 8);
 }
 size_t workspace_bytes(const Params &p, int head_dim) {
-  return (partial_bytes(p, head_dim) + 15) / 16 * 16 + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4 + 16;
+  return (partial_bytes(p, head_dim) + 15) / 16 * 16 + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4 +
+         (size_t)p.rows * 4 + 16;
 }
 
 template <class T, int D>
@@ -546,7 +650,8 @@ int launch(const Params &p, hipStream_t stream) {
   if (p.tokens > 0) {
     if (p.wide_own || p.wide_pre) rc = wide_attention(p, T::kType, D, p.wide_own, stream);
     using N = Narrow<T, D>;
-    const unsigned grid = (unsigned)ceil_div(narrow_items(p), N::kWaves);
+    const unsigned grid = p.wide_own ? 0 : (unsigned)((p.wide_pre ? 0 : ceil_div(p.items_pre, N::kWaves)) +
+                                                      ceil_div(p.waves_own, N::kWaves));
     if (rc == EKV_OK && grid > 0) {
       hipLaunchKernelGGL((narrow_kernel<T, D>), dim3(grid), dim3(N::kThreads), 0, stream, p);
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
@@ -598,8 +703,8 @@ int fill(const ekv_attention_t *a, Params &p) {
   if (a->q_start == nullptr && (a->tokens != a->rows || a->max_query != 1))
     return fail(EKV_EINVAL, "%s: %d tokens, at most %d a row, of %d rows need q_start", who, a->tokens, a->max_query,
                 a->rows);
-  if ((int64_t)a->width * a->block_size >= INT32_MAX || (int64_t)a->prefix_width * a->block_size >= INT32_MAX)
-    return fail(EKV_EINVAL, "%s: a table of %d or %d blocks of %d tokens passes 2^31", who, a->width, a->prefix_width,
+  if ((int64_t)a->width * a->block_size >= kMostKeys || (int64_t)a->prefix_width * a->block_size >= kMostKeys)
+    return fail(EKV_EINVAL, "%s: a table of %d or %d blocks of %d tokens passes 2^31 - 4096", who, a->width, a->prefix_width,
                 a->block_size);
   if ((int64_t)a->tokens * a->q_heads >= INT32_MAX - 65536 || (int64_t)a->max_query * a->q_heads >= INT32_MAX - 65536)
     return fail(EKV_EINVAL, "%s: %d tokens of %d heads pass 2^31", who, a->tokens, a->q_heads);
@@ -647,8 +752,9 @@ int fill(const ekv_attention_t *a, Params &p) {
   p.v_scale = a->v_scale;
   p.decay = a->decay;
   plan(p, a->head_dim, a->kv_dtype);
-  // a launch has fewer than 2^32 threads: 64 an item of the narrow kernel, 256 of the wide one
-  if (narrow_items(p) >= (1ll << 26) - 64 || (p.wide_own ? p.items_own : p.wide_pre ? p.items_pre : 0) >= (1ll << 24) ||
+  // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel, 256 an item of the wide one
+  if (p.waves_own + (p.wide_pre ? 0 : p.items_pre) >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
+      (p.wide_pre && p.items_pre >= (1ll << 24)) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
       (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >= (1ll << 26) - 64))
     return fail(EKV_EINVAL, "%s: %d rows of %d blocks and %d tokens of %d heads pass the threads of a launch", who,
@@ -695,7 +801,9 @@ extern "C" int ekv_prefix_attention(const ekv_attention_t *a, void *workspace, s
   const int64_t queries = (int64_t)p.tokens * p.q_heads;
   p.part_o = (float *)workspace;
   p.part_ml = (float2 *)(p.part_o + (int64_t)(p.s_own + p.s_pre) * queries * a->head_dim);
-  if (p.logit_rows > 0) p.logits = (float *)((char *)workspace + (attn::partial_bytes(p, a->head_dim) + 15) / 16 * 16);
+  char *more = (char *)workspace + (attn::partial_bytes(p, a->head_dim) + 15) / 16 * 16;
+  if (p.logit_rows > 0) p.logits = (float *)more;
+  p.row_slots = (int32_t *)(more + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4);
   hipStream_t s = (hipStream_t)stream;
   switch (a->kv_dtype) {
     case EKV_F32: return attn::launch_dim<attn::F32>(p, a->head_dim, s);

@@ -22,6 +22,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRowsPerTile = 16;  // query rows of one narrow tile (the matrix instruction's columns)
 constexpr int kWideRows = 64;     // from so many query rows a set of keys on, the wide kernel
+constexpr int kMostKeys = INT32_MAX - 4095;  // of a table row: a step past its last key is still an int
 constexpr int kMaxSlots = 64;     // partial results a query row can have from its own pages, and from its prefix
 
 struct Params {
@@ -50,7 +51,11 @@ struct Params {
   uint32_t bs_mul;  // page_divisor(block_size)
   int bs_shift;
   float scale2, v_scale, decay;  // scale2: scale * k_scale * log2(e)
-  // the split: own pages in s_own chunks of chunk_own keys, prefixes in s_pre chunks of chunk_pre
+  int32_t *row_slots;  // [rows]: the slots that a row's own keys have partial results in (narrow kernel)
+  // the split: at most s_own slots for the own keys (wide kernel: chunks of chunk_own keys; narrow kernel: the
+  // pieces of `share` waves a head and tile, waves_own in all), prefixes in s_pre chunks of chunk_pre
+  int share;
+  int64_t waves_own;
   int chunk_own, s_own, tiles_own, chunk_pre, s_pre, tiles_pre;
   int tile_own, tile_pre;  // query rows of a tile
   int64_t items_own, items_pre;
@@ -207,8 +212,13 @@ struct Stage {
       int row, col;
       if (!piece(i, row, col)) break;
       const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl(hi, row) << 32) | (uint32_t)__shfl(lo, row)) + col * 16;
-      k[i] = *as_global((const u32x4 *)(p.k + from));
-      v[i] = *as_global((const u32x4 *)(p.v + from));
+      if constexpr (THREADS == kWave) {  // read once: the stream leaves the caches to others
+        k[i] = __builtin_nontemporal_load(as_global((const u32x4 *)(p.k + from)));
+        v[i] = __builtin_nontemporal_load(as_global((const u32x4 *)(p.v + from)));
+      } else {
+        k[i] = *as_global((const u32x4 *)(p.k + from));
+        v[i] = *as_global((const u32x4 *)(p.v + from));
+      }
     }
   }
   // the values of keys that are not there as 0 (0 * NaN is no zero)
