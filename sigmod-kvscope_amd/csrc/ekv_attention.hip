@@ -212,11 +212,9 @@ constexpr int kThreads = 256;
 
 // The own keys of a decode step stream at the rate that memory has only if every wave has the same share of them to
 // the end: rows have lengths that the host does not know, and items of a fixed length left the last ones running
-// alone (128 rows of 512 to 8192 tokens: 427 us in chunks of 256 or 1024 keys against 358 us, 6.4 TB/s).  So the units of 64 keys of
+// alone (128 rows of 512 to 8192 tokens: 427 us in chunks of 256 or 1024 keys against 358 us, 6.4 TB/s).  So the steps of
 // all rows, one row after the other, are one list; each (KV head, query tile) has `share` waves, and wave j of them
-// takes units j T / share to (j + 1) T / share of the T, in at most kMaxSlots pieces a row.
-constexpr int kUnit = 64;
-
+// takes steps j T / share to (j + 1) T / share of the T, in at most kMaxSlots pieces a row.
 struct Share {
   int64_t total;  // units of all rows
   int share;      // waves that have some
@@ -224,11 +222,12 @@ struct Share {
   __device__ __forceinline__ int wave_of(int64_t x) const { return (int)(((x + 1) * share - 1) / total); }
 };
 
-__device__ __forceinline__ int row_units(const Params &p, int row) { return (row_length(p, row) + kUnit - 1) / kUnit; }
+template <int UNIT>
+__device__ __forceinline__ int row_units(const Params &p, int row) { return (row_length(p, row) + UNIT - 1) / UNIT; }
 
 // Every thread of the workgroup: the list's size, the waves that share it, and for wave w of the workgroup, number
 // w of `first` on of its head and tile, the row that its first unit is in and the units before that row.
-template <int WAVES>
+template <int WAVES, int UNIT>
 __device__ __forceinline__ Share share_out(const Params &p, int64_t first, int *start_row, int64_t *start_at) {
   constexpr int kN = WAVES * kWave;
   __shared__ int64_t s_sum[WAVES];
@@ -238,7 +237,7 @@ __device__ __forceinline__ Share share_out(const Params &p, int64_t first, int *
   int64_t mine = 0;
   int longest = 0;
   for (int r = r0; r < r1; ++r) {
-    const int n = row_units(p, r);
+    const int n = row_units<UNIT>(p, r);
     mine += n;
     longest = max(longest, n);
   }
@@ -273,7 +272,7 @@ __device__ __forceinline__ Share share_out(const Params &p, int64_t first, int *
     if (x < before || x >= before + mine) continue;
     int64_t at = before;
     for (int r = r0; r < r1; ++r) {
-      const int n = row_units(p, r);
+      const int n = row_units<UNIT>(p, r);
       if (x < at + n) {
         start_row[w] = r;
         start_at[w] = at;
@@ -302,7 +301,7 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
     return;
   }
   const int64_t first = (blockIdx.x - shared) * N::kWaves;
-  const Share share = share_out<N::kWaves>(p, first, s_row, s_at);
+  const Share share = share_out<N::kWaves, N::kKeys>(p, first, s_row, s_at);
   const int each = p.kv_heads * p.tiles_own;
   const int j = (int)((first + wave) / each), part = (int)((first + wave) % each);
   if (j >= share.share) return;
@@ -315,7 +314,7 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
   s.row = __builtin_amdgcn_readfirstlane(s_row[wave]);
   int64_t row_at = s_at[wave];  // the units before the row
   while (true) {
-    const int len = row_length(p, s.row), units = (len + kUnit - 1) / kUnit;
+    const int len = row_length(p, s.row), units = (len + N::kKeys - 1) / N::kKeys;
     if (units > 0) {
       const int j0 = share.wave_of(row_at), j1 = share.wave_of(row_at + units - 1);
       if (part == 0 && j == j0 && lane_id() == 0) p.row_slots[s.row] = j1 - j0 + 1;
@@ -326,10 +325,10 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
       s.see = len - t.count + 1;
       s.slot = j - j0;
       const int u0 = (int)(at - row_at), u1 = (int)(min(stop, row_at + units) - row_at);
-      s.begin = u0 * kUnit;
+      s.begin = u0 * N::kKeys;
       if (s.m0 < s.rows) {
         const int last = (min(s.m0 + kRowsPerTile, s.rows) - 1) / p.group;
-        s.end = (int)min((int64_t)u1 * kUnit, (int64_t)min(len, s.see + last));  // may be before s.begin: the partial result is empty
+        s.end = (int)min((int64_t)u1 * N::kKeys, (int64_t)min(len, s.see + last));  // may be before s.begin: the partial result is empty
         attend<T, D>(p, s, mine);
       }
       at = row_at + u1;
@@ -353,16 +352,17 @@ __device__ __forceinline__ int row_of(const Params &p, int token) {
   }
   return lo;
 }
-__device__ __forceinline__ void store(float *dst, float v) { *dst = v; }
-__device__ __forceinline__ void store(__bf16 *dst, float v) { *dst = (__bf16)v; }
-__device__ __forceinline__ void store(_Float16 *dst, float v) { *dst = (_Float16)v; }
-
-// One wave per (token, query head): lane t weighs slot t, then the slots' outputs are summed in slot order.
-template <class Q, int D>
-__global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
+// W waves per (token, query head), each with a share of the slots: lane t weighs slot t of 64, then the slots'
+// outputs are summed in slot order, and the waves' sums in wave order.  Few queries (one row of 8192 tokens has 32
+// of 254 slots) are a matter of latency and take 8 waves each; many have few slots each and take one (128 rows of
+// 32 heads: 4.7 us, where 4 waves took 9.2).
+template <class Q, int D, int W>
+__global__ __launch_bounds__(W == 1 ? kThreads : W *kWave) void combine_kernel(const Params p) {
+  constexpr int kWaves = W == 1 ? kThreads / kWave : W;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / kWave) + wave;
-  if (item >= (int64_t)p.tokens * p.q_heads) return;
+  const int64_t item = ((int64_t)blockIdx.x * kWaves + wave) / W;
+  const int part = wave % W;
+  if (item >= (int64_t)p.tokens * p.q_heads) return;  // W > 1: the whole workgroup
   const int lane = lane_id();
   const int token = (int)(item / p.q_heads), q_head = (int)(item - (int64_t)token * p.q_heads);
   const int row = row_of(p, token);
@@ -384,38 +384,52 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
   }
   constexpr int kPer = D > 64 ? D / 64 : 1;
   constexpr int kLanes = D / kPer;
-  float acc[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+  constexpr int kFlight = W == 1 ? 8 : 16;
+  typedef float Piece __attribute__((ext_vector_type(kPer)));
+  Piece acc = {};
   float top = -INFINITY, sum = 0.f;
   const int64_t plane = (int64_t)p.tokens * p.q_heads;
-  for (int part = 0; part < 2; ++part) {
-    const int slots = part == 0 ? own : pre, first = part == 0 ? 0 : p.s_own;
-    if (slots == 0) continue;
+  const int each = (own + pre + W - 1) / W;
+  const int end = min((part + 1) * each, own + pre);
+  auto slot = [&](int k) { return k < own ? k : p.s_own + k - own; };
+  for (int k0 = part * each; k0 < end; k0 += kWave) {
+    const int n = min(end - k0, kWave);
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < slots) ml = p.part_ml[(int64_t)(first + lane) * plane + item];
+    if (lane < n) ml = p.part_ml[(int64_t)slot(k0 + lane) * plane + item];
     const float peak = fmaxf(top, wave_max(ml.x));
     const float ref = peak == -INFINITY ? 0.f : peak;
     const float shrink = __builtin_amdgcn_exp2f(top - ref);
     const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - ref);
     sum = sum * shrink + wave_sum(ml.y * w);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] *= shrink;
+    acc *= shrink;
     top = peak;
-    const float *o = p.part_o + ((int64_t)first * plane + item) * D + (lane % kLanes) * kPer;
-    // four slots' loads in flight; past the last slot the weight is 0 and the last slot is read again
-    for (int k = 0; k < slots; k += 4) {
-      float x[4][kPer];
+    const float *o = p.part_o + item * D + (lane % kLanes) * kPer;
+    // past the last slot the weight is 0 and the last slot is read again
+    for (int k = 0; k < n; k += kFlight) {
+      Piece x[kFlight];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < kFlight; ++u) x[u] = *(const Piece *)(o + (int64_t)slot(k0 + min(k + u, n - 1)) * plane * D);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) x[u][j] = o[(int64_t)min(k + u, slots - 1) * plane * D + j];
+      for (int u = 0; u < kFlight; ++u)
+        acc += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), k + u)) * x[u];
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float s_top[W], s_sum[W];
+    __shared__ Piece s_acc[W][kLanes];
+    if (lane < kLanes) s_acc[part][lane] = acc;
+    s_top[part] = top;
+    s_sum[part] = sum;
+    __syncthreads();
+    if (part != 0) return;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), k + u));
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] += k + u < slots ? wk * x[u][j] : 0.f;
-      }
+    for (int w = 1; w < W; ++w) {
+      const float peak = fmaxf(top, s_top[w]);
+      const float ref = peak == -INFINITY ? 0.f : peak;
+      const float a = __builtin_amdgcn_exp2f(top - ref), b = __builtin_amdgcn_exp2f(s_top[w] - ref);
+      sum = sum * a + s_sum[w] * b;
+      acc = acc * a + s_acc[w][lane % kLanes] * b;
+      top = peak;
     }
   }
   // no key seen, or none with any weight: the sum is empty
@@ -424,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const Params p) {
   if (lane < kLanes) {
     Q *o = (Q *)p.out + (int64_t)token * p.o_st + (int64_t)q_head * p.o_sh + lane * kPer;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) store(o + j, none ? 0.f : acc[j] * inv);
+    for (int j = 0; j < kPer; ++j) o[j] = (Q)(none ? 0.f : acc[j] * inv);
   }
   if (lane == 0) p.lse[item] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
@@ -556,7 +570,7 @@ void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim,
   n = n < ceil_div(keys, 1024) ? ceil_div(keys, 1024) : n;
   const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
   n = n > fit ? fit : n;
-  n = n > kMaxSlots ? kMaxSlots : n < 1 ? 1 : n;
+  n = n > kMaxChunks ? kMaxChunks : n < 1 ? 1 : n;
   chunk = (int)(ceil_div(ceil_div(keys, n), 64) * 64);
   if (chunk < 64) chunk = 64;
   slots = (int)ceil_div(keys, chunk);
@@ -569,21 +583,26 @@ void split_wide(int64_t keys, int64_t items_per_chunk, int64_t queries, int head
   int64_t n = ceil_div(4 * (int64_t)cu_count(), items_per_chunk > 0 ? items_per_chunk : 1);
   const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
   n = n > fit ? fit : n;
-  n = n > kMaxSlots ? kMaxSlots : n < 1 ? 1 : n;
+  n = n > kMaxChunks ? kMaxChunks : n < 1 ? 1 : n;
   const int64_t each = ceil_div(ceil_div(keys, n), 64) * 64;
   chunk = (int)(each < 512 ? 512 : each > (1 << 30) ? INT32_MAX : each);
   slots = (int)ceil_div(keys, chunk);
   if (slots < 1) slots = 1;
 }
 
+// The narrow kernel's resident waves of a compute unit and keys of a step.
+struct Shape {
+  int waves, keys;
+};
 template <class T>
-int narrow_waves(int head_dim) {
-  return head_dim == 32 ? Narrow<T, 32>::kResident : head_dim == 64 ? Narrow<T, 64>::kResident
-         : head_dim == 128 ? Narrow<T, 128>::kResident : Narrow<T, 256>::kResident;
+Shape narrow_shape(int head_dim) {
+  auto of = [](auto n) { return Shape{decltype(n)::kResident, decltype(n)::kKeys}; };
+  return head_dim == 32 ? of(Narrow<T, 32>{}) : head_dim == 64 ? of(Narrow<T, 64>{})
+         : head_dim == 128 ? of(Narrow<T, 128>{}) : of(Narrow<T, 256>{});
 }
-int narrow_waves(int kv_dtype, int head_dim) {
-  return kv_dtype == EKV_F32 ? narrow_waves<F32>(head_dim) : kv_dtype == EKV_FP8_E4M3 ? narrow_waves<FP8>(head_dim)
-                                                                                     : narrow_waves<BF16>(head_dim);
+Shape narrow_shape(int kv_dtype, int head_dim) {
+  return kv_dtype == EKV_F32 ? narrow_shape<F32>(head_dim) : kv_dtype == EKV_FP8_E4M3 ? narrow_shape<FP8>(head_dim)
+                                                                                     : narrow_shape<BF16>(head_dim);
 }
 
 void plan(Params &p, int head_dim, int kv_dtype) {
@@ -604,12 +623,13 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   if (p.wide_own) {
     split_wide(own_keys + prefix_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
   } else {
-    // waves that a (KV head, tile) has: all together those that the chip holds, and no more than there are units
-    const int64_t each = (int64_t)p.kv_heads * p.tiles_own, units = p.rows * ceil_div(own_keys, kUnit);
-    int64_t share = (int64_t)cu_count() * narrow_waves(kv_dtype, head_dim) / each;
-    share = share > units ? units : share;
+    // waves that a (KV head, tile) has: all together those that the chip holds, and no more than there are steps
+    const Shape shape = narrow_shape(kv_dtype, head_dim);
+    const int64_t each = (int64_t)p.kv_heads * p.tiles_own, row_steps = ceil_div(own_keys, shape.keys);
+    int64_t share = (int64_t)cu_count() * shape.waves / each;
+    share = share > p.rows * row_steps ? p.rows * row_steps : share;
     p.share = (int)(share < 1 ? 1 : share);
-    int64_t slots = ceil_div(own_keys, kUnit);
+    int64_t slots = row_steps + 2;
     const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
     slots = slots > fit ? fit : slots;
     p.s_own = (int)(slots > kMaxSlots ? kMaxSlots : slots < 3 ? 3 : slots);
@@ -644,6 +664,8 @@ size_t workspace_bytes(const Params &p, int head_dim) {
          (size_t)p.rows * 4 + 16;
 }
 
+constexpr int kJoinWide = 1024;  // up to so many queries, 8 waves join the partial results of one
+
 template <class T, int D>
 int launch(const Params &p, hipStream_t stream) {
   int rc = EKV_OK;
@@ -657,8 +679,12 @@ int launch(const Params &p, hipStream_t stream) {
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
     }
     if (rc == EKV_OK && !p.direct) {
-      const unsigned joins = (unsigned)ceil_div((int64_t)p.tokens * p.q_heads, kThreads / kWave);
-      hipLaunchKernelGGL((combine_kernel<typename T::Query, D>), dim3(joins), dim3(kThreads), 0, stream, p);
+      const int64_t queries = (int64_t)p.tokens * p.q_heads;
+      typedef typename T::Query Q;
+      if (queries <= kJoinWide)
+        hipLaunchKernelGGL((combine_kernel<Q, D, 8>), dim3((unsigned)queries), dim3(8 * kWave), 0, stream, p);
+      else
+        hipLaunchKernelGGL((combine_kernel<Q, D, 1>), dim3((unsigned)ceil_div(queries, 4)), dim3(kThreads), 0, stream, p);
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention combine launch");
     }
   }

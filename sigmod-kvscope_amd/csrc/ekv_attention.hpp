@@ -23,7 +23,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRowsPerTile = 16;  // query rows of one narrow tile (the matrix instruction's columns)
 constexpr int kWideRows = 64;     // from so many query rows a set of keys on, the wide kernel
 constexpr int kMostKeys = INT32_MAX - 4095;  // of a table row: a step past its last key is still an int
-constexpr int kMaxSlots = 64;     // partial results a query row can have from its own pages, and from its prefix
+constexpr int kMaxSlots = 128;    // partial results a query row can have from the equal shares of its own keys
+constexpr int kMaxChunks = 64;    // and from chunks of keys
 
 struct Params {
   const char *q;

@@ -140,3 +140,12 @@ def test_python_checks_come_before_the_device():
     evict("budget", budget=lens.long())
     evict("seen", seen=lens.repeat(2))
     evict("new_scores", new_scores=scores[0])
+
+
+def test_attention_tables_of_the_most_keys():
+    a = attention(width=(2**31 - 4096) // 16, block_size=16, table_stride=1 << 28)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ekv_hip.call("ekv_prefix_attention", ctypes.addressof(a), P, 1 << 40, 0)
+    a = attention(width=(2**31 - 4096) // 16 - 1, block_size=16, table_stride=1 << 28)
+    with pytest.raises(ValueError, match="workspace"):
+        ekv_hip.call("ekv_prefix_attention", ctypes.addressof(a), P, 0, 0)
