@@ -15,8 +15,6 @@
 namespace ekv {
 namespace attn {
 
-__host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // What one wave works on.
 struct Segment : Range {
   int first, rows;  // first token, query rows (tokens * group)
@@ -689,6 +687,7 @@ int launch(const Params &p, hipStream_t stream) {
     }
   }
   if (rc != EKV_OK || p.scores == nullptr || p.width == 0) return rc;
+  if (p.wide_own) return wide_weights(p, T::kType, D, stream);
   const int64_t capacity = (int64_t)p.width * p.block_size, segments = (int64_t)p.rows * p.kv_heads;
   if (p.logits != nullptr) {
     const int pieces = (int)ceil_div(capacity, 4 * kThreads);
@@ -782,7 +781,8 @@ int fill(const ekv_attention_t *a, Params &p) {
   if (p.waves_own + (p.wide_pre ? 0 : p.items_pre) >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
       (p.wide_pre && p.items_pre >= (1ll << 24)) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
-      (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >= (1ll << 26) - 64))
+      (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >=
+                                  (p.wide_own ? 1ll << 24 : (1ll << 26) - 64)))
     return fail(EKV_EINVAL, "%s: %d rows of %d blocks and %d tokens of %d heads pass the threads of a launch", who,
                 p.rows, p.width, p.tokens, p.q_heads);
   return EKV_OK;

@@ -324,6 +324,10 @@ __device__ __forceinline__ bool find_tile(const Params &p, int index, int rows, 
 // The wide kernel (16-bit and fp8 keys): query rows of its tiles, and the launch over the own keys or the prefixes.
 int wide_tile_rows();
 int wide_attention(const Params &p, int kv_dtype, int head_dim, bool own, hipStream_t stream);
+// The running weights where the own keys went through it.
+int wide_weights(const Params &p, int kv_dtype, int head_dim, hipStream_t stream);
+
+__host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace attn
 }  // namespace ekv

@@ -288,6 +288,144 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
   attend_wide<T, D>(p, s, lds);
 }
 
+// -- the running weights of prompt chunks ----------------------------------------------------------------
+//
+// A workgroup per (row, KV head, 64 keys).  The keys stay in registers as the matrix instruction's rows, the query
+// rows pass by in tiles of 32, wave after wave: S^T = K Q^T again, weights exp2(s - lse), and each lane adds up its
+// keys' weights over the queries of its column.  Columns, then waves are summed in one order at the end.  A tile of
+// queries is read from L2 once per 64 keys, a tile ahead of its use.  Measured: 777 queries of 7 heads a KV head
+// against up to 2047 keys, three rows of 4 KV heads of 64: 53 us (289 us in tiles of 16 query rows, a wave to 64 keys).
+constexpr int kWeighWaves = 4;
+constexpr int kWeighKeys = 64;
+
+template <class T, int D>
+__global__ __launch_bounds__(kWeighWaves *kWave, (D == 256 ? 1 : 2)) void weigh_wide_kernel(const Params p, int pieces) {
+  typedef typename T::Half H;
+  constexpr int KT = kWeighKeys / 32, C = D / 16;
+  __shared__ float s_total[kWeighWaves][kWeighKeys];
+  const uint32_t block = blockIdx.x;
+  const int head = (int)(block % p.kv_heads), piece = (int)(block / p.kv_heads % pieces);
+  const int row = (int)(block / p.kv_heads / pieces), begin = piece * kWeighKeys;
+  const int len = row_length(p, row), end = min(begin + kWeighKeys, len);
+  if (begin >= end) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = lane_id(), half = lane / 32, n = lane % 32;
+  const RowQueries t = row_queries(p, row);
+  const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
+  const int32_t *table = p.table + (int64_t)row * p.table_stride;
+  const int at = begin + lane;
+  int page = -1;
+  if (at < end) page = table[page_of(p, at)];
+  const bool good = (uint32_t)page < (uint64_t)p.blocks;
+  const uint64_t ok = __ballot(good);
+  const int64_t off = ((int64_t)(good ? page : 0) * p.st_block + (int64_t)(good ? at - page_of(p, at) * p.block_size : 0) * p.st_pos +
+                       (int64_t)head * p.st_head) * T::kBytes;
+  const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
+  u32x4 key[KT][C];
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    const char *from = p.k + (int64_t)(((uint64_t)(uint32_t)__shfl(hi, 32 * k + n) << 32) | (uint32_t)__shfl(lo, 32 * k + n));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if constexpr (T::kBytes == 1) {
+        const u32x2 x = *as_global((const u32x2 *)(from + (2 * c + half) * 8));
+        key[k][c] = widen(x[0], x[1]);
+      } else {
+        key[k][c] = *as_global((const u32x4 *)(from + (2 * c + half) * 16));
+      }
+    }
+  }
+  struct Queries {
+    u32x4 q[C];
+    float lse2;  // +inf where the query sees nothing or is none: its weights are 0
+    int limit;   // it sees keys below this
+  };
+  auto fetch = [&](Queries &x, int m0) {
+    const int m = m0 + n;
+    const bool live = m < rows;
+    const int i_q = live ? m / p.group : 0;
+    const int token = t.first + i_q, q_head = head * p.group + (live ? m - i_q * p.group : 0);
+    const char *from = p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * 2 + half * 16;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      x.q[c] = u32x4{0, 0, 0, 0};
+      if (live) x.q[c] = *as_global((const u32x4 *)(from + c * 32));
+    }
+    const float lse = live ? p.lse[(int64_t)token * p.q_heads + q_head] : -INFINITY;
+    x.lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    x.limit = lse == -INFINITY ? 0 : min(end, see + i_q);
+  };
+  float total[KT][16];
+#pragma unroll
+  for (int k = 0; k < KT; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total[k][i] = 0.f;
+  auto add = [&](const Queries &y) {
+    f32x16 x[KT];
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      x[k] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[k] = mfma32(key[k][c], y.q[c], x[k], H{});
+    }
+    if (~ok != 0 || !__all(y.limit >= begin + kWeighKeys)) {
+      const uint64_t mine = ok >> (4 * half);
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 32 * k + 8 * (i / 4) + i % 4;
+          const bool sees = (mine >> j & 1) != 0 && begin + j + 4 * half < y.limit;
+          total[k][i] += sees ? __builtin_amdgcn_exp2f(x[k][i] * p.scale2 - y.lse2) : 0.f;
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total[k][i] += __builtin_amdgcn_exp2f(x[k][i] * p.scale2 - y.lse2);
+    }
+  };
+  // queries before the first key see none of them
+  const int64_t before = (int64_t)max(0, begin - see + 1) * p.group;
+  constexpr int kStride = 32 * kWeighWaves;
+  int m0 = (int)min(before, (int64_t)rows) / 32 * 32 + 32 * wave;
+  Queries a, b;
+  if (m0 < rows) fetch(a, m0);
+  while (m0 < rows) {
+    if (m0 + kStride < rows) fetch(b, m0 + kStride);
+    add(a);
+    m0 += kStride;
+    if (m0 >= rows) break;
+    if (m0 + kStride < rows) fetch(a, m0 + kStride);
+    add(b);
+    m0 += kStride;
+  }
+#pragma unroll
+  for (int k = 0; k < KT; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = total[k][i];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) v += shfl_xor(v, d);
+      if (n == i) s_total[wave][32 * k + 8 * (i / 4) + 4 * half + i % 4] = v;
+    }
+  __syncthreads();
+  if (threadIdx.x >= kWeighKeys || at >= end) return;
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWeighWaves; ++w) v += s_total[w][lane];
+  float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
+  out[at] = p.decay * out[at] + v;
+}
+
+template <class T, int D>
+int launch_weigh(const Params &p, hipStream_t stream) {
+  const int pieces = (int)ceil_div((int64_t)p.width * p.block_size, kWeighKeys);
+  hipLaunchKernelGGL((weigh_wide_kernel<T, D>), dim3((unsigned)((int64_t)p.rows * pieces * p.kv_heads)),
+                     dim3(kWeighWaves * kWave), 0, stream, p, pieces);
+  return check_hip(hipGetLastError(), "ekv_prefix_attention weights launch");
+}
+
 template <class T, int D>
 int launch_wide(const Params &p, bool own, hipStream_t stream) {
   const unsigned grid = (unsigned)(own ? p.items_own : p.items_pre);
@@ -295,6 +433,16 @@ int launch_wide(const Params &p, bool own, hipStream_t stream) {
   if (own) hipLaunchKernelGGL((wide_kernel<T, D, true>), dim3(grid), dim3(Wide<T, D>::kThreads), 0, stream, p);
   else hipLaunchKernelGGL((wide_kernel<T, D, false>), dim3(grid), dim3(Wide<T, D>::kThreads), 0, stream, p);
   return check_hip(hipGetLastError(), "ekv_prefix_attention wide launch");
+}
+
+template <class T>
+int weigh_dim(const Params &p, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 32: return launch_weigh<T, 32>(p, stream);
+    case 64: return launch_weigh<T, 64>(p, stream);
+    case 128: return launch_weigh<T, 128>(p, stream);
+    default: return launch_weigh<T, 256>(p, stream);
+  }
 }
 
 template <class T>
@@ -314,6 +462,14 @@ int wide_attention(const Params &p, int kv_dtype, int head_dim, bool own, hipStr
     case EKV_F16: return wide_dim<F16>(p, head_dim, own, stream);
     case EKV_BF16: return wide_dim<BF16>(p, head_dim, own, stream);
     default: return wide_dim<FP8>(p, head_dim, own, stream);
+  }
+}
+
+int wide_weights(const Params &p, int kv_dtype, int head_dim, hipStream_t stream) {
+  switch (kv_dtype) {
+    case EKV_F16: return weigh_dim<F16>(p, head_dim, stream);
+    case EKV_BF16: return weigh_dim<BF16>(p, head_dim, stream);
+    default: return weigh_dim<FP8>(p, head_dim, stream);
   }
 }
 
