@@ -213,76 +213,6 @@ constexpr int kThreads = 256;
 // alone (128 rows of 512 to 8192 tokens: 427 us in chunks of 256 or 1024 keys against 358 us, 6.4 TB/s).  So the steps of
 // all rows, one row after the other, are one list; each (KV head, query tile) has `share` waves, and wave j of them
 // takes steps j T / share to (j + 1) T / share of the T, in at most kMaxSlots pieces a row.
-struct Share {
-  int64_t total;  // units of all rows
-  int share;      // waves that have some
-  // the wave that unit x is in
-  __device__ __forceinline__ int wave_of(int64_t x) const { return (int)(((x + 1) * share - 1) / total); }
-};
-
-template <int UNIT>
-__device__ __forceinline__ int row_units(const Params &p, int row) { return (row_length(p, row) + UNIT - 1) / UNIT; }
-
-// Every thread of the workgroup: the list's size, the waves that share it, and for wave w of the workgroup, number
-// w of `first` on of its head and tile, the row that its first unit is in and the units before that row.
-template <int WAVES, int UNIT>
-__device__ __forceinline__ Share share_out(const Params &p, int64_t first, int *start_row, int64_t *start_at) {
-  constexpr int kN = WAVES * kWave;
-  __shared__ int64_t s_sum[WAVES];
-  __shared__ int s_max[WAVES];
-  const int wave = threadIdx.x / kWave, per = (p.rows + kN - 1) / kN;
-  const int r0 = min((int)threadIdx.x * per, p.rows), r1 = min(r0 + per, p.rows);
-  int64_t mine = 0;
-  int longest = 0;
-  for (int r = r0; r < r1; ++r) {
-    const int n = row_units<UNIT>(p, r);
-    mine += n;
-    longest = max(longest, n);
-  }
-  int64_t inclusive = mine;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t other = __shfl_up(inclusive, d);
-    if (lane_id() >= d) inclusive += other;
-    longest = max(longest, __shfl_xor(longest, d));
-  }
-  if (lane_id() == kWave - 1) s_sum[wave] = inclusive;
-  if (lane_id() == 0) s_max[wave] = longest;
-  __syncthreads();
-  int64_t before = inclusive - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    before += w < wave ? s_sum[w] : 0;
-    total += s_sum[w];
-    longest = max(longest, s_max[w]);
-  }
-  Share s;
-  s.total = total;
-  int64_t share = min((int64_t)p.share, total);
-  // a row of u units meets at most u share / total + 2 waves
-  if (longest > 0) share = min(share, max((int64_t)1, total * (p.s_own - 2) / longest));
-  s.share = (int)share;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const int64_t j = (first + w) / ((int64_t)p.kv_heads * p.tiles_own);
-    if (j >= share) continue;
-    const int64_t x = j * total / share;
-    if (x < before || x >= before + mine) continue;
-    int64_t at = before;
-    for (int r = r0; r < r1; ++r) {
-      const int n = row_units<UNIT>(p, r);
-      if (x < at + n) {
-        start_row[w] = r;
-        start_at[w] = at;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  return s;
-}
-
 template <class T, int D>
 __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void narrow_kernel(const Params p) {
   using N = Narrow<T, D>;
@@ -291,7 +221,7 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
   __shared__ int64_t s_at[N::kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   char *mine = lds + wave * N::kBytes;
-  const int64_t shared = p.wide_pre ? 0 : ceil_div(p.items_pre, N::kWaves);  // the prefixes' items come first
+  const int64_t shared = ceil_div(p.items_pre, N::kWaves);  // the prefixes' items come first
   Segment s;
   if (blockIdx.x < shared) {
     const int64_t item = (int64_t)blockIdx.x * N::kWaves + wave;
@@ -299,8 +229,13 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
     return;
   }
   const int64_t first = (blockIdx.x - shared) * N::kWaves;
-  const Share share = share_out<N::kWaves, N::kKeys>(p, first, s_row, s_at);
   const int each = p.kv_heads * p.tiles_own;
+  const Share share = share_out<N::kWaves, N::kWaves>(
+      p.rows, p.share, 1, p.s_own, [&](int w) { return (first + w) / each; },
+      [&](int r, int64_t &steps) {
+        steps = (row_length(p, r) + N::kKeys - 1) / N::kKeys;
+        return steps;
+      }, s_row, s_at);
   const int j = (int)((first + wave) / each), part = (int)((first + wave) % each);
   if (j >= share.share) return;
   s.head = part % p.kv_heads;
@@ -309,18 +244,18 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
   s.plen = 0;
   int64_t at = (int64_t)j * share.total / share.share;
   const int64_t stop = (int64_t)(j + 1) * share.total / share.share;
-  s.row = __builtin_amdgcn_readfirstlane(s_row[wave]);
-  int64_t row_at = s_at[wave];  // the units before the row
+  s.row = uniform(s_row[wave]);
+  int64_t row_at = uniform(s_at[wave]);  // the units before the row
   while (true) {
-    const int len = row_length(p, s.row), units = (len + N::kKeys - 1) / N::kKeys;
+    const int len = uniform(row_length(p, s.row)), units = (len + N::kKeys - 1) / N::kKeys;
     if (units > 0) {
-      const int j0 = share.wave_of(row_at), j1 = share.wave_of(row_at + units - 1);
+      const int j0 = share.worker_of(row_at), j1 = share.worker_of(row_at + units - 1);
       if (part == 0 && j == j0 && lane_id() == 0) p.row_slots[s.row] = j1 - j0 + 1;
       const RowQueries t = row_queries(p, s.row);
       s.table = p.table + (int64_t)s.row * p.table_stride;
-      s.first = t.first;
-      s.rows = min(t.count, p.max_query) * p.group;
-      s.see = len - t.count + 1;
+      s.first = uniform(t.first);
+      s.rows = uniform(min(t.count, p.max_query) * p.group);
+      s.see = uniform(len - t.count + 1);
       s.slot = j - j0;
       const int u0 = (int)(at - row_at), u1 = (int)(min(stop, row_at + units) - row_at);
       s.begin = u0 * N::kKeys;
@@ -377,7 +312,8 @@ __global__ __launch_bounds__(W == 1 ? kThreads : W *kWave) void combine_kernel(c
       own = all > 0 ? (int)((all - 1) / p.chunk_own) + 1 : 0;
     } else {
       own = seen > 0 ? p.row_slots[row] : 0;
-      pre = n > 0 ? (n - 1) / p.chunk_pre + 1 : 0;
+      if (n > 0)
+        pre = p.wide_pre ? p.pre_slots[(int64_t)token * p.group + q_head % p.group] : (n - 1) / p.chunk_pre + 1;
     }
   }
   constexpr int kPer = D > 64 ? D / 64 : 1;
@@ -578,7 +514,7 @@ void split(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim,
 // The wide kernel's: a few workgroups for each that the chip holds, no chunk shorter than 512 keys (its
 // partial outputs, written and read again, are as much traffic as 64 keys and values).
 void split_wide(int64_t keys, int64_t items_per_chunk, int64_t queries, int head_dim, int &chunk, int &slots) {
-  int64_t n = ceil_div(4 * (int64_t)cu_count(), items_per_chunk > 0 ? items_per_chunk : 1);
+  int64_t n = ceil_div(2 * (int64_t)cu_count(), items_per_chunk > 0 ? items_per_chunk : 1);
   const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
   n = n > fit ? fit : n;
   n = n > kMaxChunks ? kMaxChunks : n < 1 ? 1 : n;
@@ -633,11 +569,19 @@ void plan(Params &p, int head_dim, int kv_dtype) {
     p.s_own = (int)(slots > kMaxSlots ? kMaxSlots : slots < 3 ? 3 : slots);
     p.waves_own = each * p.share;
     if (p.groups > 0) {
-      p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
-      const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
-      if (p.wide_pre) split_wide(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
-      else split(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
-      p.items_pre = items * p.s_pre;
+      if (p.wide_pre) {
+        // workgroups that a KV head has: all together those that the chip holds
+        const int64_t groups = (int64_t)cu_count() * wide_resident(head_dim) / p.kv_heads;
+        p.share_pre = (int)(groups < 1 ? 1 : groups);
+        const int64_t most = ceil_div(prefix_keys, 32) + 2;
+        int64_t limit = most > fit ? fit : most;
+        p.s_pre = (int)(limit > kMaxChunks ? kMaxChunks : limit < 3 ? 3 : limit);
+      } else {
+        p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
+        const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
+        split(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
+        p.items_pre = items * p.s_pre;
+      }
     }
   }
   p.items_own = p.wide_own ? own_items * p.s_own : 0;
@@ -659,7 +603,7 @@ size_t partial_bytes(const Params &p, int head_dim) {
 }
 size_t workspace_bytes(const Params &p, int head_dim) {
   return (partial_bytes(p, head_dim) + 15) / 16 * 16 + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4 +
-         (size_t)p.rows * 4 + 16;
+         (size_t)p.rows * 4 + (p.wide_pre ? (size_t)p.tokens * p.group * 4 : 0) + 16;
 }
 
 constexpr int kJoinWide = 1024;  // up to so many queries, 8 waves join the partial results of one
@@ -670,8 +614,7 @@ int launch(const Params &p, hipStream_t stream) {
   if (p.tokens > 0) {
     if (p.wide_own || p.wide_pre) rc = wide_attention(p, T::kType, D, p.wide_own, stream);
     using N = Narrow<T, D>;
-    const unsigned grid = p.wide_own ? 0 : (unsigned)((p.wide_pre ? 0 : ceil_div(p.items_pre, N::kWaves)) +
-                                                      ceil_div(p.waves_own, N::kWaves));
+    const unsigned grid = (unsigned)(ceil_div(p.items_pre, N::kWaves) + ceil_div(p.waves_own, N::kWaves));
     if (rc == EKV_OK && grid > 0) {
       hipLaunchKernelGGL((narrow_kernel<T, D>), dim3(grid), dim3(N::kThreads), 0, stream, p);
       rc = check_hip(hipGetLastError(), "ekv_prefix_attention launch");
@@ -778,8 +721,7 @@ int fill(const ekv_attention_t *a, Params &p) {
   p.decay = a->decay;
   plan(p, a->head_dim, a->kv_dtype);
   // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel, 256 an item of the wide one
-  if (p.waves_own + (p.wide_pre ? 0 : p.items_pre) >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
-      (p.wide_pre && p.items_pre >= (1ll << 24)) ||
+  if (p.waves_own + p.items_pre >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
       (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >=
                                   (p.wide_own ? 1ll << 24 : (1ll << 26) - 64)))
@@ -830,6 +772,7 @@ extern "C" int ekv_prefix_attention(const ekv_attention_t *a, void *workspace, s
   char *more = (char *)workspace + (attn::partial_bytes(p, a->head_dim) + 15) / 16 * 16;
   if (p.logit_rows > 0) p.logits = (float *)more;
   p.row_slots = (int32_t *)(more + (size_t)p.rows * p.kv_heads * p.logit_rows * p.logit_stride * 4);
+  p.pre_slots = p.row_slots + p.rows;
   hipStream_t s = (hipStream_t)stream;
   switch (a->kv_dtype) {
     case EKV_F32: return attn::launch_dim<attn::F32>(p, a->head_dim, s);

@@ -54,8 +54,10 @@ struct Params {
   float scale2, v_scale, decay;  // scale2: scale * k_scale * log2(e)
   int32_t *row_slots;  // [rows]: the slots that a row's own keys have partial results in (narrow kernel)
   // the split: at most s_own slots for the own keys (wide kernel: chunks of chunk_own keys; narrow kernel: the
-  // pieces of `share` waves a head and tile, waves_own in all), prefixes in s_pre chunks of chunk_pre
-  int share;
+  // pieces of `share` waves a head and tile, waves_own in all), prefixes in s_pre chunks of chunk_pre (wide
+  // kernel: in at most s_pre pieces of share_pre workgroups a head)
+  int32_t *pre_slots;  // [tokens * group]: the slots that a query row's prefix has partial results in (wide kernel)
+  int share, share_pre;
   int64_t waves_own;
   int chunk_own, s_own, tiles_own, chunk_pre, s_pre, tiles_pre;
   int tile_own, tile_pre;  // query rows of a tile
@@ -321,8 +323,88 @@ __device__ __forceinline__ bool find_tile(const Params &p, int index, int rows, 
   return false;
 }
 
+// -- equal shares -------------------------------------------------------------------------------------
+//
+// A list of work is the units of its entries (rows, groups), one entry after the other; `share` workers take a
+// stretch each, worker j units j total / share to (j + 1) total / share.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+struct Share {
+  int64_t total;
+  int share;
+  // the worker that unit x is with
+  __device__ __forceinline__ int worker_of(int64_t x) const { return (int)(((x + 1) * share - 1) / total); }
+};
+
+// Every thread of the workgroup: the list's size, the workers that share it (at most `workers`, each with `least`
+// units, and so many that a run of units that must not be cut into more than `slots` pieces is not), and for each of
+// this workgroup's WORKERS workers, number worker(w) of all, the entry that its first unit is in and the units before
+// that entry.  size(entry, run): its units, and the longest run in it.
+template <int WAVES, int WORKERS, class Worker, class Size>
+__device__ __forceinline__ Share share_out(int entries, int workers, int least, int slots, Worker worker, Size size,
+                                           int *start_entry, int64_t *start_at) {
+  constexpr int kN = WAVES * kWave;
+  __shared__ int64_t s_sum[WAVES], s_max[WAVES];
+  const int wave = threadIdx.x / kWave, per = (entries + kN - 1) / kN;
+  const int e0 = min((int)threadIdx.x * per, entries), e1 = min(e0 + per, entries);
+  int64_t mine = 0, longest = 0;
+  for (int e = e0; e < e1; ++e) {
+    int64_t run;
+    mine += size(e, run);
+    longest = max(longest, run);
+  }
+  int64_t inclusive = mine;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t other = __shfl_up(inclusive, d);
+    if (lane_id() >= d) inclusive += other;
+    longest = max(longest, (int64_t)__shfl_xor(longest, d));
+  }
+  if (lane_id() == kWave - 1) s_sum[wave] = inclusive;
+  if (lane_id() == 0) s_max[wave] = longest;
+  __syncthreads();
+  int64_t before = inclusive - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    before += w < wave ? s_sum[w] : 0;
+    total += s_sum[w];
+    longest = max(longest, s_max[w]);
+  }
+  int64_t share = min((int64_t)workers, (total + least - 1) / least);
+  // a run of u units meets at most u share / total + 2 workers
+  if (longest > 0) share = min(share, max((int64_t)1, total * (slots - 2) / longest));
+  Share s;
+  s.total = uniform(total);
+  s.share = uniform((int)share);
+#pragma unroll
+  for (int w = 0; w < WORKERS; ++w) {
+    const int64_t j = worker(w);
+    if (j >= share) continue;
+    const int64_t x = j * total / share;
+    if (x < before || x >= before + mine) continue;
+    int64_t at = before;
+    for (int e = e0; e < e1; ++e) {
+      int64_t run;
+      const int64_t n = size(e, run);
+      if (x < at + n) {
+        start_entry[w] = e;
+        start_at[w] = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  return s;
+}
+
 // The wide kernel (16-bit and fp8 keys): query rows of its tiles, and the launch over the own keys or the prefixes.
 int wide_tile_rows();
+int wide_resident(int head_dim);  // workgroups of a compute unit
 int wide_attention(const Params &p, int kv_dtype, int head_dim, bool own, hipStream_t stream);
 // The running weights where the own keys went through it.
 int wide_weights(const Params &p, int kv_dtype, int head_dim, hipStream_t stream);
