@@ -32,7 +32,7 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, S
   const RowQueries t = group_queries(p, g);
   s.table = p.ptable + (int64_t)g * p.ptable_stride;
   s.ptable = nullptr;
-  s.plen = 0;
+  s.plen = s.own = 0;
   s.row = -1;
   s.first = t.first;
   s.rows = t.count * p.group;
@@ -79,8 +79,8 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
   const int limit = live ? min(s.end, s.see + i_q) : 0;  // this lane's query sees keys below it
   const int every = min(s.end, s.see + s.m0 / p.group);  // and every query of the tile keys below this
 
-  typename N::Step stage;
-  if (s.begin < s.end) stage.look(p, s, s.begin);
+  typedef typename N::Step St;
+  int page = s.begin < s.end ? St::look(p, s, s.begin) : -1;
   u32x4 q[QP];
 #pragma unroll
   for (int c = 0; c < QP; ++c) {
@@ -88,15 +88,20 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
     if (live)
       q[c] = *as_global((const u32x4 *)(p.q + ((int64_t)token * p.q_st + (int64_t)q_head * p.q_sh) * E + (4 * c + g) * 16));
   }
+  typename St::Rows keys, vals;
+  uint64_t coming = 0;  // the keys of the step on its way that are there
   if (s.begin < s.end) {
-    stage.load(p, s, s.begin);
-    stage.look(p, s, s.begin + N::kKeys);
+    coming = St::there(p, page);
+    const int64_t place = St::place(p, s, s.begin, page);
+    St::load(p, place, p.k, keys);
+    St::load(p, place, p.v, vals);
+    page = St::look(p, s, s.begin + N::kKeys);
   }
 
   int key_off[QP];
 #pragma unroll
   for (int c = 0; c < QP; ++c) key_off[c] = L::key_at(n, 4 * c + g);
-  const char *values = lds + N::Step::kTile;
+  const char *values = lds + St::kTile;
   float *logits = nullptr;  // of this lane's query row
   if (p.logits != nullptr && s.row >= 0 && live)
     logits = p.logits + (((int64_t)s.row * p.kv_heads + s.head) * p.logit_rows + m) * p.logit_stride;
@@ -107,12 +112,16 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
   float top = -INFINITY, sum = 0.f;
 
   for (int base = s.begin; base < s.end; base += N::kKeys) {
-    const uint64_t ok = stage.ok;
-    stage.store(lds);
+    const uint64_t ok = coming;
+    St::store_keys(keys, lds);
+    St::store_values(vals, ok, lds + St::kTile);
     asm volatile("" ::: "memory");  // the lanes of the wave read what others wrote, in order
     if (base + N::kKeys < s.end) {
-      stage.load(p, s, base + N::kKeys);
-      stage.look(p, s, base + 2 * N::kKeys);
+      coming = St::there(p, page);
+      const int64_t place = St::place(p, s, base + N::kKeys, page);
+      St::load(p, place, p.k, keys);
+      St::load(p, place, p.v, vals);
+      page = St::look(p, s, base + 2 * N::kKeys);
     }
     f32x4 x[KT];
 #pragma unroll
@@ -241,7 +250,7 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
   s.head = part % p.kv_heads;
   s.m0 = part / p.kv_heads * kRowsPerTile;
   s.ptable = nullptr;
-  s.plen = 0;
+  s.plen = s.own = 0;
   int64_t at = (int64_t)j * share.total / share.share;
   const int64_t stop = (int64_t)(j + 1) * share.total / share.share;
   s.row = uniform(s_row[wave]);
@@ -308,7 +317,7 @@ __global__ __launch_bounds__(W == 1 ? kThreads : W *kWave) void combine_kernel(c
     const int g = group_of(p, row);
     const int n = g >= 0 ? group_length(p, g) : 0;
     if (p.wide_own) {
-      const int64_t all = (int64_t)n + max(seen, 0);
+      const int64_t all = seen > 0 ? (int64_t)own_begin(n) + seen : n;
       own = all > 0 ? (int)((all - 1) / p.chunk_own) + 1 : 0;
     } else {
       own = seen > 0 ? p.row_slots[row] : 0;
@@ -540,10 +549,11 @@ Shape narrow_shape(int kv_dtype, int head_dim) {
 }
 
 void plan(Params &p, int head_dim, int kv_dtype) {
+  p.whole = p.block_size % 16 == 0 && p.st_pos >= 0 && p.st_pos < 1 << 24;
   const int64_t queries = (int64_t)p.tokens * p.q_heads;
   const int64_t own_rows = (int64_t)p.max_query * p.group;
   const bool half = kv_dtype != EKV_F32;
-  const int64_t axis = (int64_t)(p.width + (p.groups > 0 ? p.pwidth : 0)) * p.block_size;
+  const int64_t axis = (int64_t)(p.width + (p.groups > 0 ? p.pwidth : 0)) * p.block_size + 64;
   p.wide_own = half && own_rows >= kWideRows && axis < (1 << 30);
   p.wide_pre = half && !p.wide_own && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= kWideRows;
   p.tile_own = p.wide_own ? wide_tile_rows() : kRowsPerTile;
@@ -555,7 +565,7 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   p.s_pre = 0;
   p.chunk_pre = 64;
   if (p.wide_own) {
-    split_wide(own_keys + prefix_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
+    split_wide(own_begin(prefix_keys) + own_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
   } else {
     // waves that a (KV head, tile) has: all together those that the chip holds, and no more than there are steps
     const Shape shape = narrow_shape(kv_dtype, head_dim);

@@ -66,6 +66,7 @@ struct Params {
   // the prefix's own); wide_pre: the prefixes do.  direct: one chunk holds everything a query sees, so the
   // wide kernel writes the result.
   bool wide_own, wide_pre, direct;
+  bool whole;  // 16 slots from a multiple of 16 on lie in one page, at offsets below 2^31
 };
 
 __device__ __forceinline__ int page_of(const Params &p, int pos) {
@@ -167,81 +168,130 @@ struct Lds {
   }
 };
 
-// The keys that a wave or workgroup reads: numbered along one axis, a prefix's first, of it [begin, end).
+// The keys that a wave or workgroup reads, [begin, end) of one axis: a prefix's first, the own ones from `own` on, a
+// multiple of 64 (between the two there are none), so that 16 keys from a multiple of 16 on are of one page where the
+// block size is a multiple of 16.
 struct Range {
   const int32_t *ptable, *table;
-  int plen, begin, end, head;
+  int plen, own, begin, end, head;
 };
+__host__ __device__ __forceinline__ int own_begin(int plen) { return (plen + 63) / 64 * 64; }
 
 // One step of KEYS keys and values on its way from memory through registers to LDS.  Loads take whole rows, 16
-// bytes a lane, the form that memory serves fastest.  The pages come one step ahead of the rows, a lookup a lane:
+// bytes a lane, the form that memory serves fastest.  The pages come a step ahead of the rows, a lookup a lane:
 // loads return in order, so a lookup right before its rows would wait for every row ahead of it.
 template <class T, int D, int KEYS, int THREADS>
 struct Stage {
   static constexpr int kPieces = D * T::kBytes / 16;  // 16-byte pieces of a row in memory
   static constexpr int kAll = KEYS * kPieces;
   static constexpr int kLoads = (kAll + THREADS - 1) / THREADS;  // of a thread, for K and for V
-  static constexpr int kTile = KEYS * Lds<T, D>::kRow;           // LDS bytes of K, and of V behind it
-  int page;     // of this lane's key of the step after the next load
-  uint64_t ok;  // the keys of the loaded step that are there (KEYS = 32: twice)
-  u32x4 k[kLoads], v[kLoads];
+  static constexpr int kTile = KEYS * Lds<T, D>::kRow;           // LDS bytes of K, and of V
+  typedef u32x4 Rows[kLoads];
 
   // the thread's i-th piece, and whether there is one (KEYS * pieces is a multiple of 64, so a wave agrees)
-  __device__ __forceinline__ bool piece(int i, int &row, int &col) const {
+  __device__ static __forceinline__ bool piece(int i, int &row, int &col) {
     const int at = (THREADS == kWave ? lane_id() : (int)threadIdx.x) + i * THREADS;
     row = at / kPieces;
     col = at % kPieces;
     return kAll % THREADS == 0 || at < kAll;
   }
-  __device__ __forceinline__ void look(const Params &p, const Range &s, int base) {
+  // the page of this lane's key of the step at `base`; -1: there is none
+  __device__ static __forceinline__ int look(const Params &p, const Range &s, int base) {
     const int at = base + lane_id() % KEYS;
-    page = -1;
-    if (at < s.end) {
+    int page = -1;
+    if (at < s.end && (at < s.plen || at >= s.own)) {
       const bool shared = at < s.plen;
-      page = (shared ? s.ptable : s.table)[page_of(p, shared ? at : at - s.plen)];
+      page = (shared ? s.ptable : s.table)[page_of(p, shared ? at : at - s.own)];
+    }
+    return page;
+  }
+  // the keys of a step that are there (KEYS below 64: again and again)
+  __device__ static __forceinline__ uint64_t there(const Params &p, int page) {
+    return __ballot((uint32_t)page < (uint64_t)p.blocks);
+  }
+  // where this lane's key of the step at `base` lies, in bytes; page 0's first slot for one that is not there
+  __device__ static __forceinline__ int64_t place(const Params &p, const Range &s, int base, int page) {
+    const int at = base + lane_id() % KEYS;
+    const bool good = (uint32_t)page < (uint64_t)p.blocks;
+    const int pos = good ? at < s.plen ? at : at - s.own : 0;
+    return ((good ? page : 0) * p.st_block + (pos - page_of(p, pos) * p.block_size) * p.st_pos + s.head * p.st_head) * T::kBytes;
+  }
+  // Where the rows of one load are of one page (whole): its first row's place, a lane's offset from it the same in
+  // every load.
+  static constexpr bool kScalar = kWave / kPieces <= 16;
+  __device__ static __forceinline__ int first_row(int i) {
+    const int wave = THREADS == kWave ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    return (wave * kWave + i * THREADS) / kPieces;
+  }
+  __device__ static __forceinline__ int64_t place_of(int64_t place, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)place, lane);
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(place >> 32), lane) << 32 | lo);
+  }
+  __device__ static __forceinline__ uint32_t lane_offset(const Params &p) {
+    return (uint32_t)(lane_id() / kPieces) * (uint32_t)(p.st_pos * T::kBytes);
+  }
+  __device__ static __forceinline__ int64_t shuffled(int64_t place, int lane) {
+    const uint32_t lo = __shfl((int)(uint32_t)place, lane);
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)(place >> 32), lane) << 32 | lo);
+  }
+  // the rows at `place`, keys (from p.k) or values (from p.v)
+  __device__ static __forceinline__ void load(const Params &p, int64_t place, const char *from, Rows &to) {
+    if (kScalar && p.whole) {
+      const uint32_t off = lane_offset(p) + lane_id() % kPieces * 16;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int first = first_row(i);
+        if (kAll % THREADS != 0 && first >= KEYS) break;
+        to[i] = fetch(from + place_of(place, first) + off);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        int row, col;
+        if (!piece(i, row, col)) break;
+        to[i] = fetch(from + shuffled(place, row) + col * 16);
+      }
     }
   }
-  __device__ __forceinline__ void load(const Params &p, const Range &s, int base) {
-    const int at = base + lane_id() % KEYS;
-    const int pos = at < s.plen ? at : at - s.plen;
-    const bool good = at < s.end && (uint32_t)page < (uint64_t)p.blocks;
-    ok = __ballot(good);
-    const int in_page = good ? pos - page_of(p, pos) * p.block_size : 0;
-    const int64_t off = ((int64_t)(good ? page : 0) * p.st_block + (int64_t)in_page * p.st_pos +
-                         (int64_t)s.head * p.st_head) * T::kBytes;
-    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
+  __device__ static __forceinline__ u32x4 fetch(const char *from) {
+    // a wave's rows are read once: the stream leaves the caches to others (2.3 GB of rows: 427 us, not 455)
+    if constexpr (THREADS == kWave) return __builtin_nontemporal_load(as_global((const u32x4 *)from));
+    else return *as_global((const u32x4 *)from);
+  }
+  __device__ static __forceinline__ void store_keys(const Rows &k, char *keys) {
+    using L = Lds<T, D>;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       int row, col;
       if (!piece(i, row, col)) break;
-      const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl(hi, row) << 32) | (uint32_t)__shfl(lo, row)) + col * 16;
-      if constexpr (THREADS == kWave) {  // read once: the stream leaves the caches to others
-        k[i] = __builtin_nontemporal_load(as_global((const u32x4 *)(p.k + from)));
-        v[i] = __builtin_nontemporal_load(as_global((const u32x4 *)(p.v + from)));
+      if constexpr (T::kBytes == 1) {
+        *(u32x4 *)(keys + L::key_at(row, 2 * col)) = widen(k[i][0], k[i][1]);
+        *(u32x4 *)(keys + L::key_at(row, 2 * col + 1)) = widen(k[i][2], k[i][3]);
       } else {
-        k[i] = *as_global((const u32x4 *)(p.k + from));
-        v[i] = *as_global((const u32x4 *)(p.v + from));
+        *(u32x4 *)(keys + L::key_at(row, col)) = k[i];
       }
     }
   }
   // the values of keys that are not there as 0 (0 * NaN is no zero)
-  __device__ __forceinline__ void store(char *keys) const {
+  __device__ static __forceinline__ void store_values(Rows &v, uint64_t ok, char *values) {
     using L = Lds<T, D>;
-    char *values = keys + kTile;
+    if (ok != ~0ull) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        int row, col;
+        if (!piece(i, row, col)) break;
+        if (!(ok >> row & 1)) v[i] = u32x4{0, 0, 0, 0};
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       int row, col;
       if (!piece(i, row, col)) break;
-      u32x4 x = v[i];
-      if (~ok != 0 && !(ok >> row & 1)) x = u32x4{0, 0, 0, 0};
       if constexpr (T::kBytes == 1) {
-        *(u32x4 *)(keys + L::key_at(row, 2 * col)) = widen(k[i][0], k[i][1]);
-        *(u32x4 *)(keys + L::key_at(row, 2 * col + 1)) = widen(k[i][2], k[i][3]);
-        *(u32x4 *)(values + L::value_at(row, 32 * col)) = widen(x[0], x[1]);
-        *(u32x4 *)(values + L::value_at(row, 32 * col + 16)) = widen(x[2], x[3]);
+        *(u32x4 *)(values + L::value_at(row, 32 * col)) = widen(v[i][0], v[i][1]);
+        *(u32x4 *)(values + L::value_at(row, 32 * col + 16)) = widen(v[i][2], v[i][3]);
       } else {
-        *(u32x4 *)(keys + L::key_at(row, col)) = k[i];
-        *(u32x4 *)(values + L::value_at(row, 16 * col)) = x;
+        *(u32x4 *)(values + L::value_at(row, 16 * col)) = v[i];
       }
     }
   }

@@ -28,11 +28,77 @@ struct Wide {
   static constexpr int kTile = Step::kTile;
 };
 
+// One step's rows of 16-bit keys or values from memory straight to LDS, 1 KB an instruction: a lane's 16 bytes land at
+// 16 times its number, so which piece of its row a lane asks for makes the permutation.  This saves the 32 registers
+// that a step on its way would hold (with them the kernel spilled, and read the operands of one product at a time).
+template <class T, int D>
+struct Direct {
+  using W = Wide<T, D>;
+  using L = Lds<T, D>;
+  typedef typename W::Step St;
+  static constexpr int kPieces = W::kRow / 16;
+  static constexpr int kAll = W::kKeys * kPieces;
+  static constexpr int kLoads = (kAll + W::kThreads - 1) / W::kThreads;
+  // The instruction has no register to return, and waits are for all loads in flight, so the compiler need not know of
+  // it.  M0 holds the LDS address, which takes a wait state to arrive.
+  __device__ static __forceinline__ void fetch(uint32_t lds, const char *base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  }
+  __device__ static __forceinline__ void fetch(uint32_t lds, const char *from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+  }
+  // the byte of its row that a lane asks for in load i
+  template <bool VALUES>
+  __device__ static __forceinline__ uint32_t source(int i) {
+    const int row = St::first_row(i) + lane_id() / kPieces, at = lane_id() % kPieces;
+    return VALUES ? L::value_at(row, at * 16) - row * W::kRow : L::key_at(row, at) - row * W::kRow;
+  }
+  // The rows from row 16 on are permuted as the first 16, so the loads of rows 16 apart have one lane offset.
+  static constexpr int kStep = W::kThreads / kPieces;  // rows from a load to the next
+  static constexpr int kOffsets = kStep >= 16 ? 1 : 16 / kStep;
+  typedef uint32_t Offsets[kOffsets];
+  template <bool VALUES>
+  __device__ static __forceinline__ void offsets(const Params &p, Offsets &off) {
+#pragma unroll
+    for (int i = 0; i < kOffsets; ++i) off[i] = source<VALUES>(i) + (p.whole ? St::lane_offset(p) : 0);
+  }
+  __device__ static __forceinline__ void load(const Params &p, int64_t place, const char *from, const Offsets &off, char *tile) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)tile);
+    if (p.whole) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int first = St::first_row(i);
+        if (kAll % W::kThreads != 0 && first >= W::kKeys) break;
+        fetch(to + first * W::kRow, from + St::place_of(place, first), off[i % kOffsets]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int first = St::first_row(i);
+        if (kAll % W::kThreads != 0 && first >= W::kKeys) break;
+        fetch(to + first * W::kRow, from + St::shuffled(place, first + lane_id() / kPieces) + off[i % kOffsets]);
+      }
+    }
+  }
+  // the wave's rows of values that are not there become 0, once all of its loads have landed (0 * NaN is no zero)
+  __device__ static __forceinline__ void clear(uint64_t ok, char *values) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int first = St::first_row(i);
+      if (kAll % W::kThreads != 0 && first >= W::kKeys) break;
+      if (!(ok >> (first + lane / kPieces) & 1)) *(u32x4 *)(values + first * W::kRow + lane * 16) = u32x4{0, 0, 0, 0};
+    }
+  }
+};
+// every load of this wave has landed
+__device__ __forceinline__ void loads_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // What a workgroup works on.
 struct Item : Range {
   int first, rows, m0;  // first token, query rows, the tile's first one
   int slot;
-  int see;              // query token i sees keys below plen + see + i
+  int see;              // query token i sees keys below own + see + i
 };
 
 // Out 0 and lse -inf for the tokens [from, to) of KV head `head`.
@@ -77,10 +143,12 @@ __device__ __forceinline__ bool own_item(const Params &p, uint32_t index, Item &
     s.ptable = p.ptable + (int64_t)g * p.ptable_stride;
     s.plen = group_length(p, g);
   }
+  s.own = own_begin(s.plen);
   s.see = len - t.count + 1;
   const int last = (min(s.m0 + p.tile_own, s.rows) - 1) / p.group;
   const int64_t begin = (int64_t)s.slot * p.chunk_own;
-  s.end = (int)min(begin + p.chunk_own, (int64_t)s.plen + max(0, min(len, s.see + last)));
+  const int seen = min(len, s.see + last);
+  s.end = (int)min(begin + p.chunk_own, (int64_t)(seen > 0 ? s.own + seen : s.plen));
   s.begin = (int)min(begin, (int64_t)INT32_MAX);
   return s.begin < s.end || p.direct;
 }
@@ -114,10 +182,10 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
   const int i_q = live ? m / p.group : 0;
   const int token = s.first + i_q, q_head = s.head * p.group + (live ? m - i_q * p.group : 0);
   const bool any = w0 < s.rows;
-  const int limit = live ? min(s.end, s.plen + max(0, s.see + i_q)) : 0;  // this lane's query sees keys below it
-  const int every = min(s.end, s.plen + max(0, s.see + w0 / p.group));    // and every query of the wave keys below this
+  const int limit = live ? min(s.end, s.own + max(0, s.see + i_q)) : 0;  // this lane's query sees keys below it
+  const int every = min(s.end, s.own + max(0, s.see + w0 / p.group));    // and every query of the wave keys below this
   const int last_row = min(w0 + 31, s.rows - 1);
-  const int most = any ? min(s.end, s.plen + max(0, s.see + last_row / p.group)) : 0;  // none sees keys from here on
+  const int most = any ? min(s.end, s.own + max(0, s.see + last_row / p.group)) : 0;  // none sees keys from here on
 
   // a negative scale turns the query's sign; the smallest one keeps a masked logit at -inf where scale is 0
   const float scale2 = fmaxf(fabsf(p.scale2), 0x1p-126f);
@@ -145,33 +213,76 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float top = -INFINITY, sum = 0.f;
 
-  typename W::Step stage;
-  uint64_t ok = 0;
+  // The softmax of a step's logits runs beside the next step's products, so keys are a step ahead of values: step t
+  // has its logits already, stores keys t + 2 over keys t, and values t + 1 over values t - 1.
+  typedef typename W::Step St;
+  typedef Direct<T, D> Di;
+  constexpr bool kDirect = T::kBytes == 2;  // fp8 rows pass through registers, where they are widened
+  typename St::Rows keys, vals;
+  f32x16 xa[KT], xb[KT];
+  uint64_t ok = 0, ok1 = 0;  // the keys of this step and the next that are there
+  int page2 = -1;     // the pages of the step after the next
+  int64_t place1 = 0;  // the rows of the next step
+  typename Di::Offsets key_from, value_from;
+  if constexpr (kDirect) {
+    Di::template offsets<false>(p, key_from);
+    Di::template offsets<true>(p, value_from);
+  }
+  auto products = [&](f32x16 *x, const char *buffer) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k) x[k] = f32x16{};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        x[k] = mfma32(*(const u32x4 *)(buffer + key_off[c] + k * 32 * W::kRow), q[c], x[k], H{});
+  };
   if (s.begin < s.end) {
-    stage.look(p, s, s.begin);
-    stage.load(p, s, s.begin);
-    stage.look(p, s, s.begin + W::kKeys);
-    ok = stage.ok;
-    stage.store(lds);
+    const int page = St::look(p, s, s.begin), page1 = St::look(p, s, s.begin + W::kKeys);
+    page2 = St::look(p, s, s.begin + 2 * W::kKeys);
+    ok = St::there(p, page);
+    ok1 = St::there(p, page1);
+    const int64_t place = St::place(p, s, s.begin, page);
+    place1 = St::place(p, s, s.begin + W::kKeys, page1);
+    if constexpr (kDirect) {
+      Di::load(p, place, p.k, key_from, lds);
+      Di::load(p, place, p.v, value_from, lds + W::kTile);
+      Di::load(p, place1, p.k, key_from, lds + 2 * W::kTile);
+      loads_landed();
+      if (ok != ~0ull) Di::clear(ok, lds + W::kTile);
+    } else {
+      St::load(p, place, p.k, keys);
+      St::load(p, place, p.v, vals);
+      St::store_keys(keys, lds);
+      St::load(p, place1, p.k, keys);
+      St::store_values(vals, ok, lds + W::kTile);
+      St::store_keys(keys, lds + 2 * W::kTile);
+    }
+    lds_barrier();
+    if (s.begin < most) products(xa, lds);
   }
 
-  auto step = [&](int base, char *buffer, char *next) {
+  // One step: x its logits, y the next one's; `even` holds K and V of its parity, `odd` the other's.
+  auto step = [&](int base, f32x16 *x, f32x16 *y, char *even, char *odd) {
     lds_barrier();
-    const bool more = base + W::kKeys < s.end;
+    const int next = base + W::kKeys;
+    const bool more = next < s.end;
+    uint64_t ok2 = 0;
     if (more) {
-      stage.load(p, s, base + W::kKeys);
-      stage.look(p, s, base + 2 * W::kKeys);
+      const int64_t place2 = St::place(p, s, next + W::kKeys, page2);
+      if constexpr (kDirect) {
+        Di::load(p, place1, p.v, value_from, odd + W::kTile);
+        Di::load(p, place2, p.k, key_from, even);
+      } else {
+        St::load(p, place1, p.v, vals);
+        St::load(p, place2, p.k, keys);
+      }
+      place1 = place2;
+      ok2 = St::there(p, page2);
+      page2 = St::look(p, s, next + 2 * W::kKeys);
     }
     if (base < most) {
-      f32x16 x[KT];
-#pragma unroll
-      for (int k = 0; k < KT; ++k) x[k] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-        for (int k = 0; k < KT; ++k)
-          x[k] = mfma32(*(const u32x4 *)(buffer + key_off[c] + k * 32 * W::kRow), q[c], x[k], H{});
-      if (base + W::kKeys > every || ~ok != 0) {
+      if (base + W::kKeys > every || ok != ~0ull) {
         const uint64_t mine = ok >> (4 * half);
 #pragma unroll
         for (int k = 0; k < KT; ++k)
@@ -196,6 +307,7 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
         top = peak;
       }
       const float ref = top == -INFINITY ? 0.f : top;
+      products(y, odd);  // past the last step from keys that nothing needs
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -210,23 +322,30 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
         for (int i = 0; i < 4; ++i) w[i] = pack2(x[t / 2][8 * (t % 2) + 2 * i], x[t / 2][8 * (t % 2) + 2 * i + 1], H{});
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const char *from = buffer + value_off[d] + t * 16 * W::kRow;
+          const char *from = even + value_off[d] + t * 16 * W::kRow;
           const u32x2 a = read_transposed(from), b = read_transposed(from + 8 * W::kRow);
           acc[d] = mfma32(u32x4{a[0], a[1], b[0], b[1]}, w, acc[d], H{});
         }
       }
     }
+    ok = ok1;
+    ok1 = ok2;
     if (more) {
-      ok = stage.ok;
-      stage.store(next);
+      if constexpr (kDirect) {
+        loads_landed();
+        if (ok != ~0ull) Di::clear(ok, odd + W::kTile);
+      } else {
+        St::store_keys(keys, even);
+        St::store_values(vals, ok, odd + W::kTile);
+      }
     }
   };
   char *other = lds + 2 * W::kTile;
   for (int base = s.begin; base < s.end;) {
-    step(base, lds, other);
+    step(base, xa, xb, lds, other);
     base += W::kKeys;
     if (base >= s.end) break;
-    step(base, other, lds);
+    step(base, xb, xa, other, lds);
     base += W::kKeys;
   }
 
@@ -293,7 +412,7 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
   s.see = 0;
   while (true) {
     const RowQueries t = group_queries(p, g);
-    s.plen = uniform(group_length(p, g));
+    s.plen = s.own = uniform(group_length(p, g));
     s.ptable = p.ptable + (int64_t)g * p.ptable_stride;
     s.first = uniform(t.first);
     s.rows = uniform(t.count * p.group);
