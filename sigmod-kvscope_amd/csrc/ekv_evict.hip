@@ -8,8 +8,13 @@
 // behind slot b moves into the k-th freed slot below it, and every other token stays where it is.  Sources
 // are at b or above and destinations below, so all moves can run at once, in place.
 //
-// Two kernels: select_kernel finds the survivors, lists the moves and writes scores, positions and lengths;
-// move_kernel copies the keys and values of the listed tokens.
+// select_kernel, a workgroup per (row, head), holds the row's scores and positions in registers (up to 16384
+// slots; longer rows pass through memory again and again, stream_kernel), finds the b-th by three passes over 11,
+// 11 and 10 bits of the keys, writes scores, positions and lengths, and copies the keys and values of the tokens
+// that move.  Where a few workgroups would copy much, they list the moves for move_kernel instead, which spreads
+// them over the chip.  Bound: the scores and positions, read and written once, and the rows that move.
+// Measured, 128 rows of 8 KV heads of 128, bf16: a few tokens past a budget of 4096 AAA us, half of 512 to 8192
+// tokens BBB us (78 and 321 us with eight passes through memory and a copy kernel behind them).
 #include "ekv_common.hpp"
 
 namespace ekv {
@@ -62,7 +67,290 @@ __device__ __forceinline__ void keep_in_place(const Params &p, int j, const floa
   if (new_positions != positions) new_positions[j] = positions[j];
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(const Params p) {
+// -- rows that registers hold ----------------------------------------------------------------------------
+
+// Of NT threads each has 4 consecutive slots of each of R rounds: slots 4 NT i + 4 tid + e.
+constexpr int kDigit = 2048;  // bins of a pass
+typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int Int4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t Row16 __attribute__((ext_vector_type(4)));
+
+// Exclusive sums of the threads' values in slot order (round by round, thread by thread).  Contains barriers.
+template <int NT, int R>
+__device__ __forceinline__ int ordered_scan(const int (&v)[R], int (&before)[R], int *scratch) {
+  constexpr int kWaves = NT / kWave;
+  static_assert(R * kWaves <= kWave, "a wave scans the waves' sums");
+  const int lane = lane_id(), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int inc = wave_inclusive_scan(v[i]);
+    before[i] = inc - v[i];
+    if (lane == kWave - 1) scratch[i * kWaves + wave] = inc;
+  }
+  __syncthreads();
+  // every wave scans the waves' sums of the rounds
+  const int sum = lane < R * kWaves ? scratch[lane] : 0;
+  const int inc = wave_inclusive_scan(sum);
+#pragma unroll
+  for (int i = 0; i < R; ++i) before[i] += __shfl(inc - sum, i * kWaves + wave);
+  __syncthreads();
+  return __builtin_amdgcn_readlane(inc, kWave - 1);
+}
+
+// The key and value rows of `count` moves that move(k) names, 16 bytes a lane, four moves in flight.  A slot whose
+// table entry is no page of the cache is not read or written.
+template <int THREADS, class Move>
+__device__ __forceinline__ void copy_rows(const Params &p, int row, int head, int count, int first, int stride, Move move) {
+  const int pieces = p.row_bytes / 16;  // a power of two, 2 to 64
+  const int per = THREADS / pieces, piece = threadIdx.x % pieces;
+  const int32_t *table = p.table + (int64_t)row * p.table_stride;
+  constexpr int kFlight = 4;
+  for (int k0 = first * per + threadIdx.x / pieces; k0 < count; k0 += stride * per * kFlight) {
+    int64_t src[kFlight], dst[kFlight];
+    bool good[kFlight];
+    int2 m[kFlight];
+    int a[kFlight], b[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int k = k0 + u * stride * per;
+      good[u] = k < count;
+      m[u] = good[u] ? move(k) : make_int2(0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      a[u] = table[page_of(p, m[u].x)];
+      b[u] = table[page_of(p, m[u].y)];
+    }
+    Row16 x[kFlight] = {}, y[kFlight] = {};
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      good[u] = good[u] && (uint32_t)a[u] < (uint64_t)p.blocks && (uint32_t)b[u] < (uint64_t)p.blocks;
+      const int from = m[u].x - page_of(p, m[u].x) * p.block_size, to = m[u].y - page_of(p, m[u].y) * p.block_size;
+      src[u] = (int64_t)a[u] * p.st_block + (int64_t)from * p.st_pos + head * p.st_head + piece * 16;
+      dst[u] = (int64_t)b[u] * p.st_block + (int64_t)to * p.st_pos + head * p.st_head + piece * 16;
+      if (good[u]) {
+        x[u] = *(const Row16 *)(p.k + src[u]);
+        y[u] = *(const Row16 *)(p.v + src[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      if (!good[u]) continue;
+      *(Row16 *)(p.k + dst[u]) = x[u];
+      *(Row16 *)(p.v + dst[u]) = y[u];
+    }
+  }
+}
+
+template <int NT, int R, bool COPY>
+__global__ __launch_bounds__(NT) void select_kernel(const Params p) {
+  constexpr int kRound = 4 * NT, kBinsEach = kDigit / NT;
+  typedef int Bins __attribute__((ext_vector_type(kBinsEach), aligned(4)));
+  __shared__ __attribute__((aligned(16))) int s_bins[kDigit];
+  __shared__ int s_scan[64];
+  __shared__ int s_pick[3];
+  __shared__ uint16_t s_from[R * kRound / 2], s_to[R * kRound / 2];  // the k-th survivor's slot, the k-th freed slot
+  const int segment = blockIdx.x, row = segment / p.heads, head = segment - row * p.heads;
+  const int tid = threadIdx.x;
+  const int n = min(max(p.lens[row], 0), p.capacity);
+  const int b = min(n, max(p.budget != nullptr ? p.budget[row] : p.fixed_budget, 0));
+  const int64_t newest = (int64_t)p.seen[row] - p.recent;
+  const float *scores = p.scores + (int64_t)row * p.s_row + (int64_t)head * p.s_head;
+  const int32_t *positions = p.positions + (int64_t)row * p.p_row + (int64_t)head * p.p_head;
+  float *new_scores = p.new_scores + (int64_t)row * p.ns_row + (int64_t)head * p.ns_head;
+  int32_t *new_positions = p.new_positions + (int64_t)row * p.np_row + (int64_t)head * p.np_head;
+
+  Float4 s[R];
+  Int4 at[R];
+  uint32_t keep = 0, safe = 0;  // bits 4 i + e
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int j = i * kRound + 4 * tid;
+    s[i] = Float4{0.f, 0.f, 0.f, 0.f};
+    at[i] = Int4{0, 0, 0, 0};
+    if (j + 4 <= n) {
+      s[i] = *(const Float4 *)(scores + j);
+      at[i] = *(const Int4 *)(positions + j);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < n) {
+          s[i][e] = scores[j + e];
+          at[i][e] = positions[j + e];
+        }
+    }
+  }
+  // Which of the thread's slots there are
+  auto there = [&](int i, int e) { return i * kRound + 4 * tid + e < n; };
+  if (b < n) {
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (there(i, e) && is_protected(p, at[i][e], newest)) {
+          safe |= 1u << (4 * i + e);
+          ++mine;
+        }
+    // the class that the cut falls into: the protected tokens if there are b of them or more
+    const int guarded = block_sum<NT, int>(mine, s_scan);
+    const bool among_safe = guarded >= b;
+    // the `want`-th highest key of that class, digit by digit; `equal` tokens have that very key
+    int want = among_safe ? b : b - guarded, equal = 0;
+    uint32_t cut = 0;
+    auto candidate = [&](int i, int e) { return there(i, e) && ((safe >> (4 * i + e) & 1) != 0) == among_safe; };
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      if (want == 0) break;  // b is 0, or the protected tokens are b
+      *(Bins *)(s_bins + kBinsEach * tid) = Bins{};
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (i * kRound >= n || !candidate(i, e)) continue;
+          const uint32_t key = order_of(s[i][e]);
+          if (pass == 0 || key >> (shift + bits) == cut >> (shift + bits)) atomicAdd(&s_bins[key >> shift & ((1u << bits) - 1)], 1);
+        }
+      __syncthreads();
+      // the threads' bins from the highest down: the one where the running count reaches `want`
+      const int low = kDigit - kBinsEach * (tid + 1);
+      const Bins c = *(const Bins *)(s_bins + low);
+      int total, sum = 0;
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) sum += c[e];
+      int before = block_exclusive_scan<NT>(sum, s_scan, total);
+#pragma unroll
+      for (int e = kBinsEach - 1; e >= 0; --e) {
+        if (before < want && before + c[e] >= want) {
+          s_pick[0] = low + e;
+          s_pick[1] = want - before;
+          s_pick[2] = c[e];
+        }
+        before += c[e];
+      }
+      __syncthreads();
+      cut |= (uint32_t)s_pick[0] << shift;
+      want = s_pick[1];
+      equal = s_pick[2];
+    }
+    // of the tokens equal to the cut the first `want` stay
+    uint32_t ties = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!there(i, e)) continue;
+        const uint32_t bit = 1u << (4 * i + e), key = order_of(s[i][e]);
+        if (!candidate(i, e)) keep |= safe & bit;
+        else if (equal > 0 && key >= cut) (key == cut ? ties : keep) |= bit;
+      }
+    int count[R], before[R];
+    if (want < equal) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) count[i] = __popc(ties >> (4 * i) & 15u);
+      ordered_scan<NT, R>(count, before, s_scan);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bit = 1u << (4 * i + e);
+          if ((ties & bit) != 0 && before[i]++ < want) keep |= bit;
+        }
+    } else {
+      keep |= ties;
+    }
+    // freed slots and survivors behind them, each in slot order
+    uint32_t hole = 0, late = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = i * kRound + 4 * tid + e;
+        const uint32_t bit = 1u << (4 * i + e);
+        if (j < b && !(keep & bit)) hole |= bit;
+        if (j >= b && (keep & bit) != 0) late |= bit;
+      }
+      count[i] = __popc(hole >> (4 * i) & 15u) | __popc(late >> (4 * i) & 15u) << 16;
+    }
+    const int moved = ordered_scan<NT, R>(count, before, s_scan) & 0xffff;  // as many survivors as freed slots
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      int free = before[i] & 0xffff, come = before[i] >> 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = i * kRound + 4 * tid + e;
+        if (hole >> (4 * i + e) & 1) s_to[free++] = (uint16_t)j;
+        if (late >> (4 * i + e) & 1) s_from[come++] = (uint16_t)j;
+      }
+    }
+    __syncthreads();
+    // survivors to their new slots, the others where they are, nothing behind the budget
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int j = i * kRound + 4 * tid;
+      int come = before[i] >> 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (late >> (4 * i + e) & 1) {
+          const int to = s_to[come++];
+          new_scores[to] = s[i][e];
+          new_positions[to] = at[i][e];
+        }
+      const uint32_t holes = hole >> (4 * i) & 15u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e >= b) {
+          s[i][e] = 0.f;
+          at[i][e] = -1;
+        }
+      if (j + 4 <= p.capacity && holes == 0) {
+        if (j >= b || new_scores != scores || j + 4 > b) *(Float4 *)(new_scores + j) = s[i];
+        if (j >= b || new_positions != positions || j + 4 > b) *(Int4 *)(new_positions + j) = at[i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < p.capacity && !(holes >> e & 1)) {
+            new_scores[j + e] = s[i][e];
+            new_positions[j + e] = at[i][e];
+          }
+      }
+    }
+    if (COPY) {
+      copy_rows<NT>(p, row, head, moved, 0, 1, [&](int k) { return make_int2(s_from[k], s_to[k]); });
+    } else {
+      int2 *moves = p.moves + (int64_t)segment * p.half;
+      for (int k = tid; k < moved; k += NT) moves[k] = make_int2(s_from[k], s_to[k]);
+      if (tid == 0) p.count[segment] = moved;
+    }
+  } else {  // everything stays
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int j = i * kRound + 4 * tid;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e >= n) at[i][e] = -1;  // the score is 0
+      if (j + 4 <= p.capacity) {
+        if (j + 4 > n || new_scores != scores) *(Float4 *)(new_scores + j) = s[i];
+        if (j + 4 > n || new_positions != positions) *(Int4 *)(new_positions + j) = at[i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < p.capacity) {
+            new_scores[j + e] = s[i][e];
+            new_positions[j + e] = at[i][e];
+          }
+      }
+    }
+    if (!COPY && tid == 0) p.count[segment] = 0;
+  }
+  if (tid == 0 && head == 0) p.new_lens[row] = b;
+}
+
+// -- longer rows -----------------------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kThreads) void stream_kernel(const Params p) {
   __shared__ int s_bins[kBins];
   __shared__ int s_scan[kThreads / kWave];
   __shared__ int s_pick[2];
@@ -157,29 +445,20 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const Params p) {
   }
 }
 
-// The key and value rows of the listed tokens, 16 bytes a thread.  A slot whose table entry is no page of
-// the cache is not read or written.
+// The moves that were listed, several workgroups a segment.
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(const Params p) {
   const int segment = blockIdx.x, row = segment / p.heads, head = segment - row * p.heads;
-  const int pieces = p.row_bytes / 16;  // a power of two, 2 to 64
-  const int count = p.count[segment];
-  const int per = kMoveThreads / pieces, piece = threadIdx.x % pieces;
-  const int32_t *table = p.table + (int64_t)row * p.table_stride;
   const int2 *moves = p.moves + (int64_t)segment * p.half;
-  for (int k = blockIdx.y * per + threadIdx.x / pieces; k < count; k += gridDim.y * per) {
-    const int2 m = moves[k];
-    const int from = page_of(p, m.x), to = page_of(p, m.y);
-    const int a = table[from], b = table[to];
-    if ((uint32_t)a >= (uint64_t)p.blocks || (uint32_t)b >= (uint64_t)p.blocks) continue;
-    const int64_t src = (int64_t)a * p.st_block + (int64_t)(m.x - from * p.block_size) * p.st_pos + head * p.st_head;
-    const int64_t dst = (int64_t)b * p.st_block + (int64_t)(m.y - to * p.block_size) * p.st_pos + head * p.st_head;
-    const uint4 x = *(const uint4 *)(p.k + src + piece * 16), y = *(const uint4 *)(p.v + src + piece * 16);
-    *(uint4 *)(p.k + dst + piece * 16) = x;
-    *(uint4 *)(p.v + dst + piece * 16) = y;
-  }
+  copy_rows<kMoveThreads>(p, row, head, p.count[segment], blockIdx.y, gridDim.y, [&](int k) { return moves[k]; });
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <int NT, int R>
+void launch_select(const Params &p, bool copy, dim3 grid, hipStream_t stream) {
+  if (copy) hipLaunchKernelGGL((select_kernel<NT, R, true>), grid, dim3(NT), 0, stream, p);
+  else hipLaunchKernelGGL((select_kernel<NT, R, false>), grid, dim3(NT), 0, stream, p);
+}
 
 size_t workspace_bytes(int64_t segments, int64_t capacity) {
   return (size_t)(ceil_div(segments * 4, 256) * 256 + segments * (capacity / 2) * 8);
@@ -266,13 +545,22 @@ extern "C" int ekv_evict_tokens(const ekv_eviction_t *a, void *workspace, size_t
   p.bs_mul = d.mul;
   p.bs_shift = d.shift;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict::select_kernel, dim3((unsigned)segments), dim3(evict::kThreads), 0, s, p);
+  // A workgroup copies its own moves unless there are too few of them for the rows that may move.
+  const bool copy = segments >= 2 * (int64_t)cu_count() || capacity * p.row_bytes <= 512 << 10;
+  const bool held = capacity <= 16384;
+  const dim3 grid((unsigned)segments);
+  if (!held) hipLaunchKernelGGL(evict::stream_kernel, grid, dim3(evict::kThreads), 0, s, p);
+  else if (capacity <= 2048) evict::launch_select<512, 1>(p, copy, grid, s);
+  else if (capacity <= 4096) evict::launch_select<512, 2>(p, copy, grid, s);
+  else if (capacity <= 6144) evict::launch_select<512, 3>(p, copy, grid, s);
+  else if (capacity <= 8192) evict::launch_select<512, 4>(p, copy, grid, s);
+  else evict::launch_select<1024, 4>(p, copy, grid, s);
   int rc = check_hip(hipGetLastError(), "ekv_evict_tokens select launch");
-  if (rc != EKV_OK || capacity < 2) return rc;
+  if (rc != EKV_OK || capacity < 2 || (held && copy)) return rc;
   // workgroups a segment: enough to fill the chip, no more than its longest list has work for
   const int64_t per = evict::kMoveThreads / (p.row_bytes / 16);
   int64_t y = evict::ceil_div(16 * (int64_t)cu_count(), segments);
-  const int64_t most = evict::ceil_div(p.half, per);
+  const int64_t most = evict::ceil_div(p.half, 4 * per);
   y = y > most ? most : y;
   hipLaunchKernelGGL(evict::move_kernel, dim3((unsigned)segments, (unsigned)y), dim3(evict::kMoveThreads), 0, s, p);
   return check_hip(hipGetLastError(), "ekv_evict_tokens move launch");
