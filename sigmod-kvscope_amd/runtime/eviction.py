@@ -9,13 +9,13 @@ slots, so only tokens behind the budget move, each into a freed slot.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 import ekv_hip
 from observe.allocation import _workspace, check_tensors
-from runtime.prefix_attention import _cache_shape
+from runtime.prefix_attention import _FLOAT, _INT, _cache_shape, _sound
+
+_pack = ekv_hip.packer(ekv_hip.Eviction)
 
 
 def eviction_workspace_bytes(rows: int, kv_heads: int, capacity: int) -> int:
@@ -56,38 +56,44 @@ def evict_tokens(
     rows, width = table.shape
     shape = (rows, kv_heads, width * block)
     per_row = budget if isinstance(budget, torch.Tensor) else None
-    device = check_tensors(
-        ("kv_cache", kv_cache, kv_cache.dtype, kv_cache.shape), ("table", table, torch.int32, (rows, width)),
-        ("lens", lens, torch.int32, (rows,)), ("scores", scores, torch.float32, shape),
-        ("positions", positions, torch.int32, shape), ("budget", per_row, torch.int32, (rows,)),
-        ("seen", seen, torch.int32, (rows,)), ("new_lens", new_lens, torch.int32, (rows,)),
-        ("new_scores", new_scores, torch.float32, shape), ("new_positions", new_positions, torch.int32, shape))
+    device = kv_cache.device
+    if not (kv_cache.is_cuda and _sound(
+            kv_cache.get_device(),
+            ((table, (rows, width)), (lens, (rows,)), (positions, shape), (per_row, (rows,)), (seen, (rows,)),
+             (new_lens, (rows,)), (new_positions, shape)),
+            (kv_cache, kv_cache.dtype, kv_cache.shape), (scores, _FLOAT, shape), (new_scores, _FLOAT, shape))):
+        device = check_tensors(
+            ("kv_cache", kv_cache, kv_cache.dtype, kv_cache.shape), ("table", table, _INT, (rows, width)),
+            ("lens", lens, _INT, (rows,)), ("scores", scores, _FLOAT, shape),
+            ("positions", positions, _INT, shape), ("budget", per_row, _INT, (rows,)),
+            ("seen", seen, _INT, (rows,)), ("new_lens", new_lens, _INT, (rows,)),
+            ("new_scores", new_scores, _FLOAT, shape), ("new_positions", new_positions, _INT, shape))
     if new_lens is None:
-        new_lens = torch.empty(rows, dtype=torch.int32, device=device)
+        new_lens = torch.empty(rows, dtype=_INT, device=device)
     if new_scores is None:
-        new_scores = torch.empty(shape, dtype=torch.float32, device=device)
+        new_scores = torch.empty(shape, dtype=_FLOAT, device=device)
     if new_positions is None:
-        new_positions = torch.empty(shape, dtype=torch.int32, device=device)
-    a = ekv_hip.Eviction()
-    stride = kv_cache.stride()
-    a.keys = kv_cache.data_ptr()
-    a.values = a.keys + stride[1] * kv_cache.element_size() if a.keys else 0
-    a.kv_stride_block, a.kv_stride_pos, a.kv_stride_head, a.blocks = stride[0], stride[2], stride[3], pages
-    a.table, a.table_stride, a.lens, a.seen = table.data_ptr(), table.stride(0), lens.data_ptr(), seen.data_ptr()
-    if per_row is None:
-        a.fixed_budget = int(budget)
+        new_positions = torch.empty(shape, dtype=_INT, device=device)
+    kv_block, kv_part, kv_pos, kv_head, _ = kv_cache.stride()
+    keys = kv_cache.data_ptr()
+    values = keys + kv_part * kv_cache.element_size() if keys else 0
+    s_row, s_head, _ = scores.stride()
+    p_row, p_head, _ = positions.stride()
+    ns_row, ns_head, _ = new_scores.stride()
+    np_row, np_head, _ = new_positions.stride()
+    arguments = _pack(
+        keys, values, kv_block, kv_pos, kv_head, pages, table.data_ptr(), table.stride(0), lens.data_ptr(),
+        0 if per_row is None else per_row.data_ptr(), seen.data_ptr(), scores.data_ptr(), s_row, s_head,
+        positions.data_ptr(), p_row, p_head, new_scores.data_ptr(), ns_row, ns_head, new_positions.data_ptr(), np_row,
+        np_head, new_lens.data_ptr(), ekv_hip.dtype_code(kv_cache.dtype), rows, kv_heads, dim, width, block,
+        int(budget) if per_row is None else 0, int(recent), int(sinks), 0)
+    lib = ekv_hip._lib or ekv_hip.load()
+    need = lib.ekv_evict_tokens_workspace(rows, kv_heads, width * block)
+    if workspace is None:
+        workspace = torch.empty(need or 1, dtype=torch.uint8, device=device)
     else:
-        a.budget = per_row.data_ptr()
-    a.scores, (a.scores_stride_row, a.scores_stride_head, _) = scores.data_ptr(), scores.stride()
-    a.positions, (a.positions_stride_row, a.positions_stride_head, _) = positions.data_ptr(), positions.stride()
-    a.new_scores, (a.new_scores_stride_row, a.new_scores_stride_head, _) = new_scores.data_ptr(), new_scores.stride()
-    a.new_positions, (a.new_positions_stride_row, a.new_positions_stride_head, _) = (new_positions.data_ptr(),
-                                                                                     new_positions.stride())
-    a.new_lens = new_lens.data_ptr()
-    a.kv_dtype = ekv_hip.dtype_code(kv_cache.dtype)
-    a.rows, a.kv_heads, a.head_dim, a.width, a.block_size = rows, kv_heads, dim, width, block
-    a.recent, a.sinks = int(recent), int(sinks)
-    workspace = _workspace("workspace", workspace, eviction_workspace_bytes(rows, kv_heads, width * block), device)
-    ekv_hip.call("ekv_evict_tokens", ctypes.addressof(a), workspace.data_ptr(), workspace.numel(),
-                 ekv_hip.stream_handle(stream))
+        workspace = _workspace("workspace", workspace, need, device)
+    status = lib.ekv_evict_tokens(arguments, workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream))
+    if status:
+        ekv_hip.check(status, "ekv_evict_tokens")
     return new_lens, new_scores, new_positions

@@ -13,8 +13,6 @@ that ``runtime.eviction.evict_tokens`` ranks tokens by.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 import ekv_hip
@@ -35,6 +33,24 @@ def _cache_shape(kv_cache: torch.Tensor) -> tuple[int, int, int, int]:
     return pages, block, heads, dim
 
 
+_pack = ekv_hip.packer(ekv_hip.Attention)
+_INT, _FLOAT = torch.int32, torch.float32
+
+
+def _sound(device: int, ints, *rows) -> bool:
+    """Whether int32 ``(tensor or None, shape)`` pairs and ``(tensor or None, type, shape)`` triples are what the kernels
+    read: the usual call's one look at each (``check_tensors`` finds the words for one that is not)."""
+    for t, shape in ints:
+        if t is not None and not (type(t) is torch.Tensor and t.dtype is _INT and t.shape == shape
+                                  and t.get_device() == device and t.stride(-1) == 1):
+            return False
+    for t, kind, shape in rows:
+        if t is not None and not (type(t) is torch.Tensor and t.dtype is kind and t.shape == shape
+                                  and t.get_device() == device and t.stride(-1) == 1):
+            return False
+    return device >= 0
+
+
 def _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table, prefix_lens, prefix_rows,
                k_scale, v_scale, scores, decay, out, lse):
     pages, block, kv_heads, dim = _cache_shape(kv_cache)
@@ -42,7 +58,7 @@ def _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_t
         raise ValueError(f"query must be a [tokens, heads, {dim}] tensor")
     if not isinstance(table, torch.Tensor) or table.ndim != 2:
         raise ValueError("the block table must be a [rows, width] tensor")
-    tokens, q_heads, _ = query.shape
+    q_shape = tokens, q_heads, _ = query.shape
     rows, width = table.shape
     if tokens == 0:
         query = query.new_empty(query.shape)  # no rows to be contiguous: an empty tensor's strides may be anything
@@ -57,51 +73,54 @@ def _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_t
             raise ValueError(f"{groups} prefixes need prefix_rows")
     elif prefix_lens is not None or prefix_rows is not None:
         raise ValueError("prefix_lens and prefix_rows need a prefix_table")
-    device = check_tensors(
-        ("query", query, _QUERY_TYPES, (tokens, q_heads, dim)),
-        ("kv_cache", kv_cache, kv_cache.dtype, kv_cache.shape),
-        ("table", table, torch.int32, (rows, width)), ("lens", lens, torch.int32, (rows,)),
-        ("q_start", q_start, torch.int32, (rows + 1,)),
-        ("prefix_table", prefix_table, torch.int32, (groups, prefix_width)),
-        ("prefix_lens", prefix_lens, torch.int32, (groups,)),
-        ("prefix_rows", prefix_rows, torch.int32, (groups + 1,)),
-        ("out", out, query.dtype, query.shape), ("lse", lse, torch.float32, (tokens, q_heads)))
+    dtype, device = query.dtype, query.device
+    if not (dtype in _QUERY_TYPES and query.stride(2) == 1 and query.is_cuda and _sound(
+            query.get_device(),
+            ((table, (rows, width)), (lens, (rows,)), (q_start, (rows + 1,)), (prefix_table, (groups, prefix_width)),
+             (prefix_lens, (groups,)), (prefix_rows, (groups + 1,))),
+            (kv_cache, kv_cache.dtype, kv_cache.shape), (out, dtype, q_shape), (lse, _FLOAT, (tokens, q_heads)))):
+        device = check_tensors(
+            ("query", query, _QUERY_TYPES, (tokens, q_heads, dim)),
+            ("kv_cache", kv_cache, kv_cache.dtype, kv_cache.shape),
+            ("table", table, _INT, (rows, width)), ("lens", lens, _INT, (rows,)),
+            ("q_start", q_start, _INT, (rows + 1,)),
+            ("prefix_table", prefix_table, _INT, (groups, prefix_width)),
+            ("prefix_lens", prefix_lens, _INT, (groups,)),
+            ("prefix_rows", prefix_rows, _INT, (groups + 1,)),
+            ("out", out, dtype, query.shape), ("lse", lse, _FLOAT, (tokens, q_heads)))
+    at_scores = score_row = score_head = 0
     if scores is not None:
         if not isinstance(scores, torch.Tensor) or scores.ndim != 3 or scores.shape[:2] != (rows, kv_heads) \
                 or scores.shape[2] < width * block:
             raise ValueError(f"scores must be a [{rows}, {kv_heads}, {width * block} or more] tensor")
-        if check_tensors(("scores", scores, torch.float32, scores.shape)) != device:
+        if check_tensors(("scores", scores, _FLOAT, scores.shape)) != device:
             raise ValueError(f"scores must be on {device}")
+        at_scores, score_row, score_head = scores.data_ptr(), scores.stride(0), scores.stride(1)
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        out = torch.empty(q_shape, dtype=dtype, device=device)
     if lse is None:
-        lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=device)
+        lse = torch.empty(tokens, q_heads, dtype=_FLOAT, device=device)
     elif not lse.is_contiguous():
         raise ValueError("lse must be contiguous")
-    a = ekv_hip.Attention()
-    a.query, (a.q_stride_token, a.q_stride_head, _) = query.data_ptr(), query.stride()
-    stride = kv_cache.stride()
-    a.keys = kv_cache.data_ptr()
-    a.values = a.keys + stride[1] * kv_cache.element_size() if a.keys else 0
-    a.kv_stride_block, a.kv_stride_pos, a.kv_stride_head, a.blocks = stride[0], stride[2], stride[3], pages
-    a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
-    if q_start is not None:
-        a.q_start = q_start.data_ptr()
+    q_token, q_head, _ = query.stride()
+    kv_block, kv_part, kv_pos, kv_head, _ = kv_cache.stride()
+    o_token, o_head, _ = out.stride()
+    keys = kv_cache.data_ptr()
+    values = keys + kv_part * kv_cache.element_size() if keys else 0
+    at_prefix = at_prefix_lens = at_prefix_rows = prefix_stride = 0
     if groups and prefix_width:
-        a.prefix_table, a.prefix_stride, a.prefix_lens = (prefix_table.data_ptr(), prefix_table.stride(0),
-                                                          prefix_lens.data_ptr())
+        at_prefix, prefix_stride, at_prefix_lens = prefix_table.data_ptr(), prefix_table.stride(0), prefix_lens.data_ptr()
         if prefix_rows is not None:
-            a.prefix_rows = prefix_rows.data_ptr()
-        a.prefix_groups, a.prefix_width = groups, prefix_width
-    if scores is not None:
-        a.scores, a.scores_stride_row, a.scores_stride_head = scores.data_ptr(), scores.stride(0), scores.stride(1)
-    a.out, (a.out_stride_token, a.out_stride_head, _) = out.data_ptr(), out.stride()
-    a.lse = lse.data_ptr()
-    a.q_dtype, a.kv_dtype = ekv_hip.dtype_code(query.dtype), ekv_hip.dtype_code(kv_cache.dtype)
-    a.rows, a.width, a.tokens, a.max_query = rows, width, tokens, max_query
-    a.q_heads, a.kv_heads, a.head_dim, a.block_size = q_heads, kv_heads, dim, block
-    a.scale, a.k_scale, a.v_scale, a.decay = scale, k_scale, v_scale, decay
-    return a, out, lse, device
+            at_prefix_rows = prefix_rows.data_ptr()
+    else:
+        groups = prefix_width = 0
+    return _pack(
+        query.data_ptr(), q_token, q_head, keys, values, kv_block, kv_pos, kv_head, pages, table.data_ptr(),
+        table.stride(0), lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), at_prefix, prefix_stride,
+        at_prefix_lens, at_prefix_rows, at_scores, score_row, score_head, out.data_ptr(), o_token, o_head,
+        lse.data_ptr(), ekv_hip.dtype_code(dtype), ekv_hip.dtype_code(kv_cache.dtype), rows, width,
+        groups, prefix_width, tokens, max_query, q_heads, kv_heads, dim, block, scale, k_scale, v_scale,
+        decay), out, lse, device
 
 
 def prefix_attention(
@@ -143,11 +162,15 @@ def prefix_attention(
     ``ekv_prefix_attention`` documents them; ``k_scale`` / ``v_scale`` are an fp8 cache's scales.
     ``workspace``: a uint8 device tensor that the call may overwrite (one is allocated if none is given;
     under graph capture it then belongs to the graph's pool).  No gradient is taken through the call."""
-    a, out, lse, device = _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table,
-                                     prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, out, lse)
-    address = ctypes.addressof(a)
-    need = int((ekv_hip._lib or ekv_hip.load()).ekv_prefix_attention_workspace(address))
-    workspace = _workspace("workspace", workspace, need, device)
-    ekv_hip.call("ekv_prefix_attention", address, workspace.data_ptr(), workspace.numel(),
-                 ekv_hip.stream_handle(stream))
+    arguments, out, lse, device = _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table,
+                                             prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, out, lse)
+    lib = ekv_hip._lib or ekv_hip.load()
+    need = lib.ekv_prefix_attention_workspace(arguments)
+    if workspace is None:
+        workspace = torch.empty(need or 1, dtype=torch.uint8, device=device)
+    else:
+        workspace = _workspace("workspace", workspace, need, device)
+    status = lib.ekv_prefix_attention(arguments, workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream))
+    if status:
+        ekv_hip.check(status, "ekv_prefix_attention")
     return out, lse

@@ -149,3 +149,12 @@ def test_attention_tables_of_the_most_keys():
     a = attention(width=(2**31 - 4096) // 16 - 1, block_size=16, table_stride=1 << 28)
     with pytest.raises(ValueError, match="workspace"):
         ekv_hip.call("ekv_prefix_attention", ctypes.addressof(a), P, 0, 0)
+
+
+def test_argument_blocks_are_the_structures():
+    for kind in (ekv_hip.Attention, ekv_hip.Eviction):
+        values = [i + 1 for i in range(len(kind._fields_))]
+        block = kind.from_buffer_copy(ekv_hip.packer(kind)(*values))
+        assert [getattr(block, name) for name, _ in kind._fields_] == values
+    with pytest.raises(ValueError, match="range"):
+        ekv_hip.packer(ekv_hip.Eviction)(*[2**40] * len(ekv_hip.Eviction._fields_))
