@@ -554,8 +554,9 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   const int64_t own_rows = (int64_t)p.max_query * p.group;
   const bool half = kv_dtype != EKV_F32;
   const int64_t axis = (int64_t)(p.width + (p.groups > 0 ? p.pwidth : 0)) * p.block_size + 64;
-  p.wide_own = half && own_rows >= kWideRows && axis < (1 << 30);
-  p.wide_pre = half && !p.wide_own && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= kWideRows;
+  const int least = head_dim == 256 ? kWideRows256 : kWideRows;
+  p.wide_own = half && own_rows >= least && axis < (1 << 30);
+  p.wide_pre = half && !p.wide_own && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= least;
   p.tile_own = p.wide_own ? wide_tile_rows() : kRowsPerTile;
   p.tile_pre = p.wide_pre ? wide_tile_rows() : kRowsPerTile;
   p.tiles_own = (int)ceil_div(own_rows, p.tile_own);
@@ -640,8 +641,10 @@ int launch(const Params &p, hipStream_t stream) {
     }
   }
   if (rc != EKV_OK || p.scores == nullptr || p.width == 0) return rc;
-  if (p.wide_own) return wide_weights(p, T::kType, D, stream);
   const int64_t capacity = (int64_t)p.width * p.block_size, segments = (int64_t)p.rows * p.kv_heads;
+  if (p.wide_own && (int64_t)p.max_query * p.group >= kWeighWide &&
+      segments * ceil_div(capacity, kWeighKeys) < kWeighWaves * (int64_t)cu_count())
+    return wide_weights(p, T::kType, D, stream);
   if (p.logits != nullptr) {
     const int pieces = (int)ceil_div(capacity, 4 * kThreads);
     hipLaunchKernelGGL((fold_kernel<kThreads>), dim3((unsigned)(segments * pieces)), dim3(kThreads), 0, stream, p, pieces);
@@ -733,8 +736,8 @@ int fill(const ekv_attention_t *a, Params &p) {
   // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel, 256 an item of the wide one
   if (p.waves_own + p.items_pre >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
-      (p.scores != nullptr && (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >=
-                                  (p.wide_own ? 1ll << 24 : (1ll << 26) - 64)))
+      (p.scores != nullptr &&
+       (int64_t)p.rows * p.kv_heads * ceil_div((int64_t)p.width * p.block_size, kWeighKeys) >= (1ll << 26) - 64))
     return fail(EKV_EINVAL, "%s: %d rows of %d blocks and %d tokens of %d heads pass the threads of a launch", who,
                 p.rows, p.width, p.tokens, p.q_heads);
   return EKV_OK;

@@ -21,7 +21,15 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRowsPerTile = 16;  // query rows of one narrow tile (the matrix instruction's columns)
-constexpr int kWideRows = 64;     // from so many query rows a set of keys on, the wide kernel
+// From so many query rows a set of keys on, the wide kernel: it reads the keys once where the narrow one reads them once
+// for each 16 rows.  64 rows of 1000 to 4000 tokens with 20, 32, 48 and 60 query rows a KV head: 163, 160, 167 and 167 us
+// against the narrow kernel's 251, 257, 277 and 359; at head dim 256, where the narrow kernel streams and the wide one has
+// one workgroup a compute unit, 538 us with 20 to 64 query rows against 474, 477 (32), 513 (48) and 663 (64).
+constexpr int kWideRows = 17, kWideRows256 = 64;
+// The running weights: a workgroup for 64 keys from so many query rows on, where a wave for 64 keys would leave the chip
+// unfilled (2 rows of 1000 to 4000 tokens: 70, 98, 157 and 219 us with 512, 1024, 2048 and 4000 query rows a KV head, 74,
+// 119, 207 and 343 us with a wave; 55 against 51 with 256; 32 rows, 2048: 1425 against 1357).
+constexpr int kWeighWide = 512, kWeighWaves = 16;  // query rows, waves a compute unit
 constexpr int kMostKeys = INT32_MAX - 4095;  // of a table row: a step past its last key is still an int
 constexpr int kMaxSlots = 128;    // partial results a query row can have from the equal shares of its own keys
 constexpr int kMaxChunks = 64;    // and from chunks of keys

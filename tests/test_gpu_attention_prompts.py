@@ -184,3 +184,28 @@ def test_graph_replays(counts):
         assert torch.equal(out, want_out) and torch.equal(lse, want_lse) and torch.equal(args["scores"], want_scores)
         prefix_attention(**b.on_gpu())
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_weights_of_many_query_rows(dtype, dim):
+    # 600 query rows a KV head, few rows: the weights of 64 keys are a workgroup's
+    b = Batch([170, 90], counts=[150, 90], prefixes=[37], heads=1, group=4, dim=dim, dtype=dtype, seed=dim + 2).with_scores()
+    check(b, *run(b))
+
+
+@pytest.mark.parametrize("block", [16, 24])
+def test_weights_behind_bad_pages(block):
+    b = Batch([170, 130, 0], counts=[150, 129, 0], heads=1, group=4, block=block, seed=21).with_scores()
+    b.table[0, 1], b.table[0, 3], b.table[1, :] = -1, b.cache.shape[0], 2**31 - 1
+    check(b, *run(b))
+
+
+@pytest.mark.parametrize("queries", [4, 5, 16, 17])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_around_the_wide_kernels_first_rows(queries, dim):
+    b = Batch([90, 33, 200], counts=[queries, 1, queries], prefixes=[70], heads=1, group=4, dim=dim, seed=queries).with_scores()
+    check(b, *run(b))
+    b = Batch([30 + r for r in range(2 * queries)], prefixes=[70, 90], borders=[0, queries, 2 * queries], heads=1, group=4,
+              dim=dim, seed=queries)
+    check(b, *run(b))
