@@ -87,6 +87,14 @@ __device__ __forceinline__ int page_of(const Params &p, int pos) {
 // which holds them exactly, the others keep their type.  Products of 16-bit elements are exact in the float32
 // they are summed in.
 
+// kLift: weights are 2^kLift times what they are against the running maximum, and so is their sum.  f16 has no values below
+// 2^-24, and steps of that below 2^-14: lifted to its upper end the weights keep their relative rounding down to 2^-29 and
+// are lost only below 2^-40.
+template <class H>
+constexpr float kLift = 0.f;
+template <>
+inline constexpr float kLift<_Float16> = 15.f;
+
 struct F32 {
   static constexpr int kType = EKV_F32;
   static constexpr int kBytes = 4;  // of an element in the cache

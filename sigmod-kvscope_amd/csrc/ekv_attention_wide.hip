@@ -10,8 +10,8 @@
 // of one dim a lane.  The weights' rounding (half a step of the type, relative) is of the size of the
 // output's own; their sum, the maxima and the outputs are float32.
 //
-// Measured, head dim 128: 3200 f16 query rows a KV head against prefixes of 32768 tokens 639 us (630 TFLOP/s, with
-// the own tokens and the join); bf16 prompt chunks of up to 4096 rows 293 us (630 TFLOP/s).  The narrow form of the
+// Measured, head dim 128: 3200 f16 query rows a KV head against prefixes of 32768 tokens 550 us (740 TFLOP/s, with
+// the own tokens and the join); bf16 prompt chunks of up to 4096 rows 270 us (680 TFLOP/s).  The narrow form of the
 // same calls, one wave for 16 query rows, took 2456 and 1247 us.
 #include "ekv_attention.hpp"
 
@@ -165,9 +165,12 @@ __device__ __forceinline__ float other_half_sum(float v) {
   return a + b;
 }
 
-// A running maximum is kept while no row of the wave passes it by more than this (powers of two): weights
-// then reach 2^8, well inside either type, and most steps leave the outputs unscaled.
-constexpr float kSlack = 8.f;
+// A running maximum is kept while no row of the wave passes it by more than kSlack (powers of two), so that most steps
+// leave the outputs unscaled.  Weights then reach 2^kSlack: 2^8 in bf16, and in f16 2^1, which leaves 2^14 of its lift.
+template <class H>
+constexpr float kSlack = kLift<H> > 0.f ? 1.f : 8.f;
+template <class H>
+constexpr float kWideLift = kLift<H> > 0.f ? kLift<H> - kSlack<H> : 0.f;
 
 template <class T, int D>
 __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char *lds) {
@@ -297,8 +300,8 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
       for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) high = fmaxf(high, x[k][i]);
-      high = other_half_max(high) * scale2;
-      if (!__all(high <= top + kSlack)) {
+      high = other_half_max(high) * scale2 - kWideLift<H>;
+      if (!__all(high <= top + kSlack<H>)) {
         const float peak = fmaxf(top, high);
         const float shrink = __builtin_amdgcn_exp2f(top - (peak == -INFINITY ? 0.f : peak));
         sum *= shrink;

@@ -209,3 +209,18 @@ def test_around_the_wide_kernels_first_rows(queries, dim):
     b = Batch([30 + r for r in range(2 * queries)], prefixes=[70, 90], borders=[0, queries, 2 * queries], heads=1, group=4,
               dim=dim, seed=queries)
     check(b, *run(b))
+
+
+@pytest.mark.parametrize("counts", [[1], [70]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
+def test_small_weights_beside_one_large(dtype, counts):
+    # one key holds nearly all the weight, the others 2^-27 of it each, with values that matter all the same
+    b = Batch([600], counts=counts, prefixes=[200], heads=1, group=1, dim=32, dtype=dtype, seed=23)
+    b.cache[:, 0], b.query[:] = 0.0, 0.0
+    b.query[..., 0] = 27 * np.log(2.0)
+    b.scale = 1.0
+    b.cache[:, 1] = 200.0
+    page = int(b.prefix_table[0, 0])
+    b.cache[page, 0, 3, :, 0] = 1.0
+    b.cache[page, 1, 3] = 2.0**-10
+    check(b, *run(b))
