@@ -448,15 +448,18 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
 // rows pass by in tiles of 32, wave after wave: S^T = K Q^T again, weights exp2(s - lse), and each lane adds up its
 // keys' weights over the queries of its column.  Columns, then waves are summed in one order at the end.  A tile of
 // queries is read from L2 once per 64 keys, a tile ahead of its use.  Measured: 777 queries of 7 heads a KV head
-// against up to 2047 keys, three rows of 4 KV heads of 64: 53 us (289 us in tiles of 16 query rows, a wave to 64 keys).
-constexpr int kPerGroup = 4;  // waves
+// against up to 2047 keys, three rows of 4 KV heads of 64: 43 us (289 us in tiles of 16 query rows, a wave to 64 keys).
+// waves: 8 leave two a SIMD where a few hundred workgroups are all (4 took 53 us, see above, 8 take 43); head dim 256 has
+// registers for one
+template <int D>
+constexpr int kPerGroup = D == 256 ? 4 : 8;
 constexpr int kWeighKeys = 64;
 
 template <class T, int D>
-__global__ __launch_bounds__(kPerGroup *kWave, (D == 256 ? 1 : 2)) void weigh_wide_kernel(const Params p, int pieces) {
+__global__ __launch_bounds__((kPerGroup<D> * kWave), (D == 256 ? 1 : 2)) void weigh_wide_kernel(const Params p, int pieces) {
   typedef typename T::Half H;
   constexpr int KT = kWeighKeys / 32, C = D / 16;
-  __shared__ float s_total[kPerGroup][kWeighKeys];
+  __shared__ float s_total[kPerGroup<D>][kWeighKeys];
   const uint32_t block = blockIdx.x;
   const int head = (int)(block % p.kv_heads), piece = (int)(block / p.kv_heads % pieces);
   const int row = (int)(block / p.kv_heads / pieces), begin = piece * kWeighKeys;
@@ -541,7 +544,7 @@ __global__ __launch_bounds__(kPerGroup *kWave, (D == 256 ? 1 : 2)) void weigh_wi
   };
   // queries before the first key see none of them
   const int64_t before = (int64_t)max(0, begin - see + 1) * p.group;
-  constexpr int kStride = 32 * kPerGroup;
+  constexpr int kStride = 32 * kPerGroup<D>;
   int m0 = (int)min(before, (int64_t)rows) / 32 * 32 + 32 * wave;
   Queries a, b;
   if (m0 < rows) fetch(a, m0);
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(kPerGroup *kWave, (D == 256 ? 1 : 2)) void weigh_wi
   if (threadIdx.x >= kWeighKeys || at >= end) return;
   float v = 0.f;
 #pragma unroll
-  for (int w = 0; w < kPerGroup; ++w) v += s_total[w][lane];
+  for (int w = 0; w < kPerGroup<D>; ++w) v += s_total[w][lane];
   float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
   out[at] = p.decay * out[at] + v;
 }
@@ -576,7 +579,7 @@ template <class T, int D>
 int launch_weigh(const Params &p, hipStream_t stream) {
   const int pieces = (int)ceil_div((int64_t)p.width * p.block_size, kWeighKeys);
   hipLaunchKernelGGL((weigh_wide_kernel<T, D>), dim3((unsigned)((int64_t)p.rows * pieces * p.kv_heads)),
-                     dim3(kPerGroup * kWave), 0, stream, p, pieces);
+                     dim3(kPerGroup<D> * kWave), 0, stream, p, pieces);
   return check_hip(hipGetLastError(), "ekv_prefix_attention weights launch");
 }
 
