@@ -28,7 +28,8 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, S
   item /= p.kv_heads;
   const int chunk = (int)(item % p.s_pre);
   int g, tile;
-  if (!find_tile(p, (int)(item / p.s_pre), kRowsPerTile, g, tile)) return false;
+  if (!find_tile(p.groups, (int)(item / p.s_pre), [&](int e) { return (int)ceil_div((int64_t)group_queries(p, e).count * p.group, kRowsPerTile); }, g, tile))
+    return false;
   const RowQueries t = group_queries(p, g);
   s.table = p.ptable + (int64_t)g * p.ptable_stride;
   s.ptable = nullptr;
@@ -561,7 +562,12 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   p.tile_pre = p.wide_pre ? wide_tile_rows() : kRowsPerTile;
   p.tiles_own = (int)ceil_div(own_rows, p.tile_own);
   const int64_t own_keys = (int64_t)p.width * p.block_size, prefix_keys = p.groups > 0 ? (int64_t)p.pwidth * p.block_size : 0;
-  const int64_t own_items = (int64_t)p.rows * p.kv_heads * p.tiles_own;
+  // Rows of different query counts (a prompt chunk among single tokens): the tiles there can be in all, found by a search
+  // over the rows, where every row's most would be over twice as many.  (2048 queries among 63 single tokens of long rows:
+  // 286 us, 541 us with a workgroup for every row's most; among 255 of short rows 425 against 1001.)
+  const int64_t tiles_most = (int64_t)p.rows * p.tiles_own, tiles_all = ceil_div((int64_t)p.tokens * p.group, p.tile_own) + p.rows;
+  p.packed = p.wide_own && tiles_most > 2 * tiles_all;
+  const int64_t own_items = (p.packed ? tiles_all : tiles_most) * p.kv_heads;
   p.items_pre = 0;
   p.s_pre = 0;
   p.chunk_pre = 64;

@@ -69,6 +69,7 @@ struct Params {
   int64_t waves_own;
   int chunk_own, s_own, tiles_own, chunk_pre, s_pre, tiles_pre;
   int tile_own, tile_pre;  // query rows of a tile
+  bool packed;             // own items are the tiles that rows have, not the most that one can have for each row
   int64_t items_own, items_pre;
   // wide_own: the own keys of a row go through the wide kernel, behind its prefix's on one axis (no items of
   // the prefix's own); wide_pre: the prefixes do.  direct: one chunk holds everything a query sees, so the
@@ -365,23 +366,20 @@ __device__ __forceinline__ int group_of(const Params &p, int row) {
   return lo;
 }
 
-// Group and tile of tile number `index` when every group's queries are cut into tiles of `rows` query
-// rows; false past the last.  All 64 lanes call it with one index and receive one answer.
-__device__ __forceinline__ bool find_tile(const Params &p, int index, int rows, int &g, int &tile) {
-  int before = 0;
-  for (int base = 0; base < p.groups; base += kWave) {
+// Of a list of tiles, entry after entry with tiles_of(entry) each, the entry that tile number `index` is in and its number
+// there; false past the last.  All 64 lanes call it with one index and receive one answer.
+template <class Tiles>
+__device__ __forceinline__ bool find_tile(int entries, int index, Tiles tiles_of, int &entry, int &tile) {
+  int64_t before = 0;
+  for (int base = 0; base < entries; base += kWave) {
     const int mine = base + lane_id();
-    int n = 0;
-    if (mine < p.groups) {
-      const RowQueries t = group_queries(p, mine);
-      n = (int)(((int64_t)t.count * p.group + rows - 1) / rows);
-    }
+    const int n = mine < entries ? tiles_of(mine) : 0;
     const int inc = wave_inclusive_scan(n);
     const uint64_t past = __ballot(before + inc > index);
     if (past != 0) {
       const int lane = __builtin_ctzll(past);
-      g = base + lane;
-      tile = index - before - __shfl(inc - n, lane);
+      entry = base + lane;
+      tile = (int)(index - before) - __builtin_amdgcn_readlane(inc - n, lane);
       return true;
     }
     before += __builtin_amdgcn_readlane(inc, kWave - 1);

@@ -120,8 +120,17 @@ __device__ __forceinline__ bool own_item(const Params &p, uint32_t index, Item &
   index /= p.kv_heads;
   s.slot = (int)(index % p.s_own);
   index /= p.s_own;
-  // the last tiles of a row see the most keys: they start first
-  const int row = (int)(index % p.rows), tile = p.tiles_own - 1 - (int)(index / p.rows);
+  int row, tile;
+  if (p.packed) {
+    auto tiles_of = [&](int r) {  // the first and the last row clear tokens of no row, with queries or without
+      const int n = (int)ceil_div((int64_t)min(row_queries(p, r).count, p.max_query) * p.group, p.tile_own);
+      return r == 0 || r == p.rows - 1 ? max(n, 1) : n;
+    };
+    if (!find_tile(p.rows, (int)index, tiles_of, row, tile)) return false;
+  } else {  // the last tiles of a row see the most keys: they start first
+    row = (int)(index % p.rows);
+    tile = p.tiles_own - 1 - (int)(index / p.rows);
+  }
   const int len = row_length(p, row);
   const RowQueries t = row_queries(p, row);
   const int count = min(t.count, p.max_query);

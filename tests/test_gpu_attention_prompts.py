@@ -224,3 +224,33 @@ def test_small_weights_beside_one_large(dtype, counts):
     b.cache[page, 0, 3, :, 0] = 1.0
     b.cache[page, 1, 3] = 2.0**-10
     check(b, *run(b))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_a_prompt_among_single_tokens(dtype):
+    counts = [1] * 90
+    counts[7], counts[40], counts[41] = 300, 0, 66
+    b = Batch([max(n, 20 + r) for r, n in enumerate(counts)], counts=counts, prefixes=[50, 30], borders=[3, 41, 80], heads=1,
+              group=2, dim=32, dtype=dtype, seed=24).with_scores()
+    check(b, *run(b))
+
+
+@pytest.mark.parametrize("ends", [(0, 0), (1, 0), (0, 2)])
+def test_tokens_of_no_row_beside_a_prompt_among_single_tokens(ends):
+    # 70 rows, the first and the last maybe without queries
+    counts = [ends[0]] + [1] * 30 + [300] + [1] * 37 + [ends[1]]
+    b = Batch([max(n, 20 + r) for r, n in enumerate(counts)], counts=counts, heads=1, group=2, dim=32, seed=25)
+    tokens = sum(counts)
+    want = b.want()
+    b.max_query = 299  # the prompt's last query is past it
+    bounded = b.want()
+    args = b.on_gpu()
+    query = torch.randn(5 + tokens + 3, 2, 32, dtype=torch.bfloat16, device="cuda")
+    query[5 : 5 + tokens] = args["query"]
+    args.update(query=query, q_start=args["q_start"] + 5)
+    for most, expected in ((299, bounded), (300, want)):
+        out, lse = torch.full_like(query, 9.0), torch.full((8 + tokens, 2), 9.0, device="cuda")
+        prefix_attention(**dict(args, max_query=most), out=out, lse=lse)
+        for part in (slice(0, 5), slice(5 + tokens, 8 + tokens)):
+            assert not out[part].any() and torch.isneginf(lse[part]).all()
+        check(b, out[5 : 5 + tokens], lse[5 : 5 + tokens], None, expected)
