@@ -13,8 +13,8 @@
 // 11 and 10 bits of the keys, writes scores, positions and lengths, and copies the keys and values of the tokens
 // that move.  Where a few workgroups would copy much, they list the moves for move_kernel instead, which spreads
 // them over the chip.  Bound: the scores and positions, read and written once, and the rows that move.
-// Measured, 128 rows of 8 KV heads of 128, bf16: a few tokens past a budget of 4096 33 us, half of 512 to 8192
-// tokens 251 us (78 and 321 us with eight passes through memory and a copy kernel behind them).
+// Measured, 128 rows of 8 KV heads of 128, bf16: a few tokens past a budget of 4096 29 us, half of 512 to 8192
+// tokens 254 us (78 and 321 us with eight passes through memory and a copy kernel behind them).
 #include "ekv_common.hpp"
 
 namespace ekv {
@@ -142,8 +142,10 @@ __device__ __forceinline__ void copy_rows(const Params &p, int row, int head, in
   }
 }
 
+// Up to three rounds fit 64 registers, with which a compute unit holds four workgroups, all of 128 rows at once (29 us for
+// a few tokens past a budget of 4096, 33 with two); four rounds would spill there (284 us for half of 8192, 254 with two).
 template <int NT, int R, bool COPY>
-__global__ __launch_bounds__(NT, 4) void select_kernel(const Params p) {
+__global__ __launch_bounds__(NT, (NT == 512 && R <= 3 ? 8 : 4)) void select_kernel(const Params p) {
   constexpr int kRound = 4 * NT, kBinsEach = kDigit / NT;
   typedef int Bins __attribute__((ext_vector_type(kBinsEach), aligned(4)));
   __shared__ __attribute__((aligned(16))) int s_bins[kDigit];
