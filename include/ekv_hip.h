@@ -523,8 +523,8 @@ typedef struct ekv_attention {
  * of its group together.  Tokens of no row, and of a row past its max_query-th, get out 0 and lse -inf.
  * With `scores`, each own slot j < lens[r] also accumulates the weight its key received:
  *     scores[r, h, j] = decay * scores[r, h, j] + sum over the row's queries of head h of exp(s - lse)
- * (other slots are left alone).  Sums, maxima and weights are float32; no atomics, so equal calls give
- * equal bits.
+ * (other slots are left alone).  Logits, maxima, sums and scores are float32; of 16-bit and fp8 caches a weight
+ * is rounded to the queries' type before it meets a value.  No atomics, so equal calls give equal bits.
  * Types: fp32, f16 and bf16 with keys and values of the same type, or fp8 e4m3 keys and values with bf16
  * queries.  head_dim 32, 64, 128 or 256; any block size and any number of query heads per KV head; rows of
  * the query, keys and values start at multiples of 16 bytes; width * block_size below 2^31 - 4096.

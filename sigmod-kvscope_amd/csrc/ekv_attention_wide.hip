@@ -398,7 +398,7 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
 
 // The prefixes: the steps of every (group, tile) are one list, which the workgroups that the chip holds share
 // equally.  (In chunks of equal length 648 workgroups had work where 512 fit: 1.24 waves a SIMD over the launch, 574 us
-// for 3200 query rows against prefixes of 32768 tokens; in equal shares 558 us.)
+// for 3200 query rows against prefixes of 32768 tokens; in equal shares 558 us at the time, now 471.)
 template <class T, int D>
 __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wide_prefix_kernel(const Params p) {
   using W = Wide<T, D>;
@@ -458,8 +458,8 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
 // keys' weights over the queries of its column.  Columns, then waves are summed in one order at the end.  A tile of
 // queries is read from L2 once per 64 keys, a tile ahead of its use.  Measured: 777 queries of 7 heads a KV head
 // against up to 2047 keys, three rows of 4 KV heads of 64: 43 us (289 us in tiles of 16 query rows, a wave to 64 keys).
-// waves: 8 leave two a SIMD where a few hundred workgroups are all (4 took 53 us, see above, 8 take 43); head dim 256 has
-// registers for one
+// The waves of a workgroup: 8 leave two a SIMD where a few hundred workgroups are all (the 43 us above; 4 waves took 53);
+// head dim 256 has registers for one.
 template <int D>
 constexpr int kPerGroup = D == 256 ? 4 : 8;
 constexpr int kWeighKeys = 64;
