@@ -9,6 +9,7 @@ fallback: without the built library every entry point raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -271,6 +272,26 @@ def stream_handle(stream=None) -> int:
     if raw is not None:
         _raw_stream = (raw, torch.cuda.current_device)
     return current
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_stream(stream, tensor):
+    """The context a call with ``stream=`` runs in: torch's current stream of ``tensor``'s device is ``stream`` (a torch
+    stream or a raw handle; None: left alone).  What the call allocates inside is then ordered with the kernels that use
+    it: memory that the caller's own stream has freed is not handed out before that stream is done with it, and
+    a workspace dropped on return is not handed to the caller's stream while ``stream`` still uses it."""
+    if stream is None:
+        return _HERE
+    import torch
+
+    if isinstance(stream, int):
+        if not getattr(tensor, "is_cuda", False):
+            return _HERE  # the call's own checks refuse it
+        device = tensor.device
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
 
 
 def malloc(nbytes: int) -> int:

@@ -161,16 +161,20 @@ def prefix_attention(
     plus the weight its key received from this call's queries.  Types, head dims and limits as
     ``ekv_prefix_attention`` documents them; ``k_scale`` / ``v_scale`` are an fp8 cache's scales.
     ``workspace``: a uint8 device tensor that the call may overwrite (one is allocated if none is given;
-    under graph capture it then belongs to the graph's pool).  No gradient is taken through the call."""
-    arguments, out, lse, device = _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table,
-                                             prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, out, lse)
-    lib = ekv_hip._lib or ekv_hip.load()
-    need = lib.ekv_prefix_attention_workspace(arguments)
-    if workspace is None:
-        workspace = torch.empty(need or 1, dtype=torch.uint8, device=device)
-    else:
-        workspace = _workspace("workspace", workspace, need, device)
-    status = lib.ekv_prefix_attention(arguments, workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream))
+    under graph capture it then belongs to the graph's pool).  ``stream``: the call launches and allocates as
+    under ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient
+    is taken through the call."""
+    with ekv_hip.on_stream(stream, query):
+        arguments, out, lse, device = _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table,
+                                                 prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, out, lse)
+        lib = ekv_hip._lib or ekv_hip.load()
+        need = lib.ekv_prefix_attention_workspace(arguments)
+        if workspace is None:
+            workspace = torch.empty(need or 1, dtype=torch.uint8, device=device)
+        else:
+            workspace = _workspace("workspace", workspace, need, device)
+        status = lib.ekv_prefix_attention(arguments, workspace.data_ptr(), workspace.numel(),
+                                          ekv_hip.stream_handle(stream))
     if status:
         ekv_hip.check(status, "ekv_prefix_attention")
     return out, lse
