@@ -277,19 +277,19 @@ def stream_handle(stream=None) -> int:
 _HERE = contextlib.nullcontext()
 
 
-def on_stream(stream, tensor):
-    """The context a call with ``stream=`` runs in: torch's current stream of ``tensor``'s device is ``stream`` (a torch
-    stream or a raw handle; None: left alone).  What the call allocates inside is then ordered with the kernels that use
-    it: memory that the caller's own stream has freed is not handed out before that stream is done with it, and
-    a workspace dropped on return is not handed to the caller's stream while ``stream`` still uses it."""
+def on_stream(stream, where):
+    """The context a call with ``stream=`` runs in: torch's current stream of ``where``, a tensor or a device, is
+    ``stream`` (a torch stream or a raw handle; None: left alone).  What the call allocates inside is then ordered with
+    the kernels that use it: memory that the caller's own stream has freed is not handed out before that stream is done
+    with it, and a workspace dropped on return is not handed to the caller's stream while ``stream`` still uses it."""
     if stream is None:
         return _HERE
     import torch
 
     if isinstance(stream, int):
-        if not getattr(tensor, "is_cuda", False):
+        device = torch.device(getattr(where, "device", where))
+        if device.type != "cuda":
             return _HERE  # the call's own checks refuse it
-        device = tensor.device
         stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
     return torch.cuda.stream(stream)
 

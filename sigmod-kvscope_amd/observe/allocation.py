@@ -197,18 +197,19 @@ def maxmin_keep(
     rows, width = _rows_width(scores)
     dev = check_tensors(("scores", scores, (torch.float32, torch.float64), (rows, width)),
                         ("blocks", blocks, torch.int32, (rows,)), ("pinned", pinned, _MASK_DTYPES, (rows, width)))
-    scores = scores.double() if scores.dtype == torch.float32 else scores
     if budget < 0:
         raise ValueError("the budget cannot be negative")
-    out = _out(out, rows, width, dev)
-    summary = new_summary(rows, dev)
-    need = maxmin_workspace_bytes(rows, width)
-    workspace = _workspace("workspace", workspace, need, dev)
-    ekv_hip.call(
-        "ekv_rank_maxmin", scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(pinned),
-        pinned.stride(0) if pinned is not None else 0, rows, width, int(budget), out.data_ptr(), out.stride(0),
-        summary.data_ptr(), workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream),
-    )
+    with ekv_hip.on_stream(stream, scores):
+        scores = scores.double() if scores.dtype == torch.float32 else scores
+        out = _out(out, rows, width, dev)
+        summary = new_summary(rows, dev)
+        need = maxmin_workspace_bytes(rows, width)
+        workspace = _workspace("workspace", workspace, need, dev)
+        ekv_hip.call(
+            "ekv_rank_maxmin", scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(pinned),
+            pinned.stride(0) if pinned is not None else 0, rows, width, int(budget), out.data_ptr(), out.stride(0),
+            summary.data_ptr(), workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream),
+        )
     return out, summary
 
 
@@ -244,19 +245,20 @@ def sum_keep(
     dev = check_tensors(("scores", scores, (torch.float32, torch.float64), (rows, width)),
                         ("blocks", blocks, torch.int32, (rows,)), ("weights", weights, torch.float64, (rows,)),
                         ("pinned", pinned, _MASK_DTYPES, (rows, width)))
-    scores = scores.double() if scores.dtype == torch.float32 else scores
     if budget < 0:
         raise ValueError("the budget cannot be negative")
-    out = _out(out, rows, width, dev)
-    summary = new_summary(rows, dev)
-    need = sum_workspace_bytes(rows)
-    workspace = _workspace("workspace", workspace, need, dev)
-    ekv_hip.call(
-        "ekv_rank_sum", scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(weights),
-        ekv_hip.ptr(pinned), pinned.stride(0) if pinned is not None else 0, rows, width, int(budget),
-        out.data_ptr(), out.stride(0), summary.data_ptr(), workspace.data_ptr(), workspace.numel(),
-        ekv_hip.stream_handle(stream),
-    )
+    with ekv_hip.on_stream(stream, scores):
+        scores = scores.double() if scores.dtype == torch.float32 else scores
+        out = _out(out, rows, width, dev)
+        summary = new_summary(rows, dev)
+        need = sum_workspace_bytes(rows)
+        workspace = _workspace("workspace", workspace, need, dev)
+        ekv_hip.call(
+            "ekv_rank_sum", scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(weights),
+            ekv_hip.ptr(pinned), pinned.stride(0) if pinned is not None else 0, rows, width, int(budget),
+            out.data_ptr(), out.stride(0), summary.data_ptr(), workspace.data_ptr(), workspace.numel(),
+            ekv_hip.stream_handle(stream),
+        )
     return out, summary
 
 
@@ -296,22 +298,24 @@ def uniform_keep(
                         ("pinned", pinned, _MASK_DTYPES, (rows, width)),
                         ("released", released, _MASK_DTYPES, (rows, width)),
                         ("pin_from", pin_from, torch.int32, (rows,)))
-    out = _out(out, rows, width, dev)
-    summary = new_summary(rows, dev)
-    wide = scores.dtype == torch.float64
-    need = uniform_workspace_bytes(rows, scores.dtype) if (wide or pinned is not None or released is not None) else 0
-    ws = _workspace("workspace", workspace, need, dev) if need else None
-    common = (
-        scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(measured),
-        ekv_hip.ptr(pinned), pinned.stride(0) if pinned is not None else 0,
-        ekv_hip.ptr(pin_from), int(recent_blocks),
-        ekv_hip.ptr(released), released.stride(0) if released is not None else 0,
-        rows, width, float(fraction), int(budget), out.data_ptr(), out.stride(0), summary.data_ptr(),
-    )
-    if wide:
-        ekv_hip.call("ekv_rank_uniform64", *common, ws.data_ptr(), ws.numel(), ekv_hip.stream_handle(stream))
-    else:
-        ekv_hip.call("ekv_rank_uniform_ws", *common, ekv_hip.ptr(ws), ekv_hip.stream_handle(stream))
+    with ekv_hip.on_stream(stream, scores):
+        out = _out(out, rows, width, dev)
+        summary = new_summary(rows, dev)
+        wide = scores.dtype == torch.float64
+        need = uniform_workspace_bytes(rows, scores.dtype) if (wide or pinned is not None or released is not None) else 0
+        ws = _workspace("workspace", workspace, need, dev) if need else None
+        common = (
+            scores.data_ptr(), scores.stride(0), blocks.data_ptr(), ekv_hip.ptr(measured),
+            ekv_hip.ptr(pinned), pinned.stride(0) if pinned is not None else 0,
+            ekv_hip.ptr(pin_from), int(recent_blocks),
+            ekv_hip.ptr(released), released.stride(0) if released is not None else 0,
+            rows, width, float(fraction), int(budget), out.data_ptr(), out.stride(0), summary.data_ptr(),
+        )
+        if wide:
+            ekv_hip.call("ekv_rank_uniform64", *common, ws.data_ptr(), ws.numel(),
+                         ekv_hip.stream_handle(stream))
+        else:
+            ekv_hip.call("ekv_rank_uniform_ws", *common, ekv_hip.ptr(ws), ekv_hip.stream_handle(stream))
     return out, summary
 
 

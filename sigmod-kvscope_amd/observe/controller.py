@@ -68,21 +68,22 @@ def keep_rows(
                         ("audited_blocks", audited_blocks, torch.int32, (rows,)),
                         ("released", released, _MASK_DTYPES, (rows, width)),
                         ("weights", weights, torch.float64, (rows,)))
-    if out is None:
-        out = torch.empty(rows, width, dtype=torch.uint8, device=dev)
-    elif check_tensors(("out", out, torch.uint8, (rows, width))) != dev:
-        raise ValueError(f"out must be on {dev}")
-    summary = new_summary(rows, dev)
-    code = _OBJECTIVE_CODES[objective]
-    ws = _workspace("workspace", workspace, keep_rows_workspace_bytes(objective, rows, width), dev)
-    ekv_hip.call(
-        "ekv_controller_keep", code, shares.data_ptr(),
-        ekv_hip.F64 if shares.dtype == torch.float64 else ekv_hip.F32, shares.stride(0),
-        lengths.data_ptr(), evidence.data_ptr(), ekv_hip.ptr(audited_blocks), ekv_hip.ptr(released),
-        released.stride(0) if released is not None else 0, ekv_hip.ptr(weights), rows, width, int(recent_blocks),
-        int(cap_above_blocks), float(fraction), out.data_ptr(), out.stride(0), summary.data_ptr(), ws.data_ptr(),
-        ws.numel(), ekv_hip.stream_handle(stream),
-    )
+    with ekv_hip.on_stream(stream, shares):
+        if out is None:
+            out = torch.empty(rows, width, dtype=torch.uint8, device=dev)
+        elif check_tensors(("out", out, torch.uint8, (rows, width))) != dev:
+            raise ValueError(f"out must be on {dev}")
+        summary = new_summary(rows, dev)
+        code = _OBJECTIVE_CODES[objective]
+        ws = _workspace("workspace", workspace, keep_rows_workspace_bytes(objective, rows, width), dev)
+        ekv_hip.call(
+            "ekv_controller_keep", code, shares.data_ptr(),
+            ekv_hip.F64 if shares.dtype == torch.float64 else ekv_hip.F32, shares.stride(0),
+            lengths.data_ptr(), evidence.data_ptr(), ekv_hip.ptr(audited_blocks), ekv_hip.ptr(released),
+            released.stride(0) if released is not None else 0, ekv_hip.ptr(weights), rows, width, int(recent_blocks),
+            int(cap_above_blocks), float(fraction), out.data_ptr(), out.stride(0), summary.data_ptr(), ws.data_ptr(),
+            ws.numel(), ekv_hip.stream_handle(stream),
+        )
     return out, summary
 
 
@@ -116,16 +117,17 @@ def uniform_keep_rows(
         raise ValueError("the budget fraction must be in (0, 1]")
     if recent_blocks < 0 or cap_above_blocks < 0:
         raise ValueError("invalid controller settings")
-    measured = (evidence.to(torch.bool) & (lengths > cap_above_blocks)).to(torch.uint8)  # controller.py:402-408
-    blocks = torch.clamp(lengths, max=shares.shape[1]).to(torch.int32)
-    return uniform_keep(
-        shares,
-        blocks,
-        measured=measured,
-        pin_from=audited_blocks,
-        recent_blocks=recent_blocks,
-        released=released,
-        fraction=fraction,
-        out=out,
-        stream=stream,
-    )
+    with ekv_hip.on_stream(stream, shares):
+        measured = (evidence.to(torch.bool) & (lengths > cap_above_blocks)).to(torch.uint8)  # controller.py:402-408
+        blocks = torch.clamp(lengths, max=shares.shape[1]).to(torch.int32)
+        return uniform_keep(
+            shares,
+            blocks,
+            measured=measured,
+            pin_from=audited_blocks,
+            recent_blocks=recent_blocks,
+            released=released,
+            fraction=fraction,
+            out=out,
+            stream=stream,
+        )

@@ -179,25 +179,26 @@ def tile_shares(
     not written by anything else between calls; or one allocated here)."""
     code = _aggregate_code(aggregate)
     n = rows if row_ids is None else int(row_ids.shape[0])
-    if out is None:
-        out = torch.empty(n, width, dtype=torch.float32, device="cuda")
-    if out.shape != (n, width) or out.dtype != torch.float32 or out.stride(1) != 1:
-        raise ValueError("out must be float32 [rows, width] with contiguous rows")
-    for t in (row_ids, row_blocks):
-        if t is not None and (t.dtype != torch.int32 or not t.is_cuda or t.stride(0) != 1):
-            raise ValueError("row_ids and row_blocks must be contiguous int32 device tensors")
-    layer_stride = rows * width * group_rows
-    need = shares_workspace_bytes(n, width, layers)
-    if workspace is None:
-        workspace = torch.zeros(max(need, 1), dtype=torch.uint8, device=out.device)
-    if workspace.dtype != torch.uint8 or not workspace.is_cuda or workspace.numel() < need:
-        raise ValueError(f"workspace must be a uint8 device tensor of at least {need} bytes")
-    ekv_hip.call(
-        "ekv_tile_shares_ws",
-        int(base), table_layers * layer_stride, layer_stride, width * group_rows, layers, group_rows, width,
-        ekv_hip.ptr(row_ids), ekv_hip.ptr(row_blocks), n, int(tile_blocks), code, out.data_ptr(), out.stride(0),
-        workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream),
-    )
+    with ekv_hip.on_stream(stream, "cuda" if out is None else out):
+        if out is None:
+            out = torch.empty(n, width, dtype=torch.float32, device="cuda")
+        if out.shape != (n, width) or out.dtype != torch.float32 or out.stride(1) != 1:
+            raise ValueError("out must be float32 [rows, width] with contiguous rows")
+        for t in (row_ids, row_blocks):
+            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or t.stride(0) != 1):
+                raise ValueError("row_ids and row_blocks must be contiguous int32 device tensors")
+        layer_stride = rows * width * group_rows
+        need = shares_workspace_bytes(n, width, layers)
+        if workspace is None:
+            workspace = torch.zeros(max(need, 1), dtype=torch.uint8, device=out.device)
+        if workspace.dtype != torch.uint8 or not workspace.is_cuda or workspace.numel() < need:
+            raise ValueError(f"workspace must be a uint8 device tensor of at least {need} bytes")
+        ekv_hip.call(
+            "ekv_tile_shares_ws",
+            int(base), table_layers * layer_stride, layer_stride, width * group_rows, layers, group_rows, width,
+            ekv_hip.ptr(row_ids), ekv_hip.ptr(row_blocks), n, int(tile_blocks), code, out.data_ptr(), out.stride(0),
+            workspace.data_ptr(), workspace.numel(), ekv_hip.stream_handle(stream),
+        )
     return out
 
 

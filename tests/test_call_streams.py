@@ -11,6 +11,9 @@ import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import ekv_hip
+import observe.allocation
+import observe.controller
+import observe.tile_shares
 import runtime.eviction
 import runtime.prefix_attention
 
@@ -92,14 +95,44 @@ def test_eviction(host):
         cache, table, lens, scores, positions, 4, lens, stream=SIDE), 4)
 
 
+@pytest.mark.parametrize("objective", ["maxmin", "sum"])
+def test_objectives(host, objective):
+    scores, blocks = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int32)
+    keep = observe.allocation.maxmin_keep if objective == "maxmin" else observe.allocation.sum_keep
+    check(host, observe.allocation, lambda: keep(scores, blocks, budget=2, stream=SIDE), 4)  # with the float64 scores
+
+
+def test_uniform(host):
+    scores, blocks = torch.zeros(3, 8, dtype=torch.float64), torch.zeros(3, dtype=torch.int32)
+    check(host, observe.allocation, lambda: observe.allocation.uniform_keep(scores, blocks, stream=SIDE), 3)
+
+
+@pytest.mark.parametrize("objective", ["uniform", "maxmin", "sum"])
+def test_controller(host, objective):
+    shares, lengths, evidence = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int32), torch.ones(3, dtype=torch.bool)
+    host.patch.setattr(observe.allocation, "check_tensors", lambda *specs: torch.device("cpu"))
+    check(host, observe.controller, lambda: observe.controller.keep_rows(
+        shares, lengths, evidence, 0.5, objective=objective, stream=SIDE), 2)
+
+
+def test_shares(host):
+    host.patch.setattr(torch.Tensor, "is_cuda", True)
+    out = torch.zeros(3, 8)
+    check(host, observe.allocation, lambda: observe.tile_shares.tile_shares(
+        4096, table_layers=2, layers=2, rows=3, width=8, group_rows=4, row_ids=None, row_blocks=None, tile_blocks=8,
+        out=out, stream=SIDE), 1)
+
+
 def test_raw_handles(monkeypatch):
-    tensor = types.SimpleNamespace(is_cuda=True, device="device")
+    device = torch.device("cuda:0")
+    tensor = types.SimpleNamespace(device=device)
     monkeypatch.setattr(torch.cuda, "stream", lambda stream: ("under", stream))
     monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device: (handle, device))
     monkeypatch.setattr(torch.cuda, "default_stream", lambda device: ("default", device))
     assert ekv_hip.on_stream(SIDE, tensor) == ("under", SIDE)
-    assert ekv_hip.on_stream(4096, tensor) == ("under", (4096, "device"))
-    assert ekv_hip.on_stream(0, tensor) == ("under", ("default", "device"))  # 0 is the default stream's handle
+    assert ekv_hip.on_stream(4096, tensor) == ("under", (4096, device))
+    assert ekv_hip.on_stream(0, tensor) == ("under", ("default", device))  # 0 is the default stream's handle
+    assert ekv_hip.on_stream(4096, device) == ("under", (4096, device))
     with ekv_hip.on_stream(None, tensor), ekv_hip.on_stream(4096, torch.zeros(1)):
         pass  # no stream named; a host tensor, which the call's checks refuse
 
