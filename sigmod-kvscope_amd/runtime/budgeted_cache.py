@@ -44,9 +44,11 @@ class BudgetedCache:
         self.prefix_len = torch.zeros(1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
         self.seen = torch.zeros(rows, dtype=torch.int32, device=device)  # the position of a row's next token
-        slots = (rows, kv_heads, width * block)
-        self.scores = torch.zeros(slots, dtype=torch.float32, device=device)
-        self.positions = torch.full(slots, -1, dtype=torch.int32, device=device)
+        # a row more than there are, and page 0, take the tokens that an append gives to no row
+        slots = (rows + 1, kv_heads, width * block)
+        self._all_scores = torch.zeros(slots, dtype=torch.float32, device=device)
+        self._all_positions = torch.full(slots, -1, dtype=torch.int32, device=device)
+        self.scores, self.positions = self._all_scores[:rows], self._all_positions[:rows]
         self._other_lens = torch.zeros_like(self.lens)
         self.longest = 0  # no row has more tokens (the device alone knows each row's)
 
@@ -55,8 +57,12 @@ class BudgetedCache:
         """Whether a row may have no slot left for another token."""
         return self.longest >= self.capacity
 
-    def _write(self, table: torch.Tensor, row: torch.Tensor, slot: torch.Tensor, keys: torch.Tensor, values: torch.Tensor):
-        page = table[row, slot // self.block].long()
+    def _check(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        tail = self.kv.shape[3:]
+        if keys.ndim != 3 or keys.shape[1:] != tail or values.shape != keys.shape:
+            raise ValueError(f"keys and values must be [tokens, {tail[0]}, {tail[1]}], got {tuple(keys.shape)} and {tuple(values.shape)}")
+
+    def _write(self, page: torch.Tensor, slot: torch.Tensor, keys: torch.Tensor, values: torch.Tensor) -> None:
         raw = self.kv.view(torch.uint8) if self.kv.dtype == torch.float8_e4m3fn else self.kv
         for part, rows in ((0, keys), (1, values)):
             rows = rows.to(self.kv.dtype)
@@ -64,30 +70,46 @@ class BudgetedCache:
 
     def set_prefix(self, keys: torch.Tensor, values: torch.Tensor) -> None:
         """The prefix that every row shares: keys and values ``[tokens, kv_heads, dim]`` (already over an fp8 cache's scales)."""
+        self._check(keys, values)
         n = keys.shape[0]
         if self.prefix_table is None or n > self.prefix_table.shape[1] * self.block:
             raise ValueError(f"no room for a prefix of {n} tokens")
         slot = torch.arange(n, device=self.kv.device)
-        self._write(self.prefix_table, torch.zeros_like(slot), slot, keys, values)
+        self._write(self.prefix_table[0, slot // self.block].long(), slot, keys, values)
         self.prefix_len.fill_(n)
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, q_start: torch.Tensor | None = None, max_query: int = 1) -> None:
-        """Each row's next tokens, ``[tokens, kv_heads, dim]``: row r's from ``q_start[r]`` to ``q_start[r + 1]``, at most
-        ``max_query`` (None: one a row)."""
+        """Each row's next tokens, ``[tokens, kv_heads, dim]``: row r's from ``q_start[r]`` to ``q_start[r + 1]`` (None: one a
+        row), at most ``max_query``.  What passes it, or is no row's (padding before or behind the rows'), is not kept: the
+        device alone knows the counts, and no row outgrows its pages whatever they are."""
+        self._check(keys, values)
+        rows, n, device = self.lens.shape[0], keys.shape[0], self.kv.device
+        if q_start is None and n != rows:
+            raise ValueError(f"{n} tokens of {rows} rows need q_start")
+        if q_start is not None and q_start.shape != (rows + 1,):
+            raise ValueError(f"q_start must have shape {(rows + 1,)}, got {tuple(q_start.shape)}")
+        if max_query < 1:
+            raise ValueError(f"at most {max_query} tokens a row")
         if self.longest + max_query > self.capacity:
             raise ValueError(f"{max_query} more tokens pass the {self.capacity} of a row: trim first")
-        rows, device = self.lens.shape[0], self.kv.device
-        token = torch.arange(keys.shape[0], device=device)
+        token = torch.arange(n, device=device)
         if q_start is None:
-            row, nth, counts = token, torch.zeros_like(token), 1
+            row = into = token
+            slot, at, counts = self.lens.long(), self.seen, 1
+            page = self.table[row, slot // self.block].long()
         else:
-            start = q_start.long()
-            row = torch.searchsorted(start, token, right=True) - 1
-            nth, counts = token - start[row], (start[1:] - start[:-1]).int()
-        slot = self.lens.long()[row] + nth
-        self._write(self.table, row, slot, keys, values)
-        self.scores[row, :, slot] = 0.0
-        self.positions[row, :, slot] = (self.seen[row] + nth.int())[:, None]
+            start = q_start.long().clamp(0, n)
+            counts = (start[1:] - start[:-1]).clamp(0, max_query).int()
+            row = (torch.searchsorted(start, token, right=True) - 1).clamp(0, rows - 1)
+            nth = token - start[row]
+            kept = (nth >= 0) & (nth < counts[row])
+            slot = torch.where(kept, self.lens[row] + nth, 0)
+            at = self.seen[row] + nth.int()
+            page = torch.where(kept, self.table[row, slot // self.block].long(), 0)
+            into = torch.where(kept, row, rows)
+        self._write(page, slot, keys, values)
+        self._all_scores[into, :, slot] = 0.0
+        self._all_positions[into, :, slot] = at[:, None]
         self.lens += counts
         self.seen += counts
         self.longest += max_query
