@@ -520,7 +520,8 @@ typedef struct ekv_attention {
  * and a query that sees nothing has out 0 and lse -inf.  A table entry that is no page of the cache
  * (negative, or blocks and more) is as if its tokens were not there.  What the cache holds in slots that
  * no query of the row sees is never used, whatever it is.  A prefix's pages are read for all the queries
- * of its group together.  Tokens of no row, and of a row past its max_query-th, get out 0 and lse -inf.
+ * of its group together, except where rows bring so many queries each, or the prefixes (by prefix_width)
+ * are so short, that a walk of each row's own is faster.  Tokens of no row, and of a row past its max_query-th, get out 0 and lse -inf.
  * With `scores`, each own slot j < lens[r] also accumulates the weight its key received:
  *     scores[r, h, j] = decay * scores[r, h, j] + sum over the row's queries of head h of exp(s - lse)
  * (other slots are left alone).  Logits, maxima, sums and scores are float32; of 16-bit and fp8 caches a weight

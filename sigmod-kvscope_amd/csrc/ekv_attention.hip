@@ -9,7 +9,8 @@
 // into pieces; a piece leaves its maximum, sum and unnormalised output for each of its query rows, which
 // combine_kernel joins:
 //   m = max_c m_c,  l = sum_c l_c 2^(m_c - m),  out = sum_c o_c 2^(m_c - m) / l.
-// A prefix is read once per tile of its group's query rows and not once per row.
+// A prefix is read once per tile of its group's query rows and not once per row, unless the rows' own tiles are as few
+// or joining costs more (pays_together).
 #include "ekv_attention.hpp"
 
 namespace ekv {
@@ -318,13 +319,14 @@ __global__ __launch_bounds__(W == 1 ? kThreads : W *kWave) void combine_kernel(c
     const int g = group_of(p, row);
     const int n = g >= 0 ? group_length(p, g) : 0;
     if (p.wide_own) {
-      const int64_t all = seen > 0 ? (int64_t)own_begin(n) + seen : n;
+      const int ahead = p.wide_pre ? 0 : n;  // keys before the own ones on their axis
+      const int64_t all = seen > 0 ? (int64_t)own_begin(ahead) + seen : ahead;
       own = all > 0 ? (int)((all - 1) / p.chunk_own) + 1 : 0;
     } else {
       own = seen > 0 ? p.row_slots[row] : 0;
-      if (n > 0)
-        pre = p.wide_pre ? p.pre_slots[(int64_t)token * p.group + q_head % p.group] : (n - 1) / p.chunk_pre + 1;
     }
+    if (n > 0 && p.wide_pre) pre = p.pre_slots[(int64_t)token * p.group + q_head % p.group];
+    else if (n > 0 && !p.wide_own) pre = (n - 1) / p.chunk_pre + 1;
   }
   constexpr int kPer = D > 64 ? D / 64 : 1;
   constexpr int kLanes = D / kPer;
@@ -549,6 +551,25 @@ Shape narrow_shape(int kv_dtype, int head_dim) {
                                                                                      : narrow_shape<BF16>(head_dim);
 }
 
+// Where the wide kernel takes the own keys: whether the prefixes are read for all queries of a group together, as for
+// fewer query rows, and joined to the own keys' results.  Else each of the rows' `alone` tiles walks its prefix by itself,
+// ahead of its own keys, with nothing to join: the better way where rows fill their tiles (a prompt chunk each) or the
+// prefix is short.  Told apart by what the two cost the chip: a key and its value 26, 30, 38 or 108 ps a tile at head dims
+// 32 to 256, a partial result its bytes written and read at 4 TB/s, the launches more 12 us.  Measured, a walk for each
+// tile against together, 8 KV heads of 128, 4 query heads each: 200 rows of 5 queries behind two prefixes of 32768 tokens
+// 3652 against 793 us, of 8 queries 3675 against 1432; 128 rows of 5, 8, 16, 20, 24 and 32 queries behind 8192 tokens 476,
+// 482, 539, 574, 578 and 656 against 209, 267, 434, 520, 603 and 776, of 5 behind 1024 tokens 122 against 129; 2048 queries
+// among 127 single tokens behind 8192, 2048 and 256 tokens 814, 299 and 138 against 491, 269 and 208.
+bool pays_together(const Params &p, int head_dim, int64_t alone) {
+  const int64_t together = ceil_div((int64_t)p.tokens * p.group, wide_tile_rows()) + p.groups;
+  const int64_t workers = (int64_t)cu_count() * wide_resident(head_dim) / p.kv_heads;
+  const double slots = 2.0 + (double)workers / together;
+  const double key = (22.0 + head_dim / 8.0) * 2 / wide_resident(head_dim) * 1e-3;  // ns
+  const double saved = (double)(alone - together) * p.kv_heads * p.pwidth * p.block_size * key;
+  const double join = 12000.0 + (double)p.tokens * p.q_heads * slots * (head_dim * 4 + 8) / 2000.0;
+  return saved > join;
+}
+
 void plan(Params &p, int head_dim, int kv_dtype) {
   p.whole = p.block_size % 16 == 0 && p.st_pos >= 0 && p.st_pos < 1 << 24;
   const int64_t queries = (int64_t)p.tokens * p.q_heads;
@@ -557,9 +578,7 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   const int64_t axis = (int64_t)(p.width + (p.groups > 0 ? p.pwidth : 0)) * p.block_size + 64;
   const int least = head_dim == 256 ? kWideRows256 : kWideRows;
   p.wide_own = half && own_rows >= least && axis < (1 << 30);
-  p.wide_pre = half && !p.wide_own && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= least;
   p.tile_own = p.wide_own ? wide_tile_rows() : kRowsPerTile;
-  p.tile_pre = p.wide_pre ? wide_tile_rows() : kRowsPerTile;
   p.tiles_own = (int)ceil_div(own_rows, p.tile_own);
   const int64_t own_keys = (int64_t)p.width * p.block_size, prefix_keys = p.groups > 0 ? (int64_t)p.pwidth * p.block_size : 0;
   // Rows of different query counts (a prompt chunk among single tokens): the tiles there can be in all, found by a search
@@ -568,11 +587,17 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   const int64_t tiles_most = (int64_t)p.rows * p.tiles_own, tiles_all = ceil_div((int64_t)p.tokens * p.group, p.tile_own) + p.rows;
   p.packed = p.wide_own && tiles_most > 2 * tiles_all;
   const int64_t own_items = (p.packed ? tiles_all : tiles_most) * p.kv_heads;
+  if (p.wide_own)
+    p.wide_pre = p.groups > 0 && pays_together(p, head_dim, tiles_most < tiles_all ? tiles_most : tiles_all);
+  else
+    p.wide_pre = half && p.groups > 0 && (int64_t)p.tokens * p.group / p.groups >= least;
+  p.tile_pre = p.wide_pre ? wide_tile_rows() : kRowsPerTile;
   p.items_pre = 0;
   p.s_pre = 0;
   p.chunk_pre = 64;
+  const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));  // partial results of 256 MB
   if (p.wide_own) {
-    split_wide(own_begin(prefix_keys) + own_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
+    split_wide((p.wide_pre ? 0 : own_begin(prefix_keys)) + own_keys, own_items, queries, head_dim, p.chunk_own, p.s_own);
   } else {
     // waves that a (KV head, tile) has: all together those that the chip holds, and no more than there are steps
     const Shape shape = narrow_shape(kv_dtype, head_dim);
@@ -581,25 +606,22 @@ void plan(Params &p, int head_dim, int kv_dtype) {
     share = share > p.rows * row_steps ? p.rows * row_steps : share;
     p.share = (int)(share < 1 ? 1 : share);
     int64_t slots = row_steps + 2;
-    const int64_t fit = (256ll << 20) / ((queries > 0 ? queries : 1) * (head_dim * 4 + 8));
     slots = slots > fit ? fit : slots;
     p.s_own = (int)(slots > kMaxSlots ? kMaxSlots : slots < 3 ? 3 : slots);
     p.waves_own = each * p.share;
-    if (p.groups > 0) {
-      if (p.wide_pre) {
-        // workgroups that a KV head has: all together those that the chip holds
-        const int64_t groups = (int64_t)cu_count() * wide_resident(head_dim) / p.kv_heads;
-        p.share_pre = (int)(groups < 1 ? 1 : groups);
-        const int64_t most = ceil_div(prefix_keys, 32) + 2;
-        int64_t limit = most > fit ? fit : most;
-        p.s_pre = (int)(limit > kMaxChunks ? kMaxChunks : limit < 3 ? 3 : limit);
-      } else {
-        p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
-        const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
-        split(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
-        p.items_pre = items * p.s_pre;
-      }
-    }
+  }
+  if (p.wide_pre) {
+    // workgroups that a KV head has: all together those that the chip holds
+    const int64_t groups = (int64_t)cu_count() * wide_resident(head_dim) / p.kv_heads;
+    p.share_pre = (int)(groups < 1 ? 1 : groups);
+    const int64_t most = ceil_div(prefix_keys, 32) + 2;
+    const int64_t limit = most > fit ? fit : most;
+    p.s_pre = (int)(limit > kMaxChunks ? kMaxChunks : limit < 3 ? 3 : limit);
+  } else if (p.groups > 0 && !p.wide_own) {
+    p.tiles_pre = (int)(ceil_div((int64_t)p.tokens * p.group, p.tile_pre) + p.groups);
+    const int64_t items = (int64_t)p.kv_heads * p.tiles_pre;
+    split(prefix_keys, items, queries, head_dim, p.chunk_pre, p.s_pre);
+    p.items_pre = items * p.s_pre;
   }
   p.items_own = p.wide_own ? own_items * p.s_own : 0;
   // The logits of a decode step's few query rows are kept (4 bytes each, written and read, against the key read
@@ -612,7 +634,7 @@ void plan(Params &p, int head_dim, int kv_dtype) {
       p.logit_stride = stride;
     }
   }
-  p.direct = p.wide_own && p.s_own == 1;
+  p.direct = p.wide_own && !p.wide_pre && p.s_own == 1;
 }
 
 size_t partial_bytes(const Params &p, int head_dim) {
@@ -629,7 +651,8 @@ template <class T, int D>
 int launch(const Params &p, hipStream_t stream) {
   int rc = EKV_OK;
   if (p.tokens > 0) {
-    if (p.wide_own || p.wide_pre) rc = wide_attention(p, T::kType, D, p.wide_own, stream);
+    if (p.wide_pre) rc = wide_attention(p, T::kType, D, false, stream);
+    if (rc == EKV_OK && p.wide_own) rc = wide_attention(p, T::kType, D, true, stream);
     using N = Narrow<T, D>;
     const unsigned grid = (unsigned)(ceil_div(p.items_pre, N::kWaves) + ceil_div(p.waves_own, N::kWaves));
     if (rc == EKV_OK && grid > 0) {

@@ -21,10 +21,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRowsPerTile = 16;  // query rows of one narrow tile (the matrix instruction's columns)
-// From so many query rows a set of keys on, the wide kernel: it reads the keys once where the narrow one reads them once
-// for each 16 rows.  64 rows of 1000 to 4000 tokens with 20, 32, 48 and 60 query rows a KV head: 163, 160, 167 and 167 us
-// against the narrow kernel's 251, 257, 277 and 359; at head dim 256, where the narrow kernel streams and the wide one has
-// one workgroup a compute unit, 538 us with 20 to 64 query rows against 474, 477 (32), 513 (48) and 663 (64).
+// From so many query rows a set of keys on (a row's own keys, a group's prefix), the wide kernel: it reads the keys once
+// where the narrow one reads them once for each 16 rows.  Own keys alone, 64 rows of 1000 to 4000 tokens with 20, 32, 48 and
+// 60 query rows a KV head: 163, 160, 167 and 167 us against the narrow kernel's 251, 257, 277 and 359; at head dim 256, where
+// the narrow kernel streams and the wide one has one workgroup a compute unit, 538 us with 20 to 64 query rows against 474,
+// 477 (32), 513 (48) and 663 (64).
 constexpr int kWideRows = 17, kWideRows256 = 64;
 // The running weights: a workgroup for 64 keys from so many query rows on, where a wave for 64 keys would leave the chip
 // unfilled (2 rows of 1000 to 4000 tokens: 70, 98, 157 and 219 us with 512, 1024, 2048 and 4000 query rows a KV head, 74,
@@ -71,9 +72,9 @@ struct Params {
   int tile_own, tile_pre;  // query rows of a tile
   bool packed;             // own items are the tiles that rows have, not the most that one can have for each row
   int64_t items_own, items_pre;
-  // wide_own: the own keys of a row go through the wide kernel, behind its prefix's on one axis (no items of
-  // the prefix's own); wide_pre: the prefixes do.  direct: one chunk holds everything a query sees, so the
-  // wide kernel writes the result.
+  // wide_own: the own keys of a row go through the wide kernel; wide_pre: the prefixes do, each for all queries of
+  // its group.  wide_own alone: a row's tiles walk its prefix ahead of the own keys, on one axis.  direct: one chunk
+  // holds everything a query sees, so the wide kernel writes the result.
   bool wide_own, wide_pre, direct;
   bool whole;  // 16 slots from a multiple of 16 on lie in one page, at offsets below 2^31
 };

@@ -147,7 +147,7 @@ __device__ __forceinline__ bool own_item(const Params &p, uint32_t index, Item &
   s.table = p.table + (int64_t)row * p.table_stride;
   s.ptable = nullptr;
   s.plen = 0;
-  const int g = group_of(p, row);
+  const int g = p.wide_pre ? -1 : group_of(p, row);
   if (g >= 0) {
     s.ptable = p.ptable + (int64_t)g * p.ptable_stride;
     s.plen = group_length(p, g);

@@ -5,7 +5,8 @@ Requests of a service begin with the same instructions; their keys and values ar
 pages every request of the group points to.  Attention that walks each request's own table reads those
 pages once per request.  Here a group's queries read them together, once per tile of query rows, on the
 matrix cores, and the result joins the attention over each row's own pages through the logarithms of
-their sums.
+their sums.  (Rows of long prompt chunks, which fill tiles by themselves, and prefixes too short to be
+worth the joining are walked row by row.)
 
 With ``scores`` the call also adds to every own token the weight it received, the running statistic
 that ``runtime.eviction.evict_tokens`` ranks tokens by.
@@ -155,7 +156,8 @@ def prefix_attention(
 
     ``prefix_table`` int32 ``[groups, pages]`` and ``prefix_lens`` int32 ``[groups]``: shared prefixes, seen
     whole by every query of rows ``prefix_rows[g] .. prefix_rows[g + 1]`` (ascending; None: one group of
-    every row).
+    every row).  The work is laid out by the tables' widths, the lengths being the device's: tables as wide
+    as their longest rows are the fastest.
 
     ``scores`` float32 ``[rows, kv_heads, slots]``: slot j of each row's tokens becomes ``decay * scores``
     plus the weight its key received from this call's queries.  Types, head dims and limits as
