@@ -142,10 +142,16 @@ __device__ __forceinline__ void copy_rows(const Params &p, int row, int head, in
   }
 }
 
-// Up to three rounds fit 64 registers, with which a compute unit holds four workgroups, all of 128 rows at once (29 us for
-// a few tokens past a budget of 4096, 33 with two); four rounds would spill there (284 us for half of 8192, 254 with two).
+// Waves a SIMD that the registers are kept to.  Where the workgroups copy, up to three rounds fit 64, with which a compute
+// unit holds four workgroups, all of 128 rows at once (29 us for a few tokens past a budget of 4096, 33 with two); four
+// rounds would spill there (284 us for half of 8192, 254 with two).  Where they list the moves there are few workgroups, and
+// 128 registers, or 96 for four rounds, hold a row without a spill (with eight and four waves 35 to 104 registers spilled:
+// 8 rows of 8 heads and 8192 tokens cut in half 57 us, 42 without; 32 rows of 4096 and 8192 tokens 80 and 163, 66 and 147).
 template <int NT, int R, bool COPY>
-__global__ __launch_bounds__(NT, (NT == 512 && R <= 3 ? 8 : 4)) void select_kernel(const Params p) {
+constexpr int kSelectWaves = COPY ? (NT == 512 && R <= 3 ? 8 : 4) : (R <= 3 ? 4 : 5);
+
+template <int NT, int R, bool COPY>
+__global__ __launch_bounds__(NT, (kSelectWaves<NT, R, COPY>)) void select_kernel(const Params p) {
   constexpr int kRound = 4 * NT, kBinsEach = kDigit / NT;
   typedef int Bins __attribute__((ext_vector_type(kBinsEach), aligned(4)));
   __shared__ __attribute__((aligned(16))) int s_bins[kDigit];
