@@ -625,11 +625,11 @@ void plan(Params &p, int head_dim, int kv_dtype) {
   }
   p.items_own = p.wide_own ? own_items * p.s_own : 0;
   // The logits of a decode step's few query rows are kept (4 bytes each, written and read, against the key read
-  // again) where they stay below a gigabyte.
+  // again) where they stay below a gigabyte and fold_kernel's launch below 2^32 threads.
   p.logit_rows = p.logit_stride = 0;
   if (p.scores != nullptr && own_rows <= kRowsPerTile && p.tokens > 0) {
-    const int64_t stride = ceil_div(own_keys, 4) * 4;
-    if (stride * p.rows * p.kv_heads * own_rows <= (256ll << 20)) {
+    const int64_t stride = ceil_div(own_keys, 4) * 4, segments = (int64_t)p.rows * p.kv_heads;
+    if (stride * segments * own_rows <= (256ll << 20) && segments * ceil_div(own_keys, 4 * kThreads) < (1ll << 24)) {
       p.logit_rows = (int)own_rows;
       p.logit_stride = stride;
     }
@@ -762,7 +762,8 @@ int fill(const ekv_attention_t *a, Params &p) {
   p.v_scale = a->v_scale;
   p.decay = a->decay;
   plan(p, a->head_dim, a->kv_dtype);
-  // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel, 256 an item of the wide one
+  // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel and of the weights read again, 256 an
+  // item of the wide one
   if (p.waves_own + p.items_pre >= (1ll << 26) - 64 || p.items_own >= (1ll << 24) ||
       (int64_t)p.tokens * p.q_heads >= (1ll << 26) - 64 ||
       (p.scores != nullptr &&

@@ -33,3 +33,20 @@ def test_rows_that_fill_their_tiles_walk_their_prefix_in_one_pass():
     assert slots(5, 1024, 5 * 700, 1999 // 16 * 16, width=188) == 0
     assert slots(64, 64, 64 * 64, 32768) == 0
     assert slots(128, 5, 128 * 5, 64) == 0  # nothing to save by a prefix of 64 tokens
+
+
+def test_kept_logits_fit_a_launch():
+    """Folding the kept logits takes a workgroup of 256 for every (row, KV head), however short the row: from 2^24 of them on
+    that is no launch, and the weights are computed from the keys again."""
+    def more(rows):  # bytes that the scores add to the workspace
+        sizes = []
+        for scores in (0, P):
+            a = attention(rows=rows, tokens=rows, q_heads=8, kv_heads=8, head_dim=32, width=1, table_stride=1, block_size=16,
+                          scores=scores, scores_stride_row=128, scores_stride_head=16)
+            sizes.append(ekv_hip.load().ekv_prefix_attention_workspace(ctypes.addressof(a)))
+            assert sizes[-1] > 0
+        return sizes[1] - sizes[0]
+
+    kept = (1 << 21) - 1  # rows of 8 KV heads
+    assert more(kept) == kept * 8 * 16 * 4
+    assert more(1 << 21) == 0
