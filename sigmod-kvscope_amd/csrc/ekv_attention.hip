@@ -21,7 +21,7 @@ struct Segment : Range {
   int first, rows;  // first token, query rows (tokens * group)
   int m0;           // the tile's first query row
   int row, slot;    // the batch row (own keys; -1: a prefix), the slot of the partial results
-  int see;          // query token i sees keys below see + i (own pages), or INT_MAX / 2 (a prefix)
+  int see;          // query token i sees own keys below see + i, and a prefix's all
 };
 
 __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, Segment &s) {
@@ -39,7 +39,6 @@ __device__ __forceinline__ bool prefix_segment(const Params &p, uint32_t item, S
   s.first = t.first;
   s.rows = t.count * p.group;
   s.m0 = tile * kRowsPerTile;
-  s.see = INT32_MAX / 2;
   s.slot = p.s_own + chunk;
   const int64_t begin = (int64_t)chunk * p.chunk_pre;
   s.end = (int)min(begin + p.chunk_pre, (int64_t)group_length(p, g));
@@ -78,8 +77,9 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
   const bool live = m < s.rows;
   const int i_q = live ? m / p.group : 0;
   const int token = s.first + i_q, q_head = s.head * p.group + (live ? m - i_q * p.group : 0);
-  const int limit = live ? min(s.end, s.see + i_q) : 0;  // this lane's query sees keys below it
-  const int every = min(s.end, s.see + s.m0 / p.group);  // and every query of the tile keys below this
+  const bool own = s.row >= 0;
+  const int limit = !live ? 0 : own ? min(s.end, s.see + i_q) : s.end;  // this lane's query sees keys below it
+  const int every = own ? min(s.end, s.see + s.m0 / p.group) : s.end;   // and every query of the tile keys below this
 
   typedef typename N::Step St;
   int page = s.begin < s.end ? St::look(p, s, s.begin) : -1;
@@ -105,7 +105,7 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
   for (int c = 0; c < QP; ++c) key_off[c] = L::key_at(n, 4 * c + g);
   const char *values = lds + St::kTile;
   float *logits = nullptr;  // of this lane's query row
-  if (p.logits != nullptr && s.row >= 0 && live)
+  if (p.logits != nullptr && own && live)
     logits = p.logits + (((int64_t)s.row * p.kv_heads + s.head) * p.logit_rows + m) * p.logit_stride;
 
   f32x4 acc[D / 16];

@@ -421,7 +421,7 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
   int g = uniform(s_group);
   int64_t group_at = uniform(s_at);
   s.table = nullptr;
-  s.see = 0;
+  s.see = INT32_MIN / 2;  // no own keys, whatever the query token: own + see + i would pass 2^31 behind the longest prefixes
   while (true) {
     const RowQueries t = group_queries(p, g);
     s.plen = s.own = uniform(group_length(p, g));
