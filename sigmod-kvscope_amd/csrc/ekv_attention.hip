@@ -409,7 +409,8 @@ __global__ __launch_bounds__(THREADS) void fold_kernel(const Params p, int piece
     if (lse == -INFINITY || key >= see + i_q) continue;  // it sees none of them (nor wrote their logits)
     const f32x4 x = *(const f32x4 *)(logits + (int64_t)m * p.logit_stride);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) total[i] += __builtin_amdgcn_exp2f(x[i] - lse * kLog2e);  // unseen ones are -inf
+    for (int i = 0; i < 4; ++i)  // unseen ones are -inf, and get nothing from a query of NaN either
+      total[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - lse * kLog2e);
   }
   float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
 #pragma unroll
