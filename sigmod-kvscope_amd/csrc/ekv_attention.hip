@@ -151,7 +151,7 @@ __device__ __forceinline__ void attend(const Params &p, const Segment &s, char *
     for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) high = fmaxf(high, x[k][i]);
-    const float peak = fmaxf(top, rows_max(high) - kLift<typename T::Half>);
+    const float peak = fmaxf(top, lifted<typename T::Half>(rows_max(high), kLift<typename T::Half>));
     const float ref = peak == -INFINITY ? 0.f : peak;
     if (!__all(top == peak)) {
       const float shrink = __builtin_amdgcn_exp2f(top - ref);

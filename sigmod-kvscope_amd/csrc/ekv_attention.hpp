@@ -96,6 +96,15 @@ template <class H>
 constexpr float kLift = 0.f;
 template <>
 inline constexpr float kLift<_Float16> = 15.f;
+// From so large logits on (in powers of two) float32's steps are too coarse to tell weights apart by, and nothing is lifted:
+// a lift that is rounded up passes f16's largest value.
+constexpr float kFar = 0x1p20f;
+// What the weights beside the largest logit `high` are against.
+template <class H>
+__device__ __forceinline__ float lifted(float high, float lift) {
+  if constexpr (kLift<H> == 0.f) return high;
+  return fabsf(high) < kFar ? high - lift : high;
+}
 
 struct F32 {
   static constexpr int kType = EKV_F32;

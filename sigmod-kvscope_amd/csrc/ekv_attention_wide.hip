@@ -178,6 +178,7 @@ __device__ __forceinline__ float other_half_sum(float v) {
 // leave the outputs unscaled.  Weights then reach 2^kSlack: 2^8 in bf16, and in f16 2^1, which leaves 2^14 of its lift.
 template <class H>
 constexpr float kSlack = kLift<H> > 0.f ? 1.f : 8.f;
+constexpr float kRounded = 0x1p12f;
 template <class H>
 constexpr float kWideLift = kLift<H> > 0.f ? kLift<H> - kSlack<H> : 0.f;
 
@@ -309,7 +310,7 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
       for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) high = fmaxf(high, x[k][i]);
-      high = other_half_max(high) * scale2 - kWideLift<H>;
+      high = lifted<H>(other_half_max(high) * scale2, kWideLift<H>);
       if (!__all(high <= top + kSlack<H>)) {
         const float peak = fmaxf(top, high);
         const float shrink = __builtin_amdgcn_exp2f(top - (peak == -INFINITY ? 0.f : peak));
@@ -319,12 +320,23 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
         top = peak;
       }
       const float ref = top == -INFINITY ? 0.f : top;
+      // ref is a rounded product, the weights' products are not: a common factor of all weights, less than half a step of f16
+      // from 1 below kRounded.  Far out it could be any power of two (and was NaN or 0 at the lowest values of a type), so
+      // from there on the products are rounded as ref was.
+      float factor = scale2;
+      if (__any(fabsf(ref) >= kRounded)) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[k][i] *= scale2;
+        factor = 1.f;
+      }
       products(y, odd);  // past the last step from keys that nothing needs
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          x[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], scale2, -ref));
+          x[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], factor, -ref));
           sum += x[k][i];
         }
 #pragma unroll
