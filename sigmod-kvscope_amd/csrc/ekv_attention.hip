@@ -410,7 +410,7 @@ __global__ __launch_bounds__(THREADS) void fold_kernel(const Params p, int piece
     const f32x4 x = *(const f32x4 *)(logits + (int64_t)m * p.logit_stride);
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // unseen ones are -inf, and get nothing from a query of NaN either
-      total[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - lse * kLog2e);
+      total[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(below_one(x[i] - lse * kLog2e));
   }
   float *out = p.scores + (int64_t)row * p.sc_row + (int64_t)head * p.sc_head;
 #pragma unroll
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void weigh_kernel(const Params p, int pie
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool sees = (ok >> (16 * k + i) & 1) != 0 && begin + 16 * k + 4 * g + i < limit;
-        total[k][i] += sees ? __builtin_amdgcn_exp2f(x[i] * p.scale2 - lse2) : 0.f;
+        total[k][i] += sees ? __builtin_amdgcn_exp2f(below_one(x[i] * p.scale2 - lse2)) : 0.f;
       }
     }
   }

@@ -99,6 +99,8 @@ inline constexpr float kLift<_Float16> = 15.f;
 // From so large logits on (in powers of two) float32's steps are too coarse to tell weights apart by, and nothing is lifted:
 // a lift that is rounded up passes f16's largest value.
 constexpr float kFar = 0x1p20f;
+// Below this the rounding of a logit is less than half a step of f16 in its weight.
+constexpr float kRounded = 0x1p12f;
 // What the weights beside the largest logit `high` are against.
 template <class H>
 __device__ __forceinline__ float lifted(float high, float lift) {
@@ -330,6 +332,10 @@ __device__ __forceinline__ u32x2 read_transposed(const char *from) {
   typedef __attribute__((address_space(3))) s16x4 *Ptr;
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(from)));
 }
+
+// A key's logit less its query's lse.  The weight, 2 to that power, is at most 1: where logits are so large that their
+// roundings are whole powers of two, a difference above 0 is one of those.  NaN stays NaN.
+__device__ __forceinline__ float below_one(float difference) { return __builtin_elementwise_minimum(difference, 0.f); }
 
 // -- segments of work -------------------------------------------------------------------------------
 

@@ -178,7 +178,6 @@ __device__ __forceinline__ float other_half_sum(float v) {
 // leave the outputs unscaled.  Weights then reach 2^kSlack: 2^8 in bf16, and in f16 2^1, which leaves 2^14 of its lift.
 template <class H>
 constexpr float kSlack = kLift<H> > 0.f ? 1.f : 8.f;
-constexpr float kRounded = 0x1p12f;
 template <class H>
 constexpr float kWideLift = kLift<H> > 0.f ? kLift<H> - kSlack<H> : 0.f;
 
@@ -225,6 +224,7 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float top = -INFINITY, sum = 0.f;
+  bool far = false;  // a query of the wave has a maximum of kRounded or more, either sign
 
   // The softmax of a step's logits runs beside the next step's products, so keys are a step ahead of values: step t
   // has its logits already, stores keys t + 2 over keys t, and values t + 1 over values t - 1.
@@ -318,13 +318,14 @@ __device__ __forceinline__ void attend_wide(const Params &p, const Item &s, char
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] *= shrink;
         top = peak;
+        far = __any(fabsf(top) >= kRounded && top != -INFINITY);
       }
       const float ref = top == -INFINITY ? 0.f : top;
       // ref is a rounded product, the weights' products are not: a common factor of all weights, less than half a step of f16
       // from 1 below kRounded.  Far out it could be any power of two (and was NaN or 0 at the lowest values of a type), so
       // from there on the products are rounded as ref was.
       float factor = scale2;
-      if (__any(fabsf(ref) >= kRounded)) {
+      if (far) {
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -546,6 +547,15 @@ __global__ __launch_bounds__((kPerGroup<D> * kWave), (D == 256 ? 1 : 2)) void we
 #pragma unroll
       for (int c = 0; c < C; ++c) x[k] = mfma32(key[k][c], y.q[c], x[k], H{});
     }
+    float factor = p.scale2, lse2 = y.lse2;
+    if (__any(fabsf(y.lse2) >= kRounded && y.lse2 != INFINITY)) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[k][i] = below_one(x[k][i] * p.scale2 - y.lse2);
+      factor = 1.f;
+      lse2 = 0.f;
+    }
     if (~ok != 0 || !__all(y.limit >= begin + kWeighKeys)) {
       const uint64_t mine = ok >> (4 * half);
 #pragma unroll
@@ -554,13 +564,13 @@ __global__ __launch_bounds__((kPerGroup<D> * kWave), (D == 256 ? 1 : 2)) void we
         for (int i = 0; i < 16; ++i) {
           const int j = 32 * k + 8 * (i / 4) + i % 4;
           const bool sees = (mine >> j & 1) != 0 && begin + j + 4 * half < y.limit;
-          total[k][i] += sees ? __builtin_amdgcn_exp2f(x[k][i] * p.scale2 - y.lse2) : 0.f;
+          total[k][i] += sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], factor, -lse2)) : 0.f;
         }
     } else {
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) total[k][i] += __builtin_amdgcn_exp2f(x[k][i] * p.scale2 - y.lse2);
+        for (int i = 0; i < 16; ++i) total[k][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], factor, -lse2));
     }
   };
   // queries before the first key see none of them

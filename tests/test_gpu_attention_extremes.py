@@ -125,3 +125,23 @@ def test_equal_weights_of_every_size(dtype, counts, scale):
             assert np.all(np.abs(out[token].double().cpu().numpy() - mean) <= bound), (r, i)
             token += 1
     assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("scale", [-3e31, -1e9, -40.0, 7.0, 83.0, 1e3, 1e7, 3e31])
+@pytest.mark.parametrize("counts,group", [(None, 2), ([9, 9], 2), ([40, 70], 2), ([140, 150], 4)],
+                         ids=["kept", "again", "wide", "workgroups"])
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_a_weight_is_at_most_one(dtype, counts, group, scale):
+    # float32's steps of such logits are whole powers of two: what a weight is, its lse cannot say, but no more than 1
+    b = Batch([180, 190], counts=counts, prefixes=[21], heads=1, group=group, dtype=dtype, seed=45).with_scores()
+    b.k_scale = b.v_scale = 1.0
+    b.cache[:, 0], b.query[:] = 120.0, 140.0
+    b.scale = scale
+    old = b.scores.double().numpy()
+    _, _, scores = run(b)
+    got, queries = scores.double().cpu().numpy(), b.max_query * group
+    for r, n in enumerate(b.lens):
+        held = old[r, :, :n] * b.decay
+        slack = (queries + 8) * 2.0**-24 * (held + queries)  # of as many additions
+        assert np.all(got[r, :, :n] >= held - slack) and np.all(got[r, :, :n] <= held + queries + slack)
+        assert np.array_equal(got[r, :, n:], old[r, :, n:])
