@@ -519,13 +519,17 @@ typedef struct ekv_attention {
  *     lse = log sum exp(s)        out = v_scale * sum exp(s - lse) v
  * and a query that sees nothing has out 0 and lse -inf.  A table entry that is no page of the cache
  * (negative, or blocks and more) is as if its tokens were not there.  What the cache holds in slots that
- * no query of the row sees is never used, whatever it is.  A prefix's pages are read for all the queries
+ * no query of the row sees is never used, whatever it is; an infinite or NaN value that only some of a
+ * row's queries see may reach the others (0 times it is NaN).  A prefix's pages are read for all queries
  * of its group together, except where rows bring so many queries each, or the prefixes (by prefix_width)
- * are so short, that a walk of each row's own is faster.  Tokens of no row, and of a row past its max_query-th, get out 0 and lse -inf.
+ * are so short, that a walk of each row's own is faster.  Tokens of no row, and of a row past its
+ * max_query-th, get out 0 and lse -inf.
  * With `scores`, each own slot j < lens[r] also accumulates the weight its key received:
  *     scores[r, h, j] = decay * scores[r, h, j] + sum over the row's queries of head h of exp(s - lse)
- * (other slots are left alone).  Logits, maxima, sums and scores are float32; of 16-bit and fp8 caches a weight
- * is rounded to the queries' type before it meets a value.  No atomics, so equal calls give equal bits.
+ * (other slots are left alone; a weight is at most 1, and as exact as a float32 lse lets it be).  Logits,
+ * maxima, sums and scores are float32, logits times log2(e) within its range; of 16-bit and fp8 caches a
+ * weight is rounded to the queries' type before it meets a value.  No atomics, so equal calls give equal
+ * bits.
  * Types: fp32, f16 and bf16 with keys and values of the same type, or fp8 e4m3 keys and values with bf16
  * queries.  head_dim 32, 64, 128 or 256; any block size and any number of query heads per KV head; rows of
  * the query, keys and values start at multiples of 16 bytes; width * block_size below 2^31 - 4096.

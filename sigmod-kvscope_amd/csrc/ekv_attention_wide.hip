@@ -10,8 +10,8 @@
 // of one dim a lane.  The weights' rounding (half a step of the type, relative) is of the size of the
 // output's own; their sum, the maxima and the outputs are float32.
 //
-// Measured, head dim 128: 3200 f16 query rows a KV head against prefixes of 32768 tokens 550 us (740 TFLOP/s, with
-// the own tokens and the join); bf16 prompt chunks of up to 4096 rows 270 us (680 TFLOP/s).  The narrow form of the
+// Measured, head dim 128: 3200 f16 query rows a KV head against prefixes of 32768 tokens 550 to 614 us as the clock goes
+// (740 TFLOP/s at best, with the own tokens and the join); bf16 prompt chunks of up to 4096 rows 273 us (675 TFLOP/s).  The narrow form of the
 // same calls, one wave for 16 query rows, took 2456 and 1247 us.
 #include "ekv_attention.hpp"
 
@@ -411,7 +411,7 @@ __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wi
 
 // The prefixes: the steps of every (group, tile) are one list, which the workgroups that the chip holds share
 // equally.  (In chunks of equal length 648 workgroups had work where 512 fit: 1.24 waves a SIMD over the launch, 574 us
-// for 3200 query rows against prefixes of 32768 tokens; in equal shares 558 us at the time, now 471.)
+// for 3200 query rows against prefixes of 32768 tokens; in equal shares 558 us at the time, now 470 to 500.)
 template <class T, int D>
 __global__ __launch_bounds__((Wide<T, D>::kThreads), (D == 256 ? 1 : 2)) void wide_prefix_kernel(const Params p) {
   using W = Wide<T, D>;
