@@ -581,6 +581,96 @@ typedef struct ekv_eviction {
 size_t ekv_evict_tokens_workspace(int32_t rows, int32_t kv_heads, int32_t capacity);
 int ekv_evict_tokens(const ekv_eviction_t *a, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The arguments of ekv_rotate_heads.  Strides count elements; a head's elements are contiguous. */
+typedef struct ekv_rotation {
+  const void *query;            /* [tokens, q_heads, head_dim], or NULL with q_heads 0 */
+  int64_t q_stride_token, q_stride_head;
+  const void *key;              /* [tokens, kv_heads, head_dim], or NULL with kv_heads 0 */
+  int64_t k_stride_token, k_stride_head;
+  void *q_out;                  /* query itself with its strides, or a buffer that does not overlap the inputs */
+  int64_t q_out_stride_token, q_out_stride_head;
+  void *k_out;                  /* key itself with its strides, or a buffer that does not overlap the inputs */
+  int64_t k_out_stride_token, k_out_stride_head;
+  const int32_t *positions;     /* [axis_count, tokens] */
+  int64_t positions_stride;
+  const double *frequencies;    /* [pairs]: radians a position */
+  const int32_t *axes;          /* [pairs]: the axis whose position turns the pair (NULL: axis 0) */
+  const void *q_weight, *k_weight; /* [head_dim] of every head, or [heads, head_dim]; NULL: no norm */
+  int64_t q_weight_stride, k_weight_stride; /* elements from one head's weights to the next's (0: the same) */
+  int32_t dtype, weight_dtype, tokens, q_heads, kv_heads, head_dim, pairs, axis_count, adjacent;
+  float rotary_scale, eps, weight_offset;
+} ekv_rotation_t;
+
+/*
+ * Norms of each query and key head and the rotation of their positions, in one pass.  No counterpart in the
+ * reference, which leaves what runs before attention to the serving engine.
+ *
+ * Of a head's elements x, with weights w:  y_i = x_i / sqrt(mean of x^2 + eps) * (weight_offset + w_i),
+ * and y = x without weights.  Pair p is (y_p, y_{p + pairs}), or (y_{2p}, y_{2p + 1}) with `adjacent`; it
+ * turns by a = positions[axes[p]][token] * frequencies[p] radians:
+ *     (u, v) -> rotary_scale * (u cos a - v sin a, u sin a + v cos a)
+ * Elements from 2 * pairs on stay as they are.  An axis outside [0, axis_count) is position 0.  A token's
+ * norms and rotations are float32, its angles float64 until they are less than a turn; the result is
+ * rounded once, to the inputs' type.
+ * Types: fp32, f16 or bf16; weights of the same type or fp32.  head_dim a multiple of 16, at most 256; pairs
+ * a multiple of 8 (0: norms alone); rows of every tensor start at multiples of 16 bytes.
+ */
+int ekv_rotate_heads(const ekv_rotation_t *a, void *stream);
+
+/* The arguments of ekv_append_tokens.  Strides count elements; a head's elements are contiguous. */
+typedef struct ekv_append {
+  const void *query;            /* [tokens, q_heads, head_dim], or NULL with q_heads 0 */
+  int64_t q_stride_token, q_stride_head;
+  const void *new_keys, *new_values; /* [tokens, kv_heads, head_dim] */
+  int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+  void *q_out;                  /* query itself with its strides, or a buffer that does not overlap the inputs */
+  int64_t q_out_stride_token, q_out_stride_head;
+  void *keys, *values;          /* the cache: element (block, pos, head, dim), both with the strides below */
+  int64_t kv_stride_block, kv_stride_pos, kv_stride_head;
+  int64_t blocks;               /* pages of the cache */
+  const int32_t *table;         /* [rows, width]: pages that no other row uses */
+  int64_t table_stride;
+  int32_t *lens;                /* [rows]: the rows' tokens, the new ones included (not yet, with advance) */
+  int32_t *seen;                /* [rows]: the position of the row's next token, likewise; NULL: lens */
+  const int32_t *first;         /* [rows]: the position of the row's first token; NULL: 0 */
+  int64_t first_stride;         /* 0: the same for every row */
+  const int32_t *q_start;       /* [rows + 1] or NULL: a token a row */
+  const int32_t *positions;     /* [axis_count, tokens], or NULL: first + the token's place in its row */
+  int64_t positions_stride;
+  const double *frequencies;    /* as in ekv_rotation_t */
+  const int32_t *axes;
+  const void *q_weight, *k_weight;
+  int64_t q_weight_stride, k_weight_stride;
+  float *scores;                /* [rows, kv_heads, >= width * block_size] or NULL */
+  int64_t scores_stride_row, scores_stride_head;
+  int32_t *slot_positions;      /* [rows, kv_heads, >= width * block_size] or NULL */
+  int64_t slot_positions_stride_row, slot_positions_stride_head;
+  int32_t dtype, weight_dtype, kv_dtype, rows, width, tokens, max_query, q_heads, kv_heads, head_dim, block_size;
+  int32_t pairs, axis_count, adjacent, advance, saturate;
+  float rotary_scale, eps, weight_offset, k_scale, v_scale;
+  int32_t pad;
+} ekv_append_t;
+
+/*
+ * Appends a batch's new keys and values to its rows of a paged cache, the keys normed and rotated on the way
+ * as ekv_rotate_heads does, and the queries beside them.  No counterpart in the reference.
+ *
+ * Row r's t new tokens are [q_start[r], q_start[r + 1]) of the call's (ascending; what lies outside the
+ * tokens is cut off).  With n = lens[r], at most width * block_size, token i of them takes slot n - t + i,
+ * or n + i with advance.  Its index is seen[r] - t + i (seen[r] + i with advance), or its slot without
+ * `seen`; its position, where `positions` are not given, first[r] + index.
+ * The slot's key becomes the rotated key / k_scale, its value the value / v_scale, rounded once to the
+ * cache's type.  An fp8 cache holds what passes +-448 as +-448 with saturate, as NaN without; NaN stays.
+ * scores at the slot become 0 and slot_positions the index, for every KV head.  A slot outside the row's
+ * table, and one whose table entry is no page of the cache, is not written (of the latter, scores and
+ * slot_positions are).  A row keeps its first max_query tokens.  With advance, lens[r] then grows by the
+ * tokens kept, but not past width * block_size, and seen[r] by as many as there were within max_query.
+ * Tokens of no row (before the first, behind the last, past max_query) write nothing and get q_out 0.
+ * Types: new tokens and queries fp32, f16 or bf16; the cache the same, or fp8 e4m3; limits as
+ * ekv_rotate_heads has them, and width * block_size below 2^31 - 4096.
+ */
+int ekv_append_tokens(const ekv_append_t *a, void *stream);
+
 /*
  * Device memory, copies and IPC for the statistic planes.  They replace the ctypes calls
  * into libcudart of runtime/audit.py:17-23, :55-60, runtime/audit_kernel.py:146-158 and

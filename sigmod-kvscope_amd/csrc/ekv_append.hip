@@ -1,0 +1,614 @@
+// Tokens on their way from the projection to attention: norms of each query and key head, the rotation of
+// their positions, and the keys' and values' place in a paged cache.  One kernel does a token's heads in one
+// pass; ekv_rotate_heads leaves the cache out.
+//
+// Mathematics.  A head is a vector x of dim elements.  Its norm is y = x * rsqrt(mean(x^2) + eps) * w; pair p of it
+// is a complex number that turns by pos * f_p radians.  Angles of far positions lose everything in float32 (a
+// million radians have steps of 1/16), so pos * f_p / 2 pi is float64 until its whole turns are gone.
+//
+// Bound.  Every input is read once and every output written once, 3 or 4 flop an element: bandwidth, or a launch's
+// latency where the tokens are few.
+//
+// Layout.  A head's pairs are cut into units of 8, a unit a lane: the 8 elements of the first halves and the 8 of the
+// second ones, two loads of 16 bytes (of 16-bit types).  A lane then holds whole pairs in either order of them and
+// needs nothing of another lane for the rotation; elements that do not rotate are units of the same shape.  The G
+// lanes of a head (a power of two; a head dim that is none leaves some idle) lie in one row of 16 lanes, so that the
+// sum of squares is a few DPP moves.  A wave has 64 / G heads of one token at a time.  The cosines and sines of a
+// token are computed once a wave, a pair a lane, and pass through LDS to the lanes whose units they turn: 8 times
+// fewer than if each lane computed its own.
+#include "ekv_attention.hpp"
+
+namespace ekv {
+namespace append {
+
+using attn::f32x4;
+using attn::pack2;
+using attn::u32x2;
+using attn::u32x4;
+
+constexpr int kWaves = 4;         // of a workgroup
+constexpr int kMostPairs = 128;   // of a head
+constexpr int kUnit = 8;          // pairs of a lane
+
+struct Heads {  // one tensor [tokens, heads, dim]: strides in bytes
+  const char *at;
+  int64_t token, head;
+};
+// The stride of an axis of one element is whatever it is, and not used.
+inline Heads heads_of(const void *at, int64_t token, int64_t head, int tokens, int heads, int bytes) {
+  return {(const char *)at, tokens > 1 ? token * bytes : 0, heads > 1 ? head * bytes : 0};
+}
+
+struct Params {
+  Heads q, k, v, q_out, k_out;
+  char *keys, *values;  // the cache, strides in bytes
+  int64_t st_block, st_pos, st_head, blocks;
+  const int32_t *table;
+  int64_t table_stride;
+  int32_t *lens, *seen;
+  const int32_t *first;
+  int64_t first_stride;
+  const int32_t *q_start, *positions;
+  int64_t positions_stride;
+  const double *frequencies;
+  const int32_t *axes;
+  const char *q_weight, *k_weight;
+  int64_t q_weight_stride, k_weight_stride;  // bytes
+  float *scores;
+  int64_t sc_row, sc_head;
+  int32_t *slot_positions;
+  int64_t sp_row, sp_head;
+  int rows, width, tokens, max_query, q_heads, kv_heads, dim, pairs, axis_count, block_size;
+  uint32_t bs_mul;  // page_divisor(block_size)
+  int bs_shift;
+  bool adjacent, advance, saturate, weight_f32;
+  int parts;   // waves of a token: 1, 2 or 4
+  int passes;  // of 64 / G heads that the token's heads take, shared by its waves
+  float rotary_scale, eps, weight_offset, k_inverse, v_inverse, mean;  // mean: 1 / dim
+};
+
+// -- elements -------------------------------------------------------------------------------------
+
+template <class T>
+struct Unit {  // 8 elements as they lie in memory
+  u32x4 w;
+};
+template <>
+struct Unit<float> {
+  u32x4 w, more;
+};
+
+template <class T>
+__device__ __forceinline__ Unit<T> load_unit(const char *at) {
+  const auto *p = as_global((const u32x4 *)at);
+  if constexpr (sizeof(T) == 4) return {p[0], p[1]};
+  else return {p[0]};
+}
+
+__device__ __forceinline__ void widen(const Unit<float> &u, float (&x)[kUnit]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = __builtin_bit_cast(f32x4, u.w)[e];
+    x[4 + e] = __builtin_bit_cast(f32x4, u.more)[e];
+  }
+}
+__device__ __forceinline__ void widen(const Unit<__bf16> &u, float (&x)[kUnit]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __builtin_bit_cast(float, u.w[e] << 16);
+    x[2 * e + 1] = __builtin_bit_cast(float, u.w[e] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void widen(const Unit<_Float16> &u, float (&x)[kUnit]) {
+  const attn::f16x8 h = __builtin_bit_cast(attn::f16x8, u.w);
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) x[e] = (float)h[e];
+}
+
+// The largest finite e4m3 value for what passes it; NaN stays.
+__device__ __forceinline__ float within_e4m3(float x) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 448.f), -448.f);
+}
+
+template <class C>
+__device__ __forceinline__ void store_unit(char *at, const float (&x)[kUnit], bool saturate) {
+  if constexpr (std::is_same<C, float>::value) {
+    auto *p = as_global((f32x4 *)at);
+    p[0] = f32x4{x[0], x[1], x[2], x[3]};
+    p[1] = f32x4{x[4], x[5], x[6], x[7]};
+  } else if constexpr (std::is_same<C, attn::FP8>::value) {
+    float y[kUnit];
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) y[e] = saturate ? within_e4m3(x[e]) : x[e];
+    u32x2 w;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], word, true);
+    }
+    *as_global((u32x2 *)at) = w;
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1], C{});
+    *as_global((u32x4 *)at) = w;
+  }
+}
+
+template <class C>
+constexpr int kBytes = std::is_same<C, float>::value ? 4 : std::is_same<C, attn::FP8>::value ? 1 : 2;
+
+// Sum over the G lanes of a head, every one of them receiving it.  All lanes of the wave are active.
+template <int G>
+__device__ __forceinline__ float head_sum(float v) {
+  auto add = [&](auto ctrl) {
+    v += __builtin_bit_cast(float, dpp_move<decltype(ctrl)::value>(__builtin_bit_cast(int, v)));
+  };
+  add(std::integral_constant<int, 0xB1>());                         // quad_perm [1, 0, 3, 2]
+  if constexpr (G >= 4) add(std::integral_constant<int, 0x4E>());   // quad_perm [2, 3, 0, 1]
+  if constexpr (G >= 8) add(std::integral_constant<int, 0x141>());  // row_half_mirror: the other quad of 8 lanes
+  if constexpr (G >= 16) add(std::integral_constant<int, 0x140>()); // row_mirror: the other 8 of 16 lanes
+  return v;
+}
+
+// -- where a token belongs ------------------------------------------------------------------------
+
+struct Place {
+  bool live;      // the token is one of a row's first max_query
+  int row;
+  int64_t slot, index;
+  bool in_table;  // the slot is one of the row's table
+  int64_t page;   // of the slot, -1 for none
+};
+
+__device__ __forceinline__ int capacity(const Params &p) { return p.width * p.block_size; }  // below 2^31 - 4096
+
+// How many of the ascending a[0 .. n) are at most `token`: 64 ways at a step, so that a few hundred rows are two loads
+// behind each other where halving takes eight.
+__device__ __forceinline__ int count_up_to(const int32_t *a, int n, int token) {
+  const int lane = lane_id();
+  int below = 0;
+  while (n > kWave) {
+    const int step = (n + kWave - 1) / kWave, i = (lane + 1) * step - 1;
+    const bool low = i < n && a[below + i] <= token;
+    const int whole = __popcll(__ballot(low)) * step;
+    below += whole;
+    n = min(step, n - whole);
+  }
+  const bool low = lane < n && a[below + lane] <= token;
+  return below + __popcll(__ballot(low));
+}
+
+__device__ __forceinline__ Place place_of(const Params &p, int token) {
+  Place at{false, 0, 0, 0, false, -1};
+  int count = 1, nth = 0;
+  at.row = token;
+  if (p.q_start != nullptr) {
+    at.row = count_up_to(p.q_start, p.rows, token) - 1;
+    if (at.row < 0) return at;
+    const int a = min(max(p.q_start[at.row], 0), p.tokens);
+    const int b = min(max(p.q_start[at.row + 1], a), p.tokens);
+    count = b - a;
+    nth = token - a;
+  }
+  at.live = nth < count && nth < p.max_query;
+  if (!at.live) return at;
+  const int len = min(max(p.lens[at.row], 0), capacity(p));
+  const int back = p.advance ? 0 : count;
+  at.slot = (int64_t)len - back + nth;
+  at.index = p.seen != nullptr ? (int64_t)p.seen[at.row] - back + nth : at.slot;
+  at.in_table = at.slot >= 0 && at.slot < capacity(p);
+  if (at.in_table) {
+    const int32_t page = p.table[at.row * p.table_stride + (int)(__umulhi((uint32_t)at.slot << 1, p.bs_mul) >> p.bs_shift)];
+    at.page = page >= 0 && page < p.blocks ? page : -1;
+  }
+  return at;
+}
+
+// What a row of t tokens becomes when they are in.
+__device__ __forceinline__ void advance_row(const Params &p, int row, int t) {
+  const int kept = min(t, p.max_query), len = min(max(p.lens[row], 0), capacity(p));
+  if (kept <= 0) return;
+  p.lens[row] = len + min(kept, capacity(p) - len);
+  if (p.seen != nullptr) p.seen[row] += kept;
+}
+
+// -- the pass ---------------------------------------------------------------------------------------
+
+// T: the inputs' type.  C: the cache's (FP8 or T).  G: lanes of a head.  PAGED: with a cache and values; else keys go to
+// k_out.
+template <class T, class C, int G, bool PAGED>
+__global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
+  constexpr int kPer = kWave / G;  // heads of a pass
+  __shared__ __align__(16) float s_cos[kWaves][kMostPairs], s_sin[kWaves][kMostPairs];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
+  const int64_t token = item / p.parts;
+  const int part = (int)(item % p.parts);
+  const bool here = token < p.tokens;
+
+  if (here) {
+    const int heads = p.q_heads + (PAGED ? 2 : 1) * p.kv_heads;
+    const int unit = lane % G, turning = p.pairs / kUnit, rest = p.dim - 2 * p.pairs;
+    const bool active = unit * 2 * kUnit < p.dim, turns = unit < turning;
+    // the lane's elements: [a, a + 8) and [b, b + 8)
+    const int a = turns ? unit * kUnit : 2 * p.pairs + (unit - turning) * kUnit;
+    const int b = turns ? p.pairs + a : a + rest / 2;
+
+    const char *const q_at = p.q.at + token * p.q.token, *const k_at = p.k.at + token * p.k.token;
+    const char *const v_at = p.v.at + token * p.v.token;
+    auto source = [&](int head) {
+      if (head < p.q_heads) return q_at + head * p.q.head;
+      head -= p.q_heads;
+      if (!PAGED || head < p.kv_heads) return k_at + head * p.k.head;
+      return v_at + (head - p.kv_heads) * p.v.head;
+    };
+    Unit<T> ua{}, ub{};
+    auto fetch = [&](int pass) {
+      const int head = pass * kPer + lane / G;
+      if (active && head < heads) {
+        const char *x = source(head);
+        ua = load_unit<T>(x + a * sizeof(T));
+        ub = load_unit<T>(x + b * sizeof(T));
+      }
+    };
+    int pass = part;
+    if (pass < p.passes) fetch(pass);  // on their way while the token finds its place
+
+    Place at{true, 0, 0, 0, false, -1};
+    if constexpr (PAGED) at = place_of(p, (int)token);
+
+    // the token's cosines and sines
+    float cosine[kUnit], sine[kUnit];
+    if (p.pairs > 0) {
+      int64_t own = at.index;
+      if (PAGED && p.first != nullptr && at.live) own += p.first[at.row * p.first_stride];
+      for (int i = lane; i < p.pairs; i += kWave) {
+        const int axis = p.axes != nullptr ? p.axes[i] : 0;
+        double pos = (double)own;
+        if (p.positions != nullptr)
+          pos = (uint32_t)axis < (uint32_t)p.axis_count ? (double)p.positions[axis * p.positions_stride + token] : 0.0;
+        const double turn = pos * p.frequencies[i] * 0.15915494309189533577;  // 1 / 2 pi
+        const float x = (float)(turn - __builtin_rint(turn));
+        float s, c;
+        sincospif(2.f * x, &s, &c);
+        s_cos[wave][i] = c * p.rotary_scale;
+        s_sin[wave][i] = s * p.rotary_scale;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (turns) {
+        if (p.adjacent) {  // [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            cosine[e] = s_cos[wave][a / 2 + e];
+            sine[e] = s_sin[wave][a / 2 + e];
+            cosine[4 + e] = s_cos[wave][b / 2 + e];
+            sine[4 + e] = s_sin[wave][b / 2 + e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) {
+            cosine[e] = s_cos[wave][a + e];
+            sine[e] = s_sin[wave][a + e];
+          }
+        }
+      }
+    }
+
+    int64_t in_page = 0;
+    if constexpr (PAGED) {
+      if (at.page >= 0) {
+        const int64_t block = __umulhi((uint32_t)at.slot << 1, p.bs_mul) >> p.bs_shift;
+        in_page = at.page * p.st_block + (at.slot - block * p.block_size) * p.st_pos;
+      }
+      if (part == 0 && at.live && at.in_table) {  // a new slot has no weight yet
+        for (int h = lane; h < p.kv_heads; h += kWave) {
+          if (p.scores != nullptr) p.scores[at.row * p.sc_row + h * p.sc_head + at.slot] = 0.f;
+          if (p.slot_positions != nullptr) p.slot_positions[at.row * p.sp_row + h * p.sp_head + at.slot] = (int32_t)at.index;
+        }
+      }
+    }
+
+    for (; pass < p.passes; pass += p.parts) {
+      const int head = pass * kPer + lane / G;
+      const bool is_q = head < p.q_heads, is_v = PAGED && head >= p.q_heads + p.kv_heads;
+      const bool mine = active && head < heads;
+      float x[kUnit] = {}, y[kUnit] = {};
+      if (mine) {
+        widen(ua, x);
+        widen(ub, y);
+      }
+      if (pass + p.parts < p.passes) fetch(pass + p.parts);
+      if (p.q_weight != nullptr || p.k_weight != nullptr) {
+        const char *w = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
+        float squares = 0.f;
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) squares += x[e] * x[e] + y[e] * y[e];
+        squares = head_sum<G>(squares);
+        float over = rsqrtf(squares * p.mean + p.eps);
+        if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
+          float small = 0.f;
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) {
+            const float u = x[e] * 0x1p-80f, v = y[e] * 0x1p-80f;
+            small += u * u + v * v;
+          }
+          small = head_sum<G>(small);
+          if (squares == __builtin_inff()) over = rsqrtf(small * p.mean) * 0x1p-80f;
+        }
+        if (w != nullptr && mine) {
+          float wa[kUnit], wb[kUnit];
+          if (p.weight_f32) {
+            const char *row = w + (is_q ? head * p.q_weight_stride : (head - p.q_heads) * p.k_weight_stride);
+            widen(load_unit<float>(row + a * 4), wa);
+            widen(load_unit<float>(row + b * 4), wb);
+          } else {
+            const char *row = w + (is_q ? head * p.q_weight_stride : (head - p.q_heads) * p.k_weight_stride);
+            widen(load_unit<T>(row + a * sizeof(T)), wa);
+            widen(load_unit<T>(row + b * sizeof(T)), wb);
+          }
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) {
+            x[e] *= over * (p.weight_offset + wa[e]);
+            y[e] *= over * (p.weight_offset + wb[e]);
+          }
+        }
+      }
+      if (turns && !is_v) {
+        if (p.adjacent) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u = x[2 * e], v = x[2 * e + 1], r = y[2 * e], s = y[2 * e + 1];
+            x[2 * e] = u * cosine[e] - v * sine[e];
+            x[2 * e + 1] = u * sine[e] + v * cosine[e];
+            y[2 * e] = r * cosine[4 + e] - s * sine[4 + e];
+            y[2 * e + 1] = r * sine[4 + e] + s * cosine[4 + e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) {
+            const float u = x[e], v = y[e];
+            x[e] = u * cosine[e] - v * sine[e];
+            y[e] = u * sine[e] + v * cosine[e];
+          }
+        }
+      }
+      if (!mine) continue;
+      if (is_q) {
+        char *to = (char *)p.q_out.at + token * p.q_out.token + head * p.q_out.head;
+        if (!at.live) {
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) x[e] = y[e] = 0.f;
+        }
+        store_unit<T>(to + a * kBytes<T>, x, false);
+        store_unit<T>(to + b * kBytes<T>, y, false);
+      } else if constexpr (!PAGED) {
+        char *to = (char *)p.k_out.at + token * p.k_out.token + (head - p.q_heads) * p.k_out.head;
+        store_unit<T>(to + a * kBytes<T>, x, false);
+        store_unit<T>(to + b * kBytes<T>, y, false);
+      } else if (at.page >= 0) {
+        const int kv = head - p.q_heads - (is_v ? p.kv_heads : 0);
+        char *to = (is_v ? p.values : p.keys) + in_page + kv * p.st_head;
+        const float inverse = is_v ? p.v_inverse : p.k_inverse;
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) {
+          x[e] *= inverse;
+          y[e] *= inverse;
+        }
+        store_unit<C>(to + a * kBytes<C>, x, p.saturate);
+        store_unit<C>(to + b * kBytes<C>, y, p.saturate);
+      }
+    }
+  }
+  if constexpr (PAGED) {
+    // Without q_start a row's token is one workgroup's, whose waves have all read the row's length by now; else
+    // advance_kernel runs behind this one.
+    if (p.advance && p.q_start == nullptr) {
+      __syncthreads();
+      if (here && part == 0 && lane == 0) advance_row(p, (int)token, 1);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void advance_kernel(Params p) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= p.rows) return;
+  const int a = min(max(p.q_start[row], 0), p.tokens);
+  const int b = min(max(p.q_start[row + 1], a), p.tokens);
+  advance_row(p, row, b - a);
+}
+
+// -- host -----------------------------------------------------------------------------------------
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <class T, class C, int G, bool PAGED>
+int launch_group(Params p, hipStream_t stream, const char *who) {
+  const int heads = p.q_heads + (PAGED ? 2 : 1) * p.kv_heads;
+  p.passes = (int)ceil_div(heads, kWave / G);
+  // Waves of a token: four while that does not fill the chip, so that a pass of the heads is not behind another; one where
+  // there are tokens enough, which share a token's angles.
+  const int64_t enough = 16ll * cu_count();
+  p.parts = p.tokens * 4ll <= enough ? 4 : p.tokens * 2ll <= enough ? 2 : 1;
+  while (p.parts > 1 && p.parts / 2 >= p.passes) p.parts /= 2;
+  const int64_t grid = ceil_div((int64_t)p.tokens * p.parts, kWaves);
+  hipLaunchKernelGGL((heads_kernel<T, C, G, PAGED>), dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream, p);
+  return check_hip(hipGetLastError(), who);
+}
+
+template <class T, class C, bool PAGED>
+int launch_dim(const Params &p, hipStream_t stream, const char *who) {
+  if (p.dim <= 32) return launch_group<T, C, 2, PAGED>(p, stream, who);
+  if (p.dim <= 64) return launch_group<T, C, 4, PAGED>(p, stream, who);
+  if (p.dim <= 128) return launch_group<T, C, 8, PAGED>(p, stream, who);
+  return launch_group<T, C, 16, PAGED>(p, stream, who);
+}
+
+template <class T>
+int launch_cache(const Params &p, bool fp8, hipStream_t stream) {
+  return fp8 ? launch_dim<T, attn::FP8, true>(p, stream, "ekv_append_tokens launch")
+             : launch_dim<T, T, true>(p, stream, "ekv_append_tokens launch");
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+int bytes_of(int dtype) { return dtype == EKV_F32 ? 4 : dtype == EKV_FP8_E4M3 ? 1 : 2; }
+
+// The checks and parameters that both entry points share; `Block` is either one's arguments.
+template <class Block>
+int fill(const Block *a, Params &p, const char *who) {
+  if (a->dtype != EKV_F32 && a->dtype != EKV_F16 && a->dtype != EKV_BF16)
+    return fail(EKV_EUNSUPPORTED, "%s: heads of type %d", who, a->dtype);
+  if ((a->q_weight != nullptr || a->k_weight != nullptr) && a->weight_dtype != a->dtype && a->weight_dtype != EKV_F32)
+    return fail(EKV_EUNSUPPORTED, "%s: weights of type %d with heads of type %d", who, a->weight_dtype, a->dtype);
+  if (a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16 != 0)
+    return fail(EKV_EUNSUPPORTED, "%s: head dim %d (a multiple of 16, at most 256)", who, a->head_dim);
+  if (a->pairs < 0 || a->pairs % kUnit != 0 || 2 * a->pairs > a->head_dim)
+    return fail(EKV_EUNSUPPORTED, "%s: %d rotated pairs of a head of %d (a multiple of 8, at most half)", who, a->pairs,
+                a->head_dim);
+  if (a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > (1 << 20) || a->kv_heads > (1 << 20))
+    return fail(EKV_EINVAL, "%s: tokens %d, heads %d / %d", who, a->tokens, a->q_heads, a->kv_heads);
+  if (a->pairs > 0 && a->frequencies == nullptr) return fail(EKV_EINVAL, "%s: null pointer (frequencies)", who);
+  if (a->pairs > 0 && a->positions != nullptr &&
+      (a->axis_count < 1 || (a->axis_count > 1 && a->positions_stride < a->tokens)))
+    return fail(EKV_EINVAL, "%s: positions of %d axes, stride %lld", who, a->axis_count, (long long)a->positions_stride);
+  if (!(a->eps >= 0.f)) return fail(EKV_EINVAL, "%s: eps %g", who, a->eps);
+  const int e = bytes_of(a->dtype), we = bytes_of(a->weight_dtype);
+  p = Params{};
+  p.q = heads_of(a->query, a->q_stride_token, a->q_stride_head, a->tokens, a->q_heads, e);
+  p.q_out = heads_of(a->q_out, a->q_out_stride_token, a->q_out_stride_head, a->tokens, a->q_heads, e);
+  p.positions = a->pairs > 0 ? a->positions : nullptr;
+  p.positions_stride = a->positions_stride;
+  p.frequencies = a->frequencies;
+  p.axes = a->axes;
+  p.q_weight = a->q_heads > 0 ? (const char *)a->q_weight : nullptr;
+  p.k_weight = (const char *)a->k_weight;
+  p.q_weight_stride = a->q_weight_stride * we;
+  p.k_weight_stride = a->k_weight_stride * we;
+  p.tokens = a->tokens;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.dim = a->head_dim;
+  p.pairs = a->pairs;
+  p.axis_count = a->axis_count;
+  p.adjacent = a->adjacent != 0;
+  p.weight_f32 = a->weight_dtype == EKV_F32;
+  p.rotary_scale = a->rotary_scale;
+  p.eps = a->eps;
+  p.weight_offset = a->weight_offset;
+  p.mean = 1.f / a->head_dim;
+  return EKV_OK;
+}
+
+bool row_aligned(const Heads &h) { return aligned16(h.at) && h.token % 16 == 0 && h.head % 16 == 0; }
+bool weight_aligned(const char *at, int64_t stride) { return aligned16(at) && stride % 16 == 0; }
+
+}  // namespace append
+}  // namespace ekv
+
+using namespace ekv;
+
+extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
+  const char *who = "ekv_rotate_heads";
+  if (a == nullptr) return fail(EKV_EINVAL, "%s: null argument block", who);
+  append::Params p;
+  const int rc = append::fill(a, p, who);
+  if (rc != EKV_OK) return rc;
+  const int e = append::bytes_of(a->dtype);
+  p.k = append::heads_of(a->key, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.k_out = append::heads_of(a->k_out, a->k_out_stride_token, a->k_out_stride_head, a->tokens, a->kv_heads, e);
+  if (p.tokens == 0 || p.q_heads + p.kv_heads == 0) return EKV_OK;
+  if ((p.q_heads > 0 && (p.q.at == nullptr || p.q_out.at == nullptr)) ||
+      (p.kv_heads > 0 && (p.k.at == nullptr || p.k_out.at == nullptr)) || (p.pairs > 0 && p.positions == nullptr))
+    return fail(EKV_EINVAL, "%s: null pointer", who);
+  if (!append::row_aligned(p.q) || !append::row_aligned(p.q_out) || !append::row_aligned(p.k) ||
+      !append::row_aligned(p.k_out) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
+      !append::weight_aligned(p.k_weight, p.k_weight_stride))
+    return fail(EKV_EINVAL, "%s: heads and weights start at multiples of 16 bytes", who);
+  if (p.tokens >= 1 << 26) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
+  hipStream_t s = (hipStream_t)stream;
+  switch (a->dtype) {
+    case EKV_F32: return append::launch_dim<float, float, false>(p, s, "ekv_rotate_heads launch");
+    case EKV_F16: return append::launch_dim<_Float16, _Float16, false>(p, s, "ekv_rotate_heads launch");
+    default: return append::launch_dim<__bf16, __bf16, false>(p, s, "ekv_rotate_heads launch");
+  }
+}
+
+extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
+  const char *who = "ekv_append_tokens";
+  if (a == nullptr) return fail(EKV_EINVAL, "%s: null argument block", who);
+  append::Params p;
+  const int rc = append::fill(a, p, who);
+  if (rc != EKV_OK) return rc;
+  if (a->kv_dtype != a->dtype && a->kv_dtype != EKV_FP8_E4M3)
+    return fail(EKV_EUNSUPPORTED, "%s: tokens of type %d for a cache of type %d", who, a->dtype, a->kv_dtype);
+  if (a->rows < 0 || a->width < 0 || a->max_query < 1 || a->kv_heads < 1 || a->block_size < 1 || a->blocks < 0)
+    return fail(EKV_EINVAL, "%s: rows %d, width %d, at most %d tokens a row, %d KV heads, block size %d", who, a->rows,
+                a->width, a->max_query, a->kv_heads, a->block_size);
+  if (a->q_start == nullptr && (a->tokens != a->rows || a->max_query != 1))
+    return fail(EKV_EINVAL, "%s: %d tokens, at most %d a row, of %d rows need q_start", who, a->tokens, a->max_query,
+                a->rows);
+  if ((int64_t)a->width * a->block_size >= attn::kMostKeys)
+    return fail(EKV_EINVAL, "%s: a table of %d blocks of %d tokens passes 2^31 - 4096", who, a->width, a->block_size);
+  if (!(a->k_scale > 0.f) || !(a->v_scale > 0.f))
+    return fail(EKV_EINVAL, "%s: scales %g and %g", who, a->k_scale, a->v_scale);
+  const int e = append::bytes_of(a->dtype), ce = append::bytes_of(a->kv_dtype);
+  p.k = append::heads_of(a->new_keys, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.v = append::heads_of(a->new_values, a->v_stride_token, a->v_stride_head, a->tokens, a->kv_heads, e);
+  p.keys = (char *)a->keys;
+  p.values = (char *)a->values;
+  p.st_block = a->blocks > 1 ? a->kv_stride_block * ce : 0;
+  p.st_pos = a->block_size > 1 ? a->kv_stride_pos * ce : 0;
+  p.st_head = a->kv_heads > 1 ? a->kv_stride_head * ce : 0;
+  p.blocks = a->blocks;
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.lens = a->lens;
+  p.seen = a->seen;
+  p.first = a->first;
+  p.first_stride = a->first_stride;
+  p.q_start = a->q_start;
+  p.scores = a->scores;
+  p.sc_row = a->scores_stride_row;
+  p.sc_head = a->scores_stride_head;
+  p.slot_positions = a->slot_positions;
+  p.sp_row = a->slot_positions_stride_row;
+  p.sp_head = a->slot_positions_stride_head;
+  p.rows = a->rows;
+  p.width = a->width;
+  p.max_query = a->max_query;
+  p.block_size = a->block_size;
+  const PageDivisor d = page_divisor(a->block_size);
+  p.bs_mul = d.mul;
+  p.bs_shift = d.shift;
+  p.advance = a->advance != 0;
+  p.saturate = a->saturate != 0;
+  p.k_inverse = (float)(1.0 / a->k_scale);
+  p.v_inverse = (float)(1.0 / a->v_scale);
+  if (p.tokens == 0) return EKV_OK;
+  if (p.rows == 0) return fail(EKV_EINVAL, "%s: %d tokens of no row", who, p.tokens);
+  if (p.k.at == nullptr || p.v.at == nullptr || p.lens == nullptr ||
+      (p.q_heads > 0 && (p.q.at == nullptr || p.q_out.at == nullptr)) ||
+      (p.width > 0 && (p.keys == nullptr || p.values == nullptr || p.table == nullptr)))
+    return fail(EKV_EINVAL, "%s: null pointer", who);
+  if (p.blocks < 1 && p.width > 0) return fail(EKV_EINVAL, "%s: tables of an empty cache", who);
+  if (!append::row_aligned(p.q) || !append::row_aligned(p.q_out) || !append::row_aligned(p.k) ||
+      !append::row_aligned(p.v) || !append::aligned16(p.keys) || !append::aligned16(p.values) || p.st_block % 16 != 0 ||
+      p.st_pos % 16 != 0 || p.st_head % 16 != 0 || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
+      !append::weight_aligned(p.k_weight, p.k_weight_stride))
+    return fail(EKV_EINVAL, "%s: heads, weights and the cache's rows start at multiples of 16 bytes", who);
+  if (p.table_stride < p.width)
+    return fail(EKV_EINVAL, "%s: table rows of %d blocks, stride %lld", who, p.width, (long long)p.table_stride);
+  if (p.tokens >= 1 << 26) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
+  hipStream_t s = (hipStream_t)stream;
+  const bool fp8 = a->kv_dtype == EKV_FP8_E4M3;
+  int status;
+  switch (a->dtype) {
+    case EKV_F32: status = append::launch_cache<float>(p, fp8, s); break;
+    case EKV_F16: status = append::launch_cache<_Float16>(p, fp8, s); break;
+    default: status = append::launch_cache<__bf16>(p, fp8, s); break;
+  }
+  if (status != EKV_OK || !p.advance || p.q_start == nullptr) return status;
+  hipLaunchKernelGGL(append::advance_kernel, dim3((unsigned)append::ceil_div(p.rows, 256)), dim3(256), 0, s, p);
+  return check_hip(hipGetLastError(), "ekv_append_tokens advance launch");
+}

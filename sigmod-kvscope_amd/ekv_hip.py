@@ -79,6 +79,44 @@ class Eviction(ctypes.Structure):
     ]
 
 
+class Rotation(ctypes.Structure):
+    """``ekv_rotation_t``: the arguments of ``ekv_rotate_heads``."""
+
+    _fields_ = [
+        ("query", _p), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("key", _p), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("q_out", _p), ("q_out_stride_token", _i64), ("q_out_stride_head", _i64),
+        ("k_out", _p), ("k_out_stride_token", _i64), ("k_out_stride_head", _i64),
+        ("positions", _p), ("positions_stride", _i64), ("frequencies", _p), ("axes", _p),
+        ("q_weight", _p), ("k_weight", _p), ("q_weight_stride", _i64), ("k_weight_stride", _i64),
+        ("dtype", _i32), ("weight_dtype", _i32), ("tokens", _i32), ("q_heads", _i32), ("kv_heads", _i32),
+        ("head_dim", _i32), ("pairs", _i32), ("axis_count", _i32), ("adjacent", _i32),
+        ("rotary_scale", _f32), ("eps", _f32), ("weight_offset", _f32),
+    ]
+
+
+class Append(ctypes.Structure):
+    """``ekv_append_t``: the arguments of ``ekv_append_tokens``."""
+
+    _fields_ = [
+        ("query", _p), ("q_stride_token", _i64), ("q_stride_head", _i64), ("new_keys", _p), ("new_values", _p),
+        ("k_stride_token", _i64), ("k_stride_head", _i64), ("v_stride_token", _i64), ("v_stride_head", _i64),
+        ("q_out", _p), ("q_out_stride_token", _i64), ("q_out_stride_head", _i64),
+        ("keys", _p), ("values", _p), ("kv_stride_block", _i64), ("kv_stride_pos", _i64), ("kv_stride_head", _i64),
+        ("blocks", _i64), ("table", _p), ("table_stride", _i64), ("lens", _p), ("seen", _p), ("first", _p),
+        ("first_stride", _i64), ("q_start", _p), ("positions", _p), ("positions_stride", _i64),
+        ("frequencies", _p), ("axes", _p), ("q_weight", _p), ("k_weight", _p),
+        ("q_weight_stride", _i64), ("k_weight_stride", _i64),
+        ("scores", _p), ("scores_stride_row", _i64), ("scores_stride_head", _i64),
+        ("slot_positions", _p), ("slot_positions_stride_row", _i64), ("slot_positions_stride_head", _i64),
+        ("dtype", _i32), ("weight_dtype", _i32), ("kv_dtype", _i32), ("rows", _i32), ("width", _i32), ("tokens", _i32),
+        ("max_query", _i32), ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32),
+        ("pairs", _i32), ("axis_count", _i32), ("adjacent", _i32), ("advance", _i32), ("saturate", _i32),
+        ("rotary_scale", _f32), ("eps", _f32), ("weight_offset", _f32), ("k_scale", _f32), ("v_scale", _f32),
+        ("pad", _i32),
+    ]
+
+
 def packer(block: type[ctypes.Structure]):
     """A function of an argument block's fields in order: the bytes that a call takes in the block's place (one call,
     where setting the fields one by one costs a few microseconds).  ``ValueError`` for a value no field holds."""
@@ -189,6 +227,8 @@ _SIGNATURES: dict[str, list] = {
     "ekv_prefix_attention": [_p, _p, _sz, _p],
     "ekv_evict_tokens_workspace": [_i32, _i32, _i32],
     "ekv_evict_tokens": [_p, _p, _sz, _p],  # ctypes.addressof an Eviction
+    "ekv_rotate_heads": [_p, _p],  # ctypes.addressof a Rotation
+    "ekv_append_tokens": [_p, _p],  # ctypes.addressof an Append
     "ekv_malloc": [ctypes.POINTER(ctypes.c_void_p), _sz],
     "ekv_free": [_p],
     "ekv_memset": [_p, ctypes.c_int, _sz],
@@ -292,6 +332,21 @@ def on_stream(stream, where):
             return _HERE  # the call's own checks refuse it
         stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
     return torch.cuda.stream(stream)
+
+
+def beside(stream, tensor):
+    """The context of a call whose tensors may be on another device than the current one: that device is current in it,
+    and so is ``stream``, as in ``on_stream``.  ``ValueError`` for a torch stream of another device than the tensor's."""
+    device = tensor.get_device()
+    if device < 0:
+        return on_stream(stream, tensor)
+    import torch
+
+    if stream is None:
+        return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
+    if not isinstance(stream, int) and stream.device.index != device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {tensor.device}")
+    return on_stream(stream, tensor)
 
 
 def malloc(nbytes: int) -> int:
