@@ -39,8 +39,11 @@ inline Heads heads_of(const void *at, int64_t token, int64_t head, int tokens, i
   return {(const char *)at, tokens > 1 ? token * bytes : 0, heads > 1 ? head * bytes : 0};
 }
 
+enum Kind { kQuery, kKey, kValue };
+enum Norm { kNone, kShared, kOfHeads };  // no weights; the same of every head; each head's own
+
 struct Params {
-  Heads q, k, v, q_out, k_out;
+  Heads in[3], out[2];  // by Kind
   char *keys, *values;  // the cache, strides in bytes
   int64_t st_block, st_pos, st_head, blocks;
   const int32_t *table;
@@ -62,15 +65,16 @@ struct Params {
   uint32_t bs_mul;  // page_divisor(block_size)
   int bs_shift;
   bool adjacent, advance, saturate, weight_f32;
-  int parts;   // waves of a token: 1, 2 or 4
-  int passes;  // of 64 / G heads that the token's heads take, shared by its waves
+  int parts;               // waves of a token: 1, 2 or 4
+  int lanes_log;            // of a head: 2, 4, 8 or 16 lanes
+  int q_passes, kv_passes;  // of 64 / lanes heads, that the queries and that the keys (and the values) of a token take
   float rotary_scale, eps, weight_offset, k_inverse, v_inverse, mean;  // mean: 1 / dim
 };
 
 // -- elements -------------------------------------------------------------------------------------
 
 template <class T>
-struct Unit {  // 8 elements as they lie in memory
+struct Unit {  // 8 elements as they lie in memory (16 of an fp8 cache)
   u32x4 w;
 };
 template <>
@@ -78,11 +82,20 @@ struct Unit<float> {
   u32x4 w, more;
 };
 
-template <class T>
+// PAST the caches: where a launch moves more than the 256 MB Infinity Cache holds, its loads and stores are non-temporal
+// (launch_norm).
+template <class T, bool PAST>
 __device__ __forceinline__ Unit<T> load_unit(const char *at) {
   const auto *p = as_global((const u32x4 *)at);
-  if constexpr (sizeof(T) == 4) return {p[0], p[1]};
-  else return {p[0]};
+  Unit<T> u;
+  if constexpr (PAST) {
+    u.w = __builtin_nontemporal_load(p);
+    if constexpr (sizeof(T) == 4) u.more = __builtin_nontemporal_load(p + 1);
+  } else {
+    u.w = p[0];
+    if constexpr (sizeof(T) == 4) u.more = p[1];
+  }
+  return u;
 }
 
 __device__ __forceinline__ void widen(const Unit<float> &u, float (&x)[kUnit]) {
@@ -105,49 +118,83 @@ __device__ __forceinline__ void widen(const Unit<_Float16> &u, float (&x)[kUnit]
   for (int e = 0; e < kUnit; ++e) x[e] = (float)h[e];
 }
 
+template <class T>
+__device__ __forceinline__ void load_weights(const char *at, float (&x)[kUnit]) {
+  const auto *p = as_global((const u32x4 *)at);
+  if constexpr (sizeof(T) == 4) widen(Unit<T>{p[0], p[1]}, x);
+  else widen(Unit<T>{p[0]}, x);
+}
+
 // The largest finite e4m3 value for what passes it; NaN stays.
 __device__ __forceinline__ float within_e4m3(float x) {
   return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 448.f), -448.f);
 }
 
 template <class C>
-__device__ __forceinline__ void store_unit(char *at, const float (&x)[kUnit], bool saturate) {
+__device__ __forceinline__ Unit<C> narrow(const float (&x)[kUnit]) {
   if constexpr (std::is_same<C, float>::value) {
-    auto *p = as_global((f32x4 *)at);
-    p[0] = f32x4{x[0], x[1], x[2], x[3]};
-    p[1] = f32x4{x[4], x[5], x[6], x[7]};
-  } else if constexpr (std::is_same<C, attn::FP8>::value) {
-    float y[kUnit];
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) y[e] = saturate ? within_e4m3(x[e]) : x[e];
-    u32x2 w;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
-      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], word, true);
-    }
-    *as_global((u32x2 *)at) = w;
+    return {__builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]}), __builtin_bit_cast(u32x4, f32x4{x[4], x[5], x[6], x[7]})};
   } else {
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1], C{});
-    *as_global((u32x4 *)at) = w;
+    return {w};
+  }
+}
+__device__ __forceinline__ u32x2 narrow_e4m3(const float (&x)[kUnit], bool saturate) {
+  float y[kUnit];
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) y[e] = saturate ? within_e4m3(x[e]) : x[e];
+  u32x2 w;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], word, true);
+  }
+  return w;
+}
+template <class C, bool PAST>
+__device__ __forceinline__ void store_unit(char *at, const Unit<C> &u) {
+  auto *p = as_global((u32x4 *)at);
+  if constexpr (PAST) {
+    __builtin_nontemporal_store(u.w, p);
+    if constexpr (sizeof(C) == 4) __builtin_nontemporal_store(u.more, p + 1);
+  } else {
+    p[0] = u.w;
+    if constexpr (sizeof(C) == 4) p[1] = u.more;
+  }
+}
+// A lane's two units of 8 bytes.  Where a lane and its neighbour hold 16 bytes of the first unit and 16 of the second
+// beside each other (`paired`), one stores the first and one the second: whole pieces of 128 bytes of a head, where 8 bytes
+// a lane leave lines half written.
+template <bool PAST>
+__device__ __forceinline__ void store_e4m3(char *at, int a, int b, u32x2 x, u32x2 y, bool paired) {
+  if (paired) {
+    const bool odd = lane_id() & 1;
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // the neighbour's share: the even lane gives its second unit for the odd lane's first
+      const uint32_t got = (uint32_t)dpp_move<0xB1>((int)(odd ? x[i] : y[i]));
+      w[i] = odd ? got : x[i];
+      w[2 + i] = odd ? y[i] : got;
+    }
+    store_unit<attn::FP8, PAST>(at + (odd ? b - kUnit : a), {w});
+  } else {
+    *as_global((u32x2 *)(at + a)) = x;
+    *as_global((u32x2 *)(at + b)) = y;
   }
 }
 
-template <class C>
-constexpr int kBytes = std::is_same<C, float>::value ? 4 : std::is_same<C, attn::FP8>::value ? 1 : 2;
-
-// Sum over the G lanes of a head, every one of them receiving it.  All lanes of the wave are active.
-template <int G>
-__device__ __forceinline__ float head_sum(float v) {
+// Sum over the lanes of a head (2, 4, 8 or 16), every one of them receiving it.  All lanes of the wave are active.
+__device__ __forceinline__ float head_sum(float v, int lanes) {
   auto add = [&](auto ctrl) {
     v += __builtin_bit_cast(float, dpp_move<decltype(ctrl)::value>(__builtin_bit_cast(int, v)));
   };
-  add(std::integral_constant<int, 0xB1>());                         // quad_perm [1, 0, 3, 2]
-  if constexpr (G >= 4) add(std::integral_constant<int, 0x4E>());   // quad_perm [2, 3, 0, 1]
-  if constexpr (G >= 8) add(std::integral_constant<int, 0x141>());  // row_half_mirror: the other quad of 8 lanes
-  if constexpr (G >= 16) add(std::integral_constant<int, 0x140>()); // row_mirror: the other 8 of 16 lanes
+  add(std::integral_constant<int, 0xB1>());                   // quad_perm [1, 0, 3, 2]
+  if (lanes >= 4) add(std::integral_constant<int, 0x4E>());   // quad_perm [2, 3, 0, 1]
+  if (lanes >= 8) add(std::integral_constant<int, 0x141>());  // row_half_mirror: the other quad of 8 lanes
+  if (lanes >= 16) add(std::integral_constant<int, 0x140>()); // row_mirror: the other 8 of 16 lanes
   return v;
 }
 
@@ -163,20 +210,27 @@ struct Place {
 
 __device__ __forceinline__ int capacity(const Params &p) { return p.width * p.block_size; }  // below 2^31 - 4096
 
-// How many of the ascending a[0 .. n) are at most `token`: 64 ways at a step, so that a few hundred rows are two loads
-// behind each other where halving takes eight.
-__device__ __forceinline__ int count_up_to(const int32_t *a, int n, int token) {
+// The row of a token, and the row's first token and the next row's: the last of the ascending start[0 .. rows) that is
+// at most `token`, 62 ways at a step (a load for up to 62 rows and two for 3844, where halving takes a dozen), and its
+// neighbour out of the same load.  Row -1 for a token before the first.
+struct Span {
+  int row, begin, end;
+};
+__device__ __forceinline__ Span span_of(const int32_t *start, int rows, int token) {
+  constexpr int kWays = kWave - 2;
   const int lane = lane_id();
-  int below = 0;
-  while (n > kWave) {
-    const int step = (n + kWave - 1) / kWave, i = (lane + 1) * step - 1;
-    const bool low = i < n && a[below + i] <= token;
+  int below = 0, n = rows;  // start[0 .. below) are at most `token`, start[below + n ..] are not
+  while (n > kWays) {
+    const int step = (n + kWays - 1) / kWays, i = (lane + 1) * step - 1;
+    const bool low = i < n && start[below + i] <= token;
     const int whole = __popcll(__ballot(low)) * step;
     below += whole;
     n = min(step, n - whole);
   }
-  const bool low = lane < n && a[below + lane] <= token;
-  return below + __popcll(__ballot(low));
+  const int i = below - 1 + lane;  // lane 0 has the last one known to be at most `token`
+  const int value = lane <= n + 1 && i >= 0 ? start[i] : 0;
+  const int found = __popcll(__ballot(lane >= 1 && lane <= n && value <= token));
+  return {below + found - 1, __builtin_amdgcn_readlane(value, found), __builtin_amdgcn_readlane(value, found + 1)};
 }
 
 __device__ __forceinline__ Place place_of(const Params &p, int token) {
@@ -184,10 +238,11 @@ __device__ __forceinline__ Place place_of(const Params &p, int token) {
   int count = 1, nth = 0;
   at.row = token;
   if (p.q_start != nullptr) {
-    at.row = count_up_to(p.q_start, p.rows, token) - 1;
+    const Span s = span_of(p.q_start, p.rows, token);
+    at.row = s.row;
     if (at.row < 0) return at;
-    const int a = min(max(p.q_start[at.row], 0), p.tokens);
-    const int b = min(max(p.q_start[at.row + 1], a), p.tokens);
+    const int a = min(max(s.begin, 0), p.tokens);
+    const int b = min(max(s.end, a), p.tokens);
     count = b - a;
     nth = token - a;
   }
@@ -215,48 +270,49 @@ __device__ __forceinline__ void advance_row(const Params &p, int row, int t) {
 
 // -- the pass ---------------------------------------------------------------------------------------
 
-// T: the inputs' type.  C: the cache's (FP8 or T).  G: lanes of a head.  PAGED: with a cache and values; else keys go to
-// k_out.
-template <class T, class C, int G, bool PAGED>
+// T: the inputs' type.  C: the cache's (FP8 or T).  PAGED: with a cache and values; else keys go to k_out.  NORM: with
+// weights.  ADJACENT: the order of the pairs.  PAST: as load_unit
+// has it.
+template <class T, class C, bool PAGED, Norm NORM, bool ADJACENT, bool PAST>
 __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
-  constexpr int kPer = kWave / G;  // heads of a pass
   __shared__ __align__(16) float s_cos[kWaves][kMostPairs], s_sin[kWaves][kMostPairs];
+  __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2 * kMostPairs];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int lanes = 1 << p.lanes_log, per = kWave >> p.lanes_log;  // of a head; heads of a pass
   const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
-  const int64_t token = item / p.parts;
-  const int part = (int)(item % p.parts);
-  const bool here = token < p.tokens;
+  const int token = (int)(item / p.parts), part = (int)(item % p.parts);
 
-  if (here) {
-    const int heads = p.q_heads + (PAGED ? 2 : 1) * p.kv_heads;
-    const int unit = lane % G, turning = p.pairs / kUnit, rest = p.dim - 2 * p.pairs;
-    const bool active = unit * 2 * kUnit < p.dim, turns = unit < turning;
-    // the lane's elements: [a, a + 8) and [b, b + 8)
-    const int a = turns ? unit * kUnit : 2 * p.pairs + (unit - turning) * kUnit;
-    const int b = turns ? p.pairs + a : a + rest / 2;
+  const int nth = lane >> p.lanes_log, turning = p.pairs / kUnit, rest = p.dim - 2 * p.pairs;
+  const bool active = (lane & (lanes - 1)) * 2 * kUnit < p.dim;
+  const int unit = active ? lane & (lanes - 1) : 0;  // an idle lane reads what lane 0 of its head does, and writes nothing
+  const bool turns = unit < turning;
+  // the lane's elements: [a, a + 8) and [b, b + 8)
+  const int a = turns ? unit * kUnit : 2 * p.pairs + (unit - turning) * kUnit;
+  const int b = turns ? p.pairs + a : a + rest / 2;
+  const bool paired = turning % 2 == 0 && p.dim % 32 == 0;  // fp8 caches: store_e4m3
 
-    const char *const q_at = p.q.at + token * p.q.token, *const k_at = p.k.at + token * p.k.token;
-    const char *const v_at = p.v.at + token * p.v.token;
-    auto source = [&](int head) {
-      if (head < p.q_heads) return q_at + head * p.q.head;
-      head -= p.q_heads;
-      if (!PAGED || head < p.kv_heads) return k_at + head * p.k.head;
-      return v_at + (head - p.kv_heads) * p.v.head;
-    };
-    Unit<T> ua{}, ub{};
-    auto fetch = [&](int pass) {
-      const int head = pass * kPer + lane / G;
-      if (active && head < heads) {
-        const char *x = source(head);
-        ua = load_unit<T>(x + a * sizeof(T));
-        ub = load_unit<T>(x + b * sizeof(T));
-      }
-    };
-    int pass = part;
-    if (pass < p.passes) fetch(pass);  // on their way while the token finds its place
+  // The passes of the queries, then the keys, then the values; the wave takes every parts-th.  A pass has heads of one
+  // kind, so that what depends on the kind is scalar.
+  const int passes = p.q_passes + (PAGED ? 2 : 1) * p.kv_passes;
+  auto kind_of = [&](int pass) { return pass < p.q_passes ? kQuery : pass < p.q_passes + p.kv_passes ? kKey : kValue; };
+  auto first_head = [&](int pass, int kind) {
+    return (pass - (kind == kQuery ? 0 : p.q_passes + (kind == kValue ? p.kv_passes : 0))) * per;
+  };
+  auto heads_of = [&](int kind) { return kind == kQuery ? p.q_heads : p.kv_heads; };
+  Unit<T> ua, ub;
+  auto fetch = [&](int pass) {
+    const int kind = kind_of(pass), head = min(first_head(pass, kind) + nth, heads_of(kind) - 1);
+    const Heads &from = p.in[kind];
+    const char *x = from.at + token * from.token + head * from.head;
+    ua = load_unit<T, PAST>(x + a * sizeof(T));
+    ub = load_unit<T, PAST>(x + b * sizeof(T));
+  };
 
+  if (token < p.tokens && part < passes) fetch(part);  // on its way while the token finds its place
+  int weighed = -1;  // the kind whose weights, the same for every head, s_weight holds
+  if (token < p.tokens) {
     Place at{true, 0, 0, 0, false, -1};
-    if constexpr (PAGED) at = place_of(p, (int)token);
+    if constexpr (PAGED) at = place_of(p, token);
 
     // the token's cosines and sines
     float cosine[kUnit], sine[kUnit];
@@ -277,22 +333,14 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
       }
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (turns) {
-        if (p.adjacent) {  // [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
+      // adjacent: [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
+      const int low = !turns ? 0 : ADJACENT ? a / 2 : a, high = !turns ? 0 : ADJACENT ? b / 2 : a + 4;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            cosine[e] = s_cos[wave][a / 2 + e];
-            sine[e] = s_sin[wave][a / 2 + e];
-            cosine[4 + e] = s_cos[wave][b / 2 + e];
-            sine[4 + e] = s_sin[wave][b / 2 + e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e) {
-            cosine[e] = s_cos[wave][a + e];
-            sine[e] = s_sin[wave][a + e];
-          }
-        }
+      for (int e = 0; e < 4; ++e) {
+        cosine[e] = s_cos[wave][low + e];
+        sine[e] = s_sin[wave][low + e];
+        cosine[4 + e] = s_cos[wave][high + e];
+        sine[4 + e] = s_sin[wave][high + e];
       }
     }
 
@@ -302,30 +350,45 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         const int64_t block = __umulhi((uint32_t)at.slot << 1, p.bs_mul) >> p.bs_shift;
         in_page = at.page * p.st_block + (at.slot - block * p.block_size) * p.st_pos;
       }
-      if (part == 0 && at.live && at.in_table) {  // a new slot has no weight yet
-        for (int h = lane; h < p.kv_heads; h += kWave) {
+      if (part == 0 && at.live && at.in_table && (p.scores != nullptr || p.slot_positions != nullptr)) {
+        for (int h = lane; h < p.kv_heads; h += kWave) {  // a new slot has no weight yet
           if (p.scores != nullptr) p.scores[at.row * p.sc_row + h * p.sc_head + at.slot] = 0.f;
           if (p.slot_positions != nullptr) p.slot_positions[at.row * p.sp_row + h * p.sp_head + at.slot] = (int32_t)at.index;
         }
       }
     }
 
-    for (; pass < p.passes; pass += p.parts) {
-      const int head = pass * kPer + lane / G;
-      const bool is_q = head < p.q_heads, is_v = PAGED && head >= p.q_heads + p.kv_heads;
+    for (int pass = part; pass < passes; pass += p.parts) {
+      const int kind = kind_of(pass), head = first_head(pass, kind) + nth, heads = heads_of(kind);
       const bool mine = active && head < heads;
-      float x[kUnit] = {}, y[kUnit] = {};
-      if (mine) {
-        widen(ua, x);
-        widen(ub, y);
+      const Unit<T> va = ua, vb = ub;
+      if (pass + p.parts < passes) fetch(pass + p.parts);
+      // where a token of no row has nothing to write but 0 for its queries
+      if (PAGED && (kind == kQuery ? !at.live : at.page < 0)) {
+        if (kind == kQuery && mine) {
+          char *to = (char *)p.out[kQuery].at + token * p.out[kQuery].token + head * p.out[kQuery].head;
+          store_unit<T, PAST>(to + a * sizeof(T), Unit<T>{});
+          store_unit<T, PAST>(to + b * sizeof(T), Unit<T>{});
+        }
+        continue;
       }
-      if (pass + p.parts < p.passes) fetch(pass + p.parts);
-      if (p.q_weight != nullptr || p.k_weight != nullptr) {
-        const char *w = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
+      float x[kUnit], y[kUnit];
+      widen(va, x);
+      widen(vb, y);
+      if (NORM != kNone && (!PAGED || kind != kValue)) {
+        const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
+        if (NORM == kShared && weighed != kind) {
+          weighed = kind;
+          for (int i = lane; i < p.dim; i += kWave)
+            s_weight[wave][i] = weight == nullptr ? 1.f : p.weight_offset + (p.weight_f32 ? ((const float *)weight)[i]
+                                                                                          : (float)((const T *)weight)[i]);
+          __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
         float squares = 0.f;
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) squares += x[e] * x[e] + y[e] * y[e];
-        squares = head_sum<G>(squares);
+        squares = head_sum(mine ? squares : 0.f, lanes);
         float over = rsqrtf(squares * p.mean + p.eps);
         if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
           float small = 0.f;
@@ -334,29 +397,44 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
             const float u = x[e] * 0x1p-80f, v = y[e] * 0x1p-80f;
             small += u * u + v * v;
           }
-          small = head_sum<G>(small);
+          small = head_sum(mine ? small : 0.f, lanes);
           if (squares == __builtin_inff()) over = rsqrtf(small * p.mean) * 0x1p-80f;
         }
-        if (w != nullptr && mine) {
-          float wa[kUnit], wb[kUnit];
-          if (p.weight_f32) {
-            const char *row = w + (is_q ? head * p.q_weight_stride : (head - p.q_heads) * p.k_weight_stride);
-            widen(load_unit<float>(row + a * 4), wa);
-            widen(load_unit<float>(row + b * 4), wb);
-          } else {
-            const char *row = w + (is_q ? head * p.q_weight_stride : (head - p.q_heads) * p.k_weight_stride);
-            widen(load_unit<T>(row + a * sizeof(T)), wa);
-            widen(load_unit<T>(row + b * sizeof(T)), wb);
-          }
+        if (weight == nullptr) over = 1.f;  // the other one's heads are normed, not these
+        float wa[kUnit], wb[kUnit];
+        if constexpr (NORM == kShared) {
 #pragma unroll
           for (int e = 0; e < kUnit; ++e) {
-            x[e] *= over * (p.weight_offset + wa[e]);
-            y[e] *= over * (p.weight_offset + wb[e]);
+            wa[e] = s_weight[wave][a + e];
+            wb[e] = s_weight[wave][b + e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e) wa[e] = wb[e] = 1.f;
+          if (weight != nullptr) {
+            const char *row = weight + min(head, heads - 1) * (kind == kQuery ? p.q_weight_stride : p.k_weight_stride);
+            if (p.weight_f32) {
+              load_weights<float>(row + a * 4, wa);
+              load_weights<float>(row + b * 4, wb);
+            } else {
+              load_weights<T>(row + a * sizeof(T), wa);
+              load_weights<T>(row + b * sizeof(T), wb);
+            }
+#pragma unroll
+            for (int e = 0; e < kUnit; ++e) {
+              wa[e] += p.weight_offset;
+              wb[e] += p.weight_offset;
+            }
           }
         }
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) {
+          x[e] *= over * wa[e];
+          y[e] *= over * wb[e];
+        }
       }
-      if (turns && !is_v) {
-        if (p.adjacent) {
+      if (turns && (!PAGED || kind != kValue)) {
+        if constexpr (ADJACENT) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float u = x[2 * e], v = x[2 * e + 1], r = y[2 * e], s = y[2 * e + 1];
@@ -374,30 +452,28 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
           }
         }
       }
-      if (!mine) continue;
-      if (is_q) {
-        char *to = (char *)p.q_out.at + token * p.q_out.token + head * p.q_out.head;
-        if (!at.live) {
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e) x[e] = y[e] = 0.f;
+      if (!PAGED || kind == kQuery) {
+        if (mine) {
+          const Heads &out = p.out[kind];
+          char *to = (char *)out.at + (int64_t)token * out.token + head * out.head;
+          store_unit<T, PAST>(to + a * sizeof(T), narrow<T>(x));
+          store_unit<T, PAST>(to + b * sizeof(T), narrow<T>(y));
         }
-        store_unit<T>(to + a * kBytes<T>, x, false);
-        store_unit<T>(to + b * kBytes<T>, y, false);
-      } else if constexpr (!PAGED) {
-        char *to = (char *)p.k_out.at + token * p.k_out.token + (head - p.q_heads) * p.k_out.head;
-        store_unit<T>(to + a * kBytes<T>, x, false);
-        store_unit<T>(to + b * kBytes<T>, y, false);
-      } else if (at.page >= 0) {
-        const int kv = head - p.q_heads - (is_v ? p.kv_heads : 0);
-        char *to = (is_v ? p.values : p.keys) + in_page + kv * p.st_head;
-        const float inverse = is_v ? p.v_inverse : p.k_inverse;
+      } else {  // the slot's key or value
+        const float inverse = kind == kValue ? p.v_inverse : p.k_inverse;
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) {
           x[e] *= inverse;
           y[e] *= inverse;
         }
-        store_unit<C>(to + a * kBytes<C>, x, p.saturate);
-        store_unit<C>(to + b * kBytes<C>, y, p.saturate);
+        char *to = (kind == kValue ? p.values : p.keys) + in_page + head * p.st_head;
+        if constexpr (std::is_same<C, attn::FP8>::value) {
+          const u32x2 xa = narrow_e4m3(x, p.saturate), yb = narrow_e4m3(y, p.saturate);
+          if (mine) store_e4m3<PAST>(to, a, b, xa, yb, paired);
+        } else if (mine) {
+          store_unit<T, PAST>(to + a * sizeof(T), narrow<T>(x));
+          store_unit<T, PAST>(to + b * sizeof(T), narrow<T>(y));
+        }
       }
     }
   }
@@ -406,7 +482,7 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
     // advance_kernel runs behind this one.
     if (p.advance && p.q_start == nullptr) {
       __syncthreads();
-      if (here && part == 0 && lane == 0) advance_row(p, (int)token, 1);
+      if (token < p.tokens && part == 0 && lane == 0) advance_row(p, token, 1);
     }
   }
 }
@@ -423,32 +499,45 @@ __global__ __launch_bounds__(256) void advance_kernel(Params p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <class T, class C, int G, bool PAGED>
-int launch_group(Params p, hipStream_t stream, const char *who) {
-  const int heads = p.q_heads + (PAGED ? 2 : 1) * p.kv_heads;
-  p.passes = (int)ceil_div(heads, kWave / G);
+template <class T, class C, bool PAGED, Norm NORM>
+int launch_norm(Params p, hipStream_t stream, const char *who) {
+  p.lanes_log = p.dim <= 32 ? 1 : p.dim <= 64 ? 2 : p.dim <= 128 ? 3 : 4;
+  p.q_passes = (int)ceil_div(p.q_heads, kWave >> p.lanes_log);
+  p.kv_passes = (int)ceil_div(p.kv_heads, kWave >> p.lanes_log);
+  const int passes = p.q_passes + (PAGED ? 2 : 1) * p.kv_passes;
   // Waves of a token: four while that does not fill the chip, so that a pass of the heads is not behind another; one where
   // there are tokens enough, which share a token's angles.
   const int64_t enough = 16ll * cu_count();
   p.parts = p.tokens * 4ll <= enough ? 4 : p.tokens * 2ll <= enough ? 2 : 1;
-  while (p.parts > 1 && p.parts / 2 >= p.passes) p.parts /= 2;
-  const int64_t grid = ceil_div((int64_t)p.tokens * p.parts, kWaves);
-  hipLaunchKernelGGL((heads_kernel<T, C, G, PAGED>), dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream, p);
+  while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
+  // Loads and stores past the caches, us with against without, 32 query and 8 KV heads of 128 in bf16: 41000 tokens of
+  // prompts (1.0 GB) 172 / 186, into an fp8 cache (0.8 GB) 146 / 171; 16384 tokens' norms (0.34 GB) 63 / 68; prompts of 0.24
+  // GB 47 / 45, into an fp8 cache 0.25 GB 50 / 48, 0.13 GB 26 / 26, 0.06 GB 15 / 13.
+  const int64_t cache_bytes = std::is_same<C, attn::FP8>::value ? 1 : sizeof(T);
+  const int64_t moved = (2ll * p.q_heads + 2 * p.kv_heads) * sizeof(T) + 2 * p.kv_heads * cache_bytes;  // of a token's element
+  const bool past = p.tokens * p.dim * moved > 256ll << 20;
+  const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.parts, kWaves)), block(kWaves * kWave);
+  if (p.adjacent) {
+    if (past) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, false>), grid, block, 0, stream, p);
+  } else {
+    if (past) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, false>), grid, block, 0, stream, p);
+  }
   return check_hip(hipGetLastError(), who);
 }
 
 template <class T, class C, bool PAGED>
-int launch_dim(const Params &p, hipStream_t stream, const char *who) {
-  if (p.dim <= 32) return launch_group<T, C, 2, PAGED>(p, stream, who);
-  if (p.dim <= 64) return launch_group<T, C, 4, PAGED>(p, stream, who);
-  if (p.dim <= 128) return launch_group<T, C, 8, PAGED>(p, stream, who);
-  return launch_group<T, C, 16, PAGED>(p, stream, who);
+int launch(const Params &p, hipStream_t stream, const char *who) {
+  if (p.q_weight == nullptr && p.k_weight == nullptr) return launch_norm<T, C, PAGED, kNone>(p, stream, who);
+  if (p.q_weight_stride == 0 && p.k_weight_stride == 0) return launch_norm<T, C, PAGED, kShared>(p, stream, who);
+  return launch_norm<T, C, PAGED, kOfHeads>(p, stream, who);
 }
 
 template <class T>
 int launch_cache(const Params &p, bool fp8, hipStream_t stream) {
-  return fp8 ? launch_dim<T, attn::FP8, true>(p, stream, "ekv_append_tokens launch")
-             : launch_dim<T, T, true>(p, stream, "ekv_append_tokens launch");
+  return fp8 ? launch<T, attn::FP8, true>(p, stream, "ekv_append_tokens launch")
+             : launch<T, T, true>(p, stream, "ekv_append_tokens launch");
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -475,8 +564,8 @@ int fill(const Block *a, Params &p, const char *who) {
   if (!(a->eps >= 0.f)) return fail(EKV_EINVAL, "%s: eps %g", who, a->eps);
   const int e = bytes_of(a->dtype), we = bytes_of(a->weight_dtype);
   p = Params{};
-  p.q = heads_of(a->query, a->q_stride_token, a->q_stride_head, a->tokens, a->q_heads, e);
-  p.q_out = heads_of(a->q_out, a->q_out_stride_token, a->q_out_stride_head, a->tokens, a->q_heads, e);
+  p.in[append::kQuery] = heads_of(a->query, a->q_stride_token, a->q_stride_head, a->tokens, a->q_heads, e);
+  p.out[append::kQuery] = heads_of(a->q_out, a->q_out_stride_token, a->q_out_stride_head, a->tokens, a->q_heads, e);
   p.positions = a->pairs > 0 ? a->positions : nullptr;
   p.positions_stride = a->positions_stride;
   p.frequencies = a->frequencies;
@@ -515,22 +604,22 @@ extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
   const int rc = append::fill(a, p, who);
   if (rc != EKV_OK) return rc;
   const int e = append::bytes_of(a->dtype);
-  p.k = append::heads_of(a->key, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
-  p.k_out = append::heads_of(a->k_out, a->k_out_stride_token, a->k_out_stride_head, a->tokens, a->kv_heads, e);
+  p.in[append::kKey] = append::heads_of(a->key, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.out[append::kKey] = append::heads_of(a->k_out, a->k_out_stride_token, a->k_out_stride_head, a->tokens, a->kv_heads, e);
   if (p.tokens == 0 || p.q_heads + p.kv_heads == 0) return EKV_OK;
-  if ((p.q_heads > 0 && (p.q.at == nullptr || p.q_out.at == nullptr)) ||
-      (p.kv_heads > 0 && (p.k.at == nullptr || p.k_out.at == nullptr)) || (p.pairs > 0 && p.positions == nullptr))
+  if ((p.q_heads > 0 && (p.in[append::kQuery].at == nullptr || p.out[append::kQuery].at == nullptr)) ||
+      (p.kv_heads > 0 && (p.in[append::kKey].at == nullptr || p.out[append::kKey].at == nullptr)) || (p.pairs > 0 && p.positions == nullptr))
     return fail(EKV_EINVAL, "%s: null pointer", who);
-  if (!append::row_aligned(p.q) || !append::row_aligned(p.q_out) || !append::row_aligned(p.k) ||
-      !append::row_aligned(p.k_out) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
+  if (!append::row_aligned(p.in[append::kQuery]) || !append::row_aligned(p.out[append::kQuery]) || !append::row_aligned(p.in[append::kKey]) ||
+      !append::row_aligned(p.out[append::kKey]) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads and weights start at multiples of 16 bytes", who);
   if (p.tokens >= 1 << 26) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
-    case EKV_F32: return append::launch_dim<float, float, false>(p, s, "ekv_rotate_heads launch");
-    case EKV_F16: return append::launch_dim<_Float16, _Float16, false>(p, s, "ekv_rotate_heads launch");
-    default: return append::launch_dim<__bf16, __bf16, false>(p, s, "ekv_rotate_heads launch");
+    case EKV_F32: return append::launch<float, float, false>(p, s, "ekv_rotate_heads launch");
+    case EKV_F16: return append::launch<_Float16, _Float16, false>(p, s, "ekv_rotate_heads launch");
+    default: return append::launch<__bf16, __bf16, false>(p, s, "ekv_rotate_heads launch");
   }
 }
 
@@ -553,8 +642,8 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   if (!(a->k_scale > 0.f) || !(a->v_scale > 0.f))
     return fail(EKV_EINVAL, "%s: scales %g and %g", who, a->k_scale, a->v_scale);
   const int e = append::bytes_of(a->dtype), ce = append::bytes_of(a->kv_dtype);
-  p.k = append::heads_of(a->new_keys, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
-  p.v = append::heads_of(a->new_values, a->v_stride_token, a->v_stride_head, a->tokens, a->kv_heads, e);
+  p.in[append::kKey] = append::heads_of(a->new_keys, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.in[append::kValue] = append::heads_of(a->new_values, a->v_stride_token, a->v_stride_head, a->tokens, a->kv_heads, e);
   p.keys = (char *)a->keys;
   p.values = (char *)a->values;
   p.st_block = a->blocks > 1 ? a->kv_stride_block * ce : 0;
@@ -587,13 +676,13 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   p.v_inverse = (float)(1.0 / a->v_scale);
   if (p.tokens == 0) return EKV_OK;
   if (p.rows == 0) return fail(EKV_EINVAL, "%s: %d tokens of no row", who, p.tokens);
-  if (p.k.at == nullptr || p.v.at == nullptr || p.lens == nullptr ||
-      (p.q_heads > 0 && (p.q.at == nullptr || p.q_out.at == nullptr)) ||
+  if (p.in[append::kKey].at == nullptr || p.in[append::kValue].at == nullptr || p.lens == nullptr ||
+      (p.q_heads > 0 && (p.in[append::kQuery].at == nullptr || p.out[append::kQuery].at == nullptr)) ||
       (p.width > 0 && (p.keys == nullptr || p.values == nullptr || p.table == nullptr)))
     return fail(EKV_EINVAL, "%s: null pointer", who);
   if (p.blocks < 1 && p.width > 0) return fail(EKV_EINVAL, "%s: tables of an empty cache", who);
-  if (!append::row_aligned(p.q) || !append::row_aligned(p.q_out) || !append::row_aligned(p.k) ||
-      !append::row_aligned(p.v) || !append::aligned16(p.keys) || !append::aligned16(p.values) || p.st_block % 16 != 0 ||
+  if (!append::row_aligned(p.in[append::kQuery]) || !append::row_aligned(p.out[append::kQuery]) || !append::row_aligned(p.in[append::kKey]) ||
+      !append::row_aligned(p.in[append::kValue]) || !append::aligned16(p.keys) || !append::aligned16(p.values) || p.st_block % 16 != 0 ||
       p.st_pos % 16 != 0 || p.st_head % 16 != 0 || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads, weights and the cache's rows start at multiples of 16 bytes", who);

@@ -335,18 +335,21 @@ def on_stream(stream, where):
 
 
 def beside(stream, tensor):
-    """The context of a call whose tensors may be on another device than the current one: that device is current in it,
-    and so is ``stream``, as in ``on_stream``.  ``ValueError`` for a torch stream of another device than the tensor's."""
+    """(context, raw stream handle) of a call whose tensors may be on another device than the current one: in the context
+    that device is current and, with ``stream``, that stream is, as in ``on_stream``.  Without a context (None) both are
+    already.  ``ValueError`` for a torch stream of another device than the tensor's."""
     device = tensor.get_device()
-    if device < 0:
-        return on_stream(stream, tensor)
-    import torch
-
     if stream is None:
-        return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
-    if not isinstance(stream, int) and stream.device.index != device:
+        if _raw_stream is not None and device == _raw_stream[1]():
+            return None, _raw_stream[0](device)
+        import torch
+
+        if device < 0 or device == torch.cuda.current_device():
+            return None, stream_handle()
+        return torch.cuda.device(device), int(torch.cuda.current_stream(device).cuda_stream)
+    if device >= 0 and not isinstance(stream, int) and stream.device.index != device:
         raise ValueError(f"a stream of {stream.device} for tensors on {tensor.device}")
-    return on_stream(stream, tensor)
+    return on_stream(stream, tensor), stream_handle(stream)
 
 
 def malloc(nbytes: int) -> int:
@@ -393,7 +396,7 @@ def synchronize() -> None:
     call("ekv_synchronize")
 
 
-_codes: dict = {}  # torch dtype -> EKV_* code
+_codes: dict = {}  # torch dtype -> EKV_* code, filled by the first dtype_code
 
 
 def dtype_code(dtype) -> int:

@@ -12,11 +12,23 @@ import torch
 
 import ekv_hip
 from observe.allocation import check_tensors
-from runtime.prefix_attention import _cache_shape
-from runtime.rotary import _heads, _turns, _weights
+from runtime.prefix_attention import _cache_shape, _sound
+from runtime.rotary import _HEAD_TYPES, _HERE, _NONE, _row, _shape_of, _turns, _weights
 
 _pack = ekv_hip.packer(ekv_hip.Append)
 _INT, _FLOAT = torch.int32, torch.float32
+_Tensor = torch.Tensor
+
+
+def _slots(name: str, t, kind, rows: int, heads: int, least: int, device: int) -> tuple[int, int, int]:
+    """(address, strides of the rows and heads) of a tensor with a value for every slot."""
+    if not isinstance(t, _Tensor) or t.ndim != 3 or t.shape[:2] != (rows, heads) or t.shape[2] < least:
+        raise ValueError(f"{name} must be a [{rows}, {heads}, {least} or more] tensor")
+    row, head, one = t.stride()
+    if t.dtype is not kind or one != 1 or t.get_device() != device:
+        if check_tensors((name, t, kind, t.shape)).index != device:
+            raise ValueError(f"{name} must be on the cache's device, got {t.device}")
+    return t.data_ptr(), row, head
 
 
 def append_tokens(
@@ -71,72 +83,77 @@ def append_tokens(
     ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
     through the call."""
     pages, block, kv_heads, dim = _cache_shape(kv_cache)
-    if not isinstance(table, torch.Tensor) or table.ndim != 2:
+    if not isinstance(table, _Tensor) or table.ndim != 2:
         raise ValueError("the block table must be a [rows, width] tensor")
-    rows, width = table.shape
-    tokens, heads, _ = _heads("keys", keys, None, dim, None)
-    if heads != kv_heads:
-        raise ValueError(f"keys must be a [tokens, {kv_heads}, {dim}] tensor, got {tuple(keys.shape)}")
-    dtype, q_heads = keys.dtype, 0
-    if kv_cache.dtype != dtype and kv_cache.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"keys of {dtype} for a cache of {kv_cache.dtype}")
+    rows, width = t_shape = table.shape
+    tokens, heads, k_dim = k_shape = _shape_of("keys", keys)
+    if heads != kv_heads or k_dim != dim:
+        raise ValueError(f"keys must be a [tokens, {kv_heads}, {dim}] tensor, got {tuple(k_shape)}")
+    dtype, kv_dtype, q_heads, q_shape = keys.dtype, kv_cache.dtype, 0, None
+    if kv_dtype is not dtype and kv_dtype is not torch.float8_e4m3fn:
+        raise ValueError(f"keys of {dtype} for a cache of {kv_dtype}")
     if query is not None:
-        q_heads = _heads("query", query, tokens, dim, dtype)[1]
+        q_tokens, q_heads, q_dim = q_shape = _shape_of("query", query)
+        if q_tokens != tokens or q_dim != dim:
+            raise ValueError(f"query must be a [{tokens}, heads, {dim}] tensor, got {tuple(q_shape)}")
     elif q_out is not None or q_weight is not None:
         raise ValueError("q_out and q_weight need a query")
     if frequencies is None and positions is not None:
         raise ValueError("positions need frequencies")
     if width == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
-        table = table.new_empty(table.shape)
+        table = table.new_empty(t_shape)
     if tokens == 0:
-        if values.shape != keys.shape or values.dtype != dtype:
-            raise ValueError(f"values must be {dtype} of shape {tuple(keys.shape)}")
-        keys, values = keys.new_empty(keys.shape), values.new_empty(values.shape)
-        query = None if query is None else query.new_empty(query.shape)
-    q_shape = None if query is None else query.shape
-    device = check_tensors(
-        ("kv_cache", kv_cache, kv_cache.dtype, kv_cache.shape), ("keys", keys, dtype, keys.shape),
-        ("values", values, dtype, keys.shape), ("query", query, dtype, q_shape), ("q_out", q_out, dtype, q_shape),
-        ("table", table, _INT, (rows, width)), ("lens", lens, _INT, (rows,)), ("q_start", q_start, _INT, (rows + 1,)),
-        ("seen", seen, _INT, (rows,)))
-    at, stride, count, turning, axis, pairs = _turns(tokens, dim, positions, frequencies, axes, device)
-    if count == 1 and axes is not None and positions is None:
-        raise ValueError("axes need positions")
-    qw, kw, qw_stride, kw_stride, w_type = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
+        if not isinstance(values, _Tensor) or values.shape != k_shape or values.dtype != dtype:
+            raise ValueError(f"values must be {dtype} of shape {tuple(k_shape)}")
+        keys, values = keys.new_empty(k_shape), values.new_empty(k_shape)
+        query = None if query is None else query.new_empty(q_shape)
+    device = kv_cache.get_device()
+    k_in, v_in = _row(keys, dtype, k_shape, device), _row(values, dtype, k_shape, device)
+    q_in = _NONE if query is None else _row(query, dtype, q_shape, device)
+    if k_in is None or v_in is None or q_in is None or dtype not in _HEAD_TYPES or not _sound(
+            device, ((table, t_shape), (lens, (rows,)))) or ((q_start is not None or seen is not None) and not _sound(
+                device, ((q_start, (rows + 1,)), (seen, (rows,))))):
+        check_tensors(
+            ("kv_cache", kv_cache, kv_dtype, kv_cache.shape), ("keys", keys, _HEAD_TYPES, k_shape),
+            ("values", values, dtype, k_shape), ("query", query, dtype, q_shape),
+            ("q_out", q_out, dtype, q_shape), ("table", table, _INT, t_shape), ("lens", lens, _INT, (rows,)), ("q_start", q_start, _INT, (rows + 1,)),
+            ("seen", seen, _INT, (rows,)))
+    turns = _turns(tokens, dim, positions, frequencies, axes, device)
+    weights = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
     at_first = first_stride = 0
     if first is not None:
-        if not isinstance(first, torch.Tensor) or first.shape != (rows,) or first.dtype != _INT or first.device != device:
-            raise ValueError(f"first must be an int32 [{rows}] tensor on {device}")
+        if not isinstance(first, _Tensor) or first.shape != (rows,) or first.dtype != _INT or first.get_device() != device:
+            raise ValueError(f"first must be an int32 [{rows}] tensor on the cache's device")
         at_first, first_stride = first.data_ptr(), first.stride(0)
-    kept = []
-    for name, t, kind in (("scores", scores, _FLOAT), ("slot_positions", slot_positions, _INT)):
-        if t is None:
-            kept += [0, 0, 0]
-            continue
-        if not isinstance(t, torch.Tensor) or t.ndim != 3 or t.shape[:2] != (rows, kv_heads) or t.shape[2] < width * block:
-            raise ValueError(f"{name} must be a [{rows}, {kv_heads}, {width * block} or more] tensor")
-        if check_tensors((name, t, kind, t.shape)) != device:
-            raise ValueError(f"{name} must be on {device}")
-        kept += [t.data_ptr(), t.stride(0), t.stride(1)]
-    with ekv_hip.beside(stream, kv_cache):
+    scores_at = _NONE if scores is None else _slots("scores", scores, _FLOAT, rows, kv_heads, width * block, device)
+    places_at = _NONE if slot_positions is None else \
+        _slots("slot_positions", slot_positions, _INT, rows, kv_heads, width * block, device)
+    context, handle = ekv_hip.beside(stream, kv_cache)
+    with context or _HERE:
         if query is None:
-            queries = queries_out = (0, 0, 0)
+            q_to = _NONE
+        elif q_out is None:
+            q_out = torch.empty(tokens, q_heads, dim, dtype=dtype, device=kv_cache.device)
+            q_to = q_out.data_ptr(), q_heads * dim, dim
         else:
-            if q_out is None:
-                q_out = torch.empty(q_shape, dtype=dtype, device=device)
-            queries = (query.data_ptr(), *query.stride()[:2])
-            queries_out = (q_out.data_ptr(), *q_out.stride()[:2])
+            q_to = _row(q_out, dtype, q_shape, device)
+            if q_to is None:
+                check_tensors(("kv_cache", kv_cache, kv_dtype, kv_cache.shape), ("q_out", q_out, dtype, q_shape))
         kv_block, kv_part, kv_pos, kv_head, _ = kv_cache.stride()
         cache = kv_cache.data_ptr()
+        k_at, k_token, k_head = k_in
+        v_at, v_token, v_head = v_in
+        q_weighs, k_weighs, q_step, k_step, w_type = weights
+        at, stride, count, turning, axis, pairs = turns
         arguments = _pack(
-            *queries, keys.data_ptr(), values.data_ptr(), *keys.stride()[:2], *values.stride()[:2], *queries_out, cache,
+            *q_in, k_at, v_at, k_token, k_head, v_token, v_head, *q_to, cache,
             cache + kv_part * kv_cache.element_size() if cache else 0, kv_block, kv_pos, kv_head, pages, table.data_ptr(),
             table.stride(0), lens.data_ptr(), 0 if seen is None else seen.data_ptr(), at_first, first_stride,
-            0 if q_start is None else q_start.data_ptr(), at, stride, turning, axis, qw, kw, qw_stride, kw_stride, *kept,
-            ekv_hip.dtype_code(dtype), w_type, ekv_hip.dtype_code(kv_cache.dtype), rows, width, tokens, max_query, q_heads,
-            kv_heads, dim, block, pairs, count, bool(adjacent), bool(advance), bool(saturate), rotary_scale, eps,
-            weight_offset, k_scale, v_scale, 0)
-        status = (ekv_hip._lib or ekv_hip.load()).ekv_append_tokens(arguments, ekv_hip.stream_handle(stream))
+            0 if q_start is None else q_start.data_ptr(), at, stride, turning, axis, q_weighs, k_weighs, q_step, k_step,
+            *scores_at, *places_at, ekv_hip.dtype_code(dtype), w_type, ekv_hip.dtype_code(kv_dtype), rows, width, tokens,
+            max_query, q_heads, kv_heads, dim, block, pairs, count, 1 if adjacent else 0, 1 if advance else 0,
+            1 if saturate else 0, rotary_scale, eps, weight_offset, k_scale, v_scale, 0)
+        status = (ekv_hip._lib or ekv_hip.load()).ekv_append_tokens(arguments, handle)
     if status:
         ekv_hip.check(status, "ekv_append_tokens")
     return q_out

@@ -8,6 +8,8 @@ way into a paged cache.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 import ekv_hip
@@ -16,6 +18,11 @@ from observe.allocation import check_tensors
 _HEAD_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _pack = ekv_hip.packer(ekv_hip.Rotation)
 _INT = torch.int32
+_Tensor = torch.Tensor
+_STILL = (0, 0, 1, 0, 0, 0)  # no rotation
+_NO_WEIGHTS = (0, 0, 0, 0, 0)
+_NONE = (0, 0, 0)
+_HERE = contextlib.nullcontext()
 
 
 def rotary_frequencies(pairs: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -42,63 +49,86 @@ def section_axes(*pairs: int, interleaved: bool = False, device="cuda") -> torch
     return torch.tensor(axis, dtype=_INT, device=device)
 
 
-def _heads(name: str, t, tokens: int | None, dim: int | None, dtype) -> tuple[int, int, int]:
-    """(tokens, heads, dim) of a ``[tokens, heads, dim]`` tensor whose other sizes and type are known."""
-    if not isinstance(t, torch.Tensor) or t.ndim != 3:
+def _shape_of(name: str, t) -> tuple[int, int, int]:
+    if not isinstance(t, _Tensor) or t.ndim != 3:
         raise ValueError(f"{name} must be a [tokens, heads, dim] tensor")
-    shape = t.shape
-    if (tokens is not None and shape[0] != tokens) or (dim is not None and shape[2] != dim):
-        raise ValueError(f"{name} must be a [{tokens}, heads, {dim}] tensor, got {tuple(shape)}")
-    if t.dtype not in _HEAD_TYPES or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be {_HEAD_TYPES if dtype is None else dtype}, got {t.dtype}")
-    return shape
+    return t.shape
 
 
-def _turns(tokens: int, dim: int, positions, frequencies, axes, device) -> tuple[int, ...]:
-    """The fields (positions, stride, axes of them, frequencies, axes, pairs)."""
+def _row(t, dtype, shape, device: int):
+    """(address, strides of the tokens and heads) of a sound ``[tokens, heads, dim]`` tensor, else None: the usual call's
+    one look at it (``check_tensors`` finds the words for one that is not)."""
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == shape:
+        token, head, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), token, head
+    return None
+
+
+def _turns(tokens: int, dim: int, positions, frequencies, axes, device: int) -> tuple[int, ...]:
+    """The fields (positions, their stride and axes, frequencies, axes, pairs)."""
     if frequencies is None:
-        if axes is not None:
-            raise ValueError("axes need frequencies")
-        return 0, 0, 1, 0, 0, 0
-    if not isinstance(frequencies, torch.Tensor) or frequencies.ndim != 1:
+        if axes is not None or positions is not None:
+            raise ValueError("axes and positions need frequencies")
+        return _STILL
+    if not isinstance(frequencies, _Tensor) or frequencies.ndim != 1:
         raise ValueError("frequencies must be a [pairs] tensor")
-    pairs = frequencies.shape[0]
+    pairs, = frequencies.shape
     if 2 * pairs > dim:
         raise ValueError(f"{pairs} pairs of heads of {dim}")
-    at = stride = 0
+    at = stride = axis = 0
     count = 1
+    sound = frequencies.dtype is torch.float64 and frequencies.get_device() == device and frequencies.stride() == (1,)
     if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.ndim not in (1, 2) or positions.shape[-1] != tokens:
+        if not isinstance(positions, _Tensor) or positions.ndim not in (1, 2) or positions.shape[-1] != tokens:
             raise ValueError(f"positions must be a [{tokens}] or [axes, {tokens}] tensor")
-        if positions.ndim == 2:
-            count, stride = positions.shape[0], positions.stride(0)
+        steps = positions.stride()
+        if len(steps) == 2:
+            count, stride = positions.shape[0], steps[0]
         at = positions.data_ptr()
-    if check_tensors(("frequencies", frequencies, torch.float64, (pairs,)), ("axes", axes, _INT, (pairs,)),
-                     ("positions", positions if tokens else None, _INT, None if positions is None else positions.shape)) != device:
-        raise ValueError(f"frequencies must be on {device}")
-    if axes is None and count > 1:
+        sound = sound and positions.dtype is _INT and positions.get_device() == device and (steps[-1] == 1 or tokens == 0)
+    elif axes is not None:
+        raise ValueError("axes need positions")
+    if axes is not None:
+        axis = axes.data_ptr() if isinstance(axes, _Tensor) else 0
+        sound = sound and isinstance(axes, _Tensor) and axes.dtype is _INT and axes.shape == (pairs,) \
+            and axes.get_device() == device and axes.stride() == (1,)
+    elif count > 1:
         raise ValueError(f"positions of {count} axes need axes")
-    return at, stride, count, frequencies.data_ptr(), 0 if axes is None else axes.data_ptr(), pairs
+    if not sound:
+        there = check_tensors(("frequencies", frequencies, torch.float64, (pairs,)), ("axes", axes, _INT, (pairs,)),
+                              ("positions", positions if tokens else None, _INT, None if positions is None else positions.shape))
+        if there.index != device:
+            raise ValueError(f"frequencies must be on the heads' device, got {there}")
+    return at, stride, count, frequencies.data_ptr(), axis, pairs
 
 
-def _weights(q_weight, q_heads: int, k_weight, kv_heads: int, dim: int, dtype, device) -> tuple[int, int, int, int, int]:
+def _weight(name: str, w, heads: int, dim: int, dtype, device: int) -> tuple[int, int]:
+    """(address, stride of the heads) of a norm's weights."""
+    if not isinstance(w, _Tensor) or w.shape not in ((dim,), (heads, dim)):
+        raise ValueError(f"{name} must be a [{dim}] or [{heads}, {dim}] tensor")
+    if w.dtype != dtype and w.dtype != torch.float32:
+        raise ValueError(f"{name} must be {dtype} or float32, got {w.dtype}")
+    if w.stride(-1) != 1 or w.get_device() != device:
+        if check_tensors((name, w, w.dtype, w.shape)).index != device:
+            raise ValueError(f"{name} must be on the heads' device, got {w.device}")
+    return w.data_ptr(), w.stride(0) if w.ndim == 2 and heads > 1 else 0
+
+
+def _weights(q_weight, q_heads: int, k_weight, kv_heads: int, dim: int, dtype, device: int) -> tuple[int, int, int, int, int]:
     """The fields (q weight, k weight, their strides, type)."""
-    kind, fields = None, []
-    for name, w, heads in (("q_weight", q_weight, q_heads), ("k_weight", k_weight, kv_heads)):
-        if w is None:
-            fields.append((0, 0))
-            continue
-        if not isinstance(w, torch.Tensor) or w.shape not in ((dim,), (heads, dim)):
-            raise ValueError(f"{name} must be a [{dim}] or [{heads}, {dim}] tensor")
-        if w.dtype != dtype and w.dtype != torch.float32:
-            raise ValueError(f"{name} must be {dtype} or float32, got {w.dtype}")
-        if kind is not None and w.dtype != kind:
-            raise ValueError(f"k_weight must be {kind} as q_weight is, got {w.dtype}")
-        kind = w.dtype
-        if check_tensors((name, w, kind, w.shape)) != device:
-            raise ValueError(f"{name} must be on {device}")
-        fields.append((w.data_ptr(), w.stride(0) if w.ndim == 2 and heads > 1 else 0))
-    return fields[0][0], fields[1][0], fields[0][1], fields[1][1], ekv_hip.dtype_code(dtype if kind is None else kind)
+    if q_weight is None and k_weight is None:
+        return _NO_WEIGHTS
+    q_at = q_stride = k_at = k_stride = 0
+    if q_weight is not None:
+        q_at, q_stride = _weight("q_weight", q_weight, q_heads, dim, dtype, device)
+        kind = q_weight.dtype
+    if k_weight is not None:
+        k_at, k_stride = _weight("k_weight", k_weight, kv_heads, dim, dtype, device)
+        if q_weight is not None and k_weight.dtype != kind:
+            raise ValueError(f"k_weight must be {kind} as q_weight is, got {k_weight.dtype}")
+        kind = k_weight.dtype
+    return q_at, k_at, q_stride, k_stride, ekv_hip.dtype_code(kind)
 
 
 def rotate_heads(
@@ -133,32 +163,49 @@ def rotate_heads(
     limits as ``ekv_rotate_heads`` documents them.  ``stream``: the call launches and allocates as under
     ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
     through the call."""
-    tokens, q_heads, dim = _heads("query", query, None, None, None)
-    dtype, kv_heads = query.dtype, 0
+    tokens, q_heads, dim = q_shape = _shape_of("query", query)
+    dtype, kv_heads, k_shape = query.dtype, 0, None
     if key is not None:
-        kv_heads = _heads("key", key, tokens, dim, dtype)[1]
+        k_tokens, kv_heads, k_dim = k_shape = _shape_of("key", key)
+        if k_tokens != tokens or k_dim != dim:
+            raise ValueError(f"key must be a [{tokens}, heads, {dim}] tensor, got {tuple(k_shape)}")
     elif k_out is not None or k_weight is not None:
         raise ValueError("k_out and k_weight need a key")
     if frequencies is not None and positions is None:
         raise ValueError("frequencies need positions")
     if tokens == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
-        query, key = query.new_empty(query.shape), None if key is None else key.new_empty(key.shape)
-    device = check_tensors(("query", query, dtype, query.shape), ("key", key, dtype, None if key is None else key.shape),
-                           ("q_out", q_out, dtype, query.shape), ("k_out", k_out, dtype, None if key is None else key.shape))
-    at, stride, count, turning, axis, pairs = _turns(tokens, dim, positions, frequencies, axes, device)
-    qw, kw, qw_stride, kw_stride, w_type = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
-    with ekv_hip.beside(stream, query):
+        query, key = query.new_empty(q_shape), None if key is None else key.new_empty(k_shape)
+    device = query.get_device()
+    q_in, k_in = _row(query, dtype, q_shape, device), _NONE if key is None else _row(key, dtype, k_shape, device)
+    if device < 0 or dtype not in _HEAD_TYPES or q_in is None or k_in is None:
+        check_tensors(("query", query, _HEAD_TYPES, q_shape), ("key", key, dtype, k_shape), ("q_out", q_out, dtype, q_shape),
+                      ("k_out", k_out, dtype, k_shape))
+    turns = _turns(tokens, dim, positions, frequencies, axes, device)
+    weights = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
+    context, handle = ekv_hip.beside(stream, query)
+    with context or _HERE:
+        # an output made here is contiguous
         if q_out is None:
-            q_out = torch.empty(query.shape, dtype=dtype, device=device)
-        if k_out is None and key is not None:
-            k_out = torch.empty(key.shape, dtype=dtype, device=device)
-        keys = (0, 0, 0) if key is None else (key.data_ptr(), *key.stride()[:2])
-        keys_out = (0, 0, 0) if key is None else (k_out.data_ptr(), *k_out.stride()[:2])
+            q_out = torch.empty(tokens, q_heads, dim, dtype=dtype, device=query.device)
+            q_to = q_out.data_ptr(), q_heads * dim, dim
+        else:
+            q_to = _row(q_out, dtype, q_shape, device)
+        if key is None:
+            k_to = _NONE
+        elif k_out is None:
+            k_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=query.device)
+            k_to = k_out.data_ptr(), kv_heads * dim, dim
+        else:
+            k_to = _row(k_out, dtype, k_shape, device)
+        if q_to is None or k_to is None:
+            check_tensors(("query", query, dtype, q_shape), ("q_out", q_out, dtype, q_shape), ("k_out", k_out, dtype, k_shape))
+        q_weighs, k_weighs, q_step, k_step, w_type = weights
+        at, stride, count, turning, axis, pairs = turns
         arguments = _pack(
-            query.data_ptr(), *query.stride()[:2], *keys, q_out.data_ptr(), *q_out.stride()[:2], *keys_out, at, stride,
-            turning, axis, qw, kw, qw_stride, kw_stride, ekv_hip.dtype_code(dtype), w_type, tokens, q_heads, kv_heads, dim,
-            pairs, count, bool(adjacent), rotary_scale, eps, weight_offset)
-        status = (ekv_hip._lib or ekv_hip.load()).ekv_rotate_heads(arguments, ekv_hip.stream_handle(stream))
+            *q_in, *k_in, *q_to, *k_to, at, stride, turning, axis, q_weighs, k_weighs, q_step, k_step,
+            ekv_hip.dtype_code(dtype), w_type, tokens, q_heads, kv_heads, dim, pairs, count, 1 if adjacent else 0, rotary_scale,
+            eps, weight_offset)
+        status = (ekv_hip._lib or ekv_hip.load()).ekv_rotate_heads(arguments, handle)
     if status:
         ekv_hip.check(status, "ekv_rotate_heads")
     return q_out, k_out

@@ -162,7 +162,7 @@ def host(monkeypatch):
     monkeypatch.setattr(ekv_hip, "_lib", Library())
     monkeypatch.setattr(ekv_hip, "stream_handle", lambda stream=None: 5 if stream is None else stream.cuda_stream)
     for module in (runtime.append, runtime.rotary):
-        monkeypatch.setattr(module, "check_tensors", lambda *specs: torch.device("cpu"))
+        monkeypatch.setattr(module, "check_tensors", lambda *specs: types.SimpleNamespace(index=-1))
     return types.SimpleNamespace(launches=launches, patch=monkeypatch)
 
 
@@ -242,18 +242,21 @@ def test_another_device_and_its_streams(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(torch.cuda, "stream", lambda stream: ("under", stream))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=0: types.SimpleNamespace(cuda_stream=100 + device))
+    monkeypatch.setattr(ekv_hip, "stream_handle", lambda stream=None: 9 if stream is None else stream.cuda_stream)
     there = types.SimpleNamespace(get_device=lambda: 1, device=torch.device("cuda:1"))
-    with ekv_hip.beside(None, there):
-        assert entered == [1]
     here = types.SimpleNamespace(get_device=lambda: 0, device=torch.device("cuda:0"))
-    with ekv_hip.beside(None, here):
-        assert entered == [1]
     side = types.SimpleNamespace(cuda_stream=77, device=torch.device("cuda:0"))
-    assert ekv_hip.beside(side, here) == ("under", side)
-    with pytest.raises(ValueError, match="stream"):
-        ekv_hip.beside(side, there)
-    with ekv_hip.beside(None, torch.zeros(1)):
-        pass
+    for raw in (None, (lambda device: 200 + device, lambda: 0)):  # before and after the first call
+        monkeypatch.setattr(ekv_hip, "_raw_stream", raw)
+        context, handle = ekv_hip.beside(None, there)
+        with context:
+            assert entered.pop() == 1 and handle == 101
+        assert ekv_hip.beside(None, here) == (None, 9 if raw is None else 200)
+        assert ekv_hip.beside(side, here) == (("under", side), 77)
+        with pytest.raises(ValueError, match="stream"):
+            ekv_hip.beside(side, there)
+        assert ekv_hip.beside(None, torch.zeros(1)) == (None, 9)
 
 
 def test_sections():
