@@ -40,6 +40,7 @@ inline Heads heads_of(const void *at, int64_t token, int64_t head, int tokens, i
 }
 
 enum Kind { kQuery, kKey, kValue };
+enum Past { kNothing, kLoads, kAll };            // what of a pass goes past the caches
 enum Norm { kNone, kShared, kOfHeads };  // no weights; the same of every head; each head's own
 
 struct Params {
@@ -82,8 +83,7 @@ struct Unit<float> {
   u32x4 w, more;
 };
 
-// PAST the caches: where a launch moves more than the 256 MB Infinity Cache holds, its loads and stores are non-temporal
-// (launch_norm).
+// Accesses that go PAST the caches are non-temporal (launch_norm says when).
 template <class T, bool PAST>
 __device__ __forceinline__ Unit<T> load_unit(const char *at) {
   const auto *p = as_global((const u32x4 *)at);
@@ -167,7 +167,6 @@ __device__ __forceinline__ void store_unit(char *at, const Unit<C> &u) {
 // A lane's two units of 8 bytes.  Where a lane and its neighbour hold 16 bytes of the first unit and 16 of the second
 // beside each other (`paired`), one stores the first and one the second: whole pieces of 128 bytes of a head, where 8 bytes
 // a lane leave lines half written.
-template <bool PAST>
 __device__ __forceinline__ void store_e4m3(char *at, int a, int b, u32x2 x, u32x2 y, bool paired) {
   if (paired) {
     const bool odd = lane_id() & 1;
@@ -179,7 +178,7 @@ __device__ __forceinline__ void store_e4m3(char *at, int a, int b, u32x2 x, u32x
       w[i] = odd ? got : x[i];
       w[2 + i] = odd ? y[i] : got;
     }
-    store_unit<attn::FP8, PAST>(at + (odd ? b - kUnit : a), {w});
+    store_unit<attn::FP8, true>(at + (odd ? b - kUnit : a), {w});
   } else {
     *as_global((u32x2 *)(at + a)) = x;
     *as_global((u32x2 *)(at + b)) = y;
@@ -210,39 +209,64 @@ struct Place {
 
 __device__ __forceinline__ int capacity(const Params &p) { return p.width * p.block_size; }  // below 2^31 - 4096
 
-// The row of a token, and the row's first token and the next row's: the last of the ascending start[0 .. rows) that is
-// at most `token`, 62 ways at a step (a load for up to 62 rows and two for 3844, where halving takes a dozen), and its
-// neighbour out of the same load.  Row -1 for a token before the first.
-struct Span {
-  int row, begin, end;
-};
-__device__ __forceinline__ Span span_of(const int32_t *start, int rows, int token) {
-  constexpr int kWays = kWave - 2;
-  const int lane = lane_id();
-  int below = 0, n = rows;  // start[0 .. below) are at most `token`, start[below + n ..] are not
-  while (n > kWays) {
-    const int step = (n + kWays - 1) / kWays, i = (lane + 1) * step - 1;
-    const bool low = i < n && start[below + i] <= token;
-    const int whole = __popcll(__ballot(low)) * step;
-    below += whole;
-    n = min(step, n - whole);
-  }
-  const int i = below - 1 + lane;  // lane 0 has the last one known to be at most `token`
-  const int value = lane <= n + 1 && i >= 0 ? start[i] : 0;
-  const int found = __popcll(__ballot(lane >= 1 && lane <= n && value <= token));
-  return {below + found - 1, __builtin_amdgcn_readlane(value, found), __builtin_amdgcn_readlane(value, found + 1)};
-}
+// The row of a token: the last of the ascending start[0 .. rows) that is at most `token`.  load() asks for a window of 254
+// starts (of more rows, those between two of every rows / 64-th, and so on) and for their neighbours on both sides; find()
+// counts in it.  Between the two a wave asks for its first heads: what a wave asked for first is there first, so that the
+// row is known while the heads are on their way.
+struct RowSearch {
+  static constexpr int kHeld = 4;
+  int32_t value[kHeld];
+  int below, n;  // start[0 .. below) are at most `token`, start[below + n ..] are not
 
-__device__ __forceinline__ Place place_of(const Params &p, int token) {
+  __device__ __forceinline__ void load(const int32_t *start, int rows, int token) {
+    const int lane = lane_id();
+    below = 0;
+    n = rows;
+    while (n > kHeld * kWave - 2) {
+      const int step = (n + kWave - 1) / kWave, i = (lane + 1) * step - 1;
+      const bool low = i < n && start[below + i] <= token;
+      const int whole = __popcll(__ballot(low)) * step;
+      below += whole;
+      n = min(step, n - whole);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int j = k * kWave + lane, i = below - 1 + j;  // the first is the last one known to be at most `token`
+      value[k] = j <= n + 1 && i >= 0 ? start[i] : 0;
+    }
+  }
+  // (row, its first token, the next row's); row -1 for a token before the first
+  __device__ __forceinline__ void find(int token, int &row, int &begin, int &end) const {
+    const int lane = lane_id();
+    int found = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int j = k * kWave + lane;
+      found += __popcll(__ballot(j >= 1 && j <= n && value[k] <= token));
+    }
+    auto at = [&](int j) {
+      int v = __builtin_amdgcn_readlane(value[0], j & (kWave - 1));
+#pragma unroll
+      for (int k = 1; k < kHeld; ++k)
+        if (j / kWave == k) v = __builtin_amdgcn_readlane(value[k], j & (kWave - 1));
+      return v;
+    };
+    row = below + found - 1;
+    begin = at(found);
+    end = at(found + 1);
+  }
+};
+
+__device__ __forceinline__ Place place_of(const Params &p, int token, const RowSearch &search) {
   Place at{false, 0, 0, 0, false, -1};
   int count = 1, nth = 0;
   at.row = token;
   if (p.q_start != nullptr) {
-    const Span s = span_of(p.q_start, p.rows, token);
-    at.row = s.row;
+    int begin, end;
+    search.find(token, at.row, begin, end);
     if (at.row < 0) return at;
-    const int a = min(max(s.begin, 0), p.tokens);
-    const int b = min(max(s.end, a), p.tokens);
+    const int a = min(max(begin, 0), p.tokens);
+    const int b = min(max(end, a), p.tokens);
     count = b - a;
     nth = token - a;
   }
@@ -271,12 +295,12 @@ __device__ __forceinline__ void advance_row(const Params &p, int row, int t) {
 // -- the pass ---------------------------------------------------------------------------------------
 
 // T: the inputs' type.  C: the cache's (FP8 or T).  PAGED: with a cache and values; else keys go to k_out.  NORM: with
-// weights.  ADJACENT: the order of the pairs.  PAST: as load_unit
-// has it.
-template <class T, class C, bool PAGED, Norm NORM, bool ADJACENT, bool PAST>
+// weights.  ADJACENT: the order of the pairs.  PAST: what goes past
+// the caches.
+template <class T, class C, bool PAGED, Norm NORM, bool ADJACENT, Past PAST>
 __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
   __shared__ __align__(16) float s_cos[kWaves][kMostPairs], s_sin[kWaves][kMostPairs];
-  __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2 * kMostPairs];
+  __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2][2 * kMostPairs];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   const int lanes = 1 << p.lanes_log, per = kWave >> p.lanes_log;  // of a head; heads of a pass
   const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
@@ -304,44 +328,85 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
     const int kind = kind_of(pass), head = min(first_head(pass, kind) + nth, heads_of(kind) - 1);
     const Heads &from = p.in[kind];
     const char *x = from.at + token * from.token + head * from.head;
-    ua = load_unit<T, PAST>(x + a * sizeof(T));
-    ub = load_unit<T, PAST>(x + b * sizeof(T));
+    ua = load_unit<T, PAST != kNothing>(x + a * sizeof(T));
+    ub = load_unit<T, PAST != kNothing>(x + b * sizeof(T));
   };
 
-  if (token < p.tokens && part < passes) fetch(part);  // on its way while the token finds its place
-  int weighed = -1;  // the kind whose weights, the same for every head, s_weight holds
   if (token < p.tokens) {
+    // What the token's place, its angles and the norms are made of is asked for ahead of the heads.
+    RowSearch search;
+    if (PAGED && p.q_start != nullptr) search.load(p.q_start, p.rows, token);
+    constexpr int kTurns = kMostPairs / kWave;  // pairs of a lane
+    double frequency[kTurns];
+    int axis[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+      const int i = k * kWave + lane;
+      frequency[k] = i < p.pairs ? p.frequencies[i] : 0.0;
+      axis[k] = p.axes != nullptr && i < p.pairs ? p.axes[i] : 0;
+    }
+    constexpr int kWeights = NORM == kShared ? 2 * kMostPairs / kWave : 0;  // of a lane, for each of queries and keys
+    uint32_t weights[2][kWeights + 1];  // as they lie in memory: converting one here would wait for it here
+#pragma unroll
+    for (int k = 0; k < kWeights; ++k) {
+      const int i = k * kWave + lane;
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
+        weights[kind][k] = 0;
+        if (weight != nullptr && i < p.dim)
+          weights[kind][k] = p.weight_f32 ? as_global((const uint32_t *)weight)[i] : as_global((const uint16_t *)weight)[i];
+      }
+    }
+    if (part < passes) fetch(part);
+
     Place at{true, 0, 0, 0, false, -1};
-    if constexpr (PAGED) at = place_of(p, token);
+    if constexpr (PAGED) at = place_of(p, token, search);
+#pragma unroll
+    for (int k = 0; k < kWeights; ++k) {
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const uint32_t w = weights[kind][k];
+        const float x = p.weight_f32 || sizeof(T) == 4 ? __builtin_bit_cast(float, w)
+                        : std::is_same<T, __bf16>::value ? __builtin_bit_cast(float, w << 16)
+                                                         : (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+        s_weight[wave][kind][k * kWave + lane] = (kind == kQuery ? p.q_weight : p.k_weight) == nullptr ? 1.f : p.weight_offset + x;
+      }
+    }
 
     // the token's cosines and sines
     float cosine[kUnit], sine[kUnit];
     if (p.pairs > 0) {
       int64_t own = at.index;
       if (PAGED && p.first != nullptr && at.live) own += p.first[at.row * p.first_stride];
-      for (int i = lane; i < p.pairs; i += kWave) {
-        const int axis = p.axes != nullptr ? p.axes[i] : 0;
+#pragma unroll
+      for (int k = 0; k < kTurns; ++k) {
+        const int i = k * kWave + lane;
+        if (k * kWave >= p.pairs) break;
         double pos = (double)own;
-        if (p.positions != nullptr)
-          pos = (uint32_t)axis < (uint32_t)p.axis_count ? (double)p.positions[axis * p.positions_stride + token] : 0.0;
-        const double turn = pos * p.frequencies[i] * 0.15915494309189533577;  // 1 / 2 pi
+        if (p.positions != nullptr) {  // the axes' positions are scalar
+          int32_t mine = 0;
+          for (int x = 0; x < p.axis_count; ++x) mine = axis[k] == x ? p.positions[x * p.positions_stride + token] : mine;
+          pos = (double)mine;
+        }
+        const double turn = pos * frequency[k] * 0.15915494309189533577;  // 1 / 2 pi
         const float x = (float)(turn - __builtin_rint(turn));
         float s, c;
         sincospif(2.f * x, &s, &c);
         s_cos[wave][i] = c * p.rotary_scale;
         s_sin[wave][i] = s * p.rotary_scale;
       }
-      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      // adjacent: [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
-      const int low = !turns ? 0 : ADJACENT ? a / 2 : a, high = !turns ? 0 : ADJACENT ? b / 2 : a + 4;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // adjacent: [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
+    const int low = !turns ? 0 : ADJACENT ? a / 2 : a, high = !turns ? 0 : ADJACENT ? b / 2 : a + 4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        cosine[e] = s_cos[wave][low + e];
-        sine[e] = s_sin[wave][low + e];
-        cosine[4 + e] = s_cos[wave][high + e];
-        sine[4 + e] = s_sin[wave][high + e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      cosine[e] = s_cos[wave][low + e];
+      sine[e] = s_sin[wave][low + e];
+      cosine[4 + e] = s_cos[wave][high + e];
+      sine[4 + e] = s_sin[wave][high + e];
     }
 
     int64_t in_page = 0;
@@ -367,8 +432,8 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
       if (PAGED && (kind == kQuery ? !at.live : at.page < 0)) {
         if (kind == kQuery && mine) {
           char *to = (char *)p.out[kQuery].at + token * p.out[kQuery].token + head * p.out[kQuery].head;
-          store_unit<T, PAST>(to + a * sizeof(T), Unit<T>{});
-          store_unit<T, PAST>(to + b * sizeof(T), Unit<T>{});
+          store_unit<T, PAST == kAll>(to + a * sizeof(T), Unit<T>{});
+          store_unit<T, PAST == kAll>(to + b * sizeof(T), Unit<T>{});
         }
         continue;
       }
@@ -377,14 +442,6 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
       widen(vb, y);
       if (NORM != kNone && (!PAGED || kind != kValue)) {
         const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
-        if (NORM == kShared && weighed != kind) {
-          weighed = kind;
-          for (int i = lane; i < p.dim; i += kWave)
-            s_weight[wave][i] = weight == nullptr ? 1.f : p.weight_offset + (p.weight_f32 ? ((const float *)weight)[i]
-                                                                                          : (float)((const T *)weight)[i]);
-          __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-        }
         float squares = 0.f;
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) squares += x[e] * x[e] + y[e] * y[e];
@@ -405,8 +462,8 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         if constexpr (NORM == kShared) {
 #pragma unroll
           for (int e = 0; e < kUnit; ++e) {
-            wa[e] = s_weight[wave][a + e];
-            wb[e] = s_weight[wave][b + e];
+            wa[e] = s_weight[wave][kind][a + e];
+            wb[e] = s_weight[wave][kind][b + e];
           }
         } else {
 #pragma unroll
@@ -456,8 +513,8 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         if (mine) {
           const Heads &out = p.out[kind];
           char *to = (char *)out.at + (int64_t)token * out.token + head * out.head;
-          store_unit<T, PAST>(to + a * sizeof(T), narrow<T>(x));
-          store_unit<T, PAST>(to + b * sizeof(T), narrow<T>(y));
+          store_unit<T, PAST == kAll>(to + a * sizeof(T), narrow<T>(x));
+          store_unit<T, PAST == kAll>(to + b * sizeof(T), narrow<T>(y));
         }
       } else {  // the slot's key or value
         const float inverse = kind == kValue ? p.v_inverse : p.k_inverse;
@@ -469,10 +526,10 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         char *to = (kind == kValue ? p.values : p.keys) + in_page + head * p.st_head;
         if constexpr (std::is_same<C, attn::FP8>::value) {
           const u32x2 xa = narrow_e4m3(x, p.saturate), yb = narrow_e4m3(y, p.saturate);
-          if (mine) store_e4m3<PAST>(to, a, b, xa, yb, paired);
+          if (mine) store_e4m3(to, a, b, xa, yb, paired);
         } else if (mine) {
-          store_unit<T, PAST>(to + a * sizeof(T), narrow<T>(x));
-          store_unit<T, PAST>(to + b * sizeof(T), narrow<T>(y));
+          store_unit<T, true>(to + a * sizeof(T), narrow<T>(x));
+          store_unit<T, true>(to + b * sizeof(T), narrow<T>(y));
         }
       }
     }
@@ -499,32 +556,41 @@ __global__ __launch_bounds__(256) void advance_kernel(Params p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+template <class T, class C, bool PAGED, Norm NORM, Past PAST>
+int launch_pairs(const Params &p, hipStream_t stream, const char *who) {
+  const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.parts, kWaves)), block(kWaves * kWave);
+  if (p.adjacent) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, PAST>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, PAST>), grid, block, 0, stream, p);
+  return check_hip(hipGetLastError(), who);
+}
+
 template <class T, class C, bool PAGED, Norm NORM>
 int launch_norm(Params p, hipStream_t stream, const char *who) {
   p.lanes_log = p.dim <= 32 ? 1 : p.dim <= 64 ? 2 : p.dim <= 128 ? 3 : 4;
   p.q_passes = (int)ceil_div(p.q_heads, kWave >> p.lanes_log);
   p.kv_passes = (int)ceil_div(p.kv_heads, kWave >> p.lanes_log);
   const int passes = p.q_passes + (PAGED ? 2 : 1) * p.kv_passes;
-  // Waves of a token: four while that does not fill the chip, so that a pass of the heads is not behind another; one where
-  // there are tokens enough, which share a token's angles.
-  const int64_t enough = 16ll * cu_count();
-  p.parts = p.tokens * 4ll <= enough ? 4 : p.tokens * 2ll <= enough ? 2 : 1;
-  while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
-  // Loads and stores past the caches, us with against without, 32 query and 8 KV heads of 128 in bf16: 41000 tokens of
-  // prompts (1.0 GB) 172 / 186, into an fp8 cache (0.8 GB) 146 / 171; 16384 tokens' norms (0.34 GB) 63 / 68; prompts of 0.24
-  // GB 47 / 45, into an fp8 cache 0.25 GB 50 / 48, 0.13 GB 26 / 26, 0.06 GB 15 / 13.
+  // What goes past the 256 MB Infinity Cache (cache pages always do), by what the launch moves; 32 query and 8 KV heads of
+  // 128 in bf16, alone and followed by a kernel that reads the rotated queries, us: prompts of 117 MB 22 / 36 with the loads
+  // in the caches, 24 / 39 with neither loads nor queries in them; of 235 MB 49 / 75, 41 / 63 without the loads, 45 / 70
+  // without both; of 470 MB 92 / 142, 90 / 138 and 87 / 137; of 940 MB 172 / 277, 182 / 283 and 163 / 268.  Pieces that do not
+  // fill lines of 128 bytes are read twice past the caches: 500 MB of heads of 80 95 / 162, 105 / 173 and 112 / 180.
   const int64_t cache_bytes = std::is_same<C, attn::FP8>::value ? 1 : sizeof(T);
-  const int64_t moved = (2ll * p.q_heads + 2 * p.kv_heads) * sizeof(T) + 2 * p.kv_heads * cache_bytes;  // of a token's element
-  const bool past = p.tokens * p.dim * moved > 256ll << 20;
-  const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.parts, kWaves)), block(kWaves * kWave);
-  if (p.adjacent) {
-    if (past) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, false>), grid, block, 0, stream, p);
-  } else {
-    if (past) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, false>), grid, block, 0, stream, p);
+  const int64_t moved = p.tokens * (int64_t)p.dim *
+                        ((2ll * p.q_heads + 2 * p.kv_heads) * sizeof(T) + (PAGED ? 2 * p.kv_heads * cache_bytes : 0));
+  const bool whole = sizeof(T) == 2 && p.pairs % 64 == 0 && (p.dim / 2 - p.pairs) % 64 == 0;
+  const Past past = moved < 160ll << 20 ? kNothing : moved < 300ll << 20 ? kLoads : whole ? kAll : kNothing;
+  // Waves of a token: four while that does not fill the chip, so that a pass of the heads is not behind another (a decode
+  // step's 128 tokens 4.1 us, 4.7 with two, 6.4 with one); two where there are tokens enough (16384 tokens' norms 60 us, 61
+  // with one, 66 with four); four again where the launch outlasts its caches and has no weights to load (38000 tokens 156
+  // us, 167 with two, 173 with one).
+  p.parts = p.tokens * 4ll <= 16ll * cu_count() || (past == kAll && NORM == kNone) ? 4 : 2;
+  while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
+  switch (past) {
+    case kNothing: return launch_pairs<T, C, PAGED, NORM, kNothing>(p, stream, who);
+    case kLoads: return launch_pairs<T, C, PAGED, NORM, kLoads>(p, stream, who);
+    default: return launch_pairs<T, C, PAGED, NORM, kAll>(p, stream, who);
   }
-  return check_hip(hipGetLastError(), who);
 }
 
 template <class T, class C, bool PAGED>
