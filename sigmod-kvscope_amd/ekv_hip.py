@@ -123,10 +123,11 @@ def packer(block: type[ctypes.Structure]):
     codes = {_p: "P", _i64: "q", _i32: "i", _f32: "f"}
     layout = struct.Struct("@" + "".join(codes[kind] for _, kind in block._fields_) + "0q")
     assert layout.size == ctypes.sizeof(block)
+    made = layout.pack
 
     def pack(*fields) -> bytes:
         try:
-            return layout.pack(*fields)
+            return made(*fields)
         except (struct.error, OverflowError) as error:
             raise ValueError(f"arguments out of range: {error}") from None
 

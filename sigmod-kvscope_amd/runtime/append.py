@@ -110,9 +110,12 @@ def append_tokens(
     device = kv_cache.get_device()
     k_in, v_in = _row(keys, dtype, k_shape, device), _row(values, dtype, k_shape, device)
     q_in = _NONE if query is None else _row(query, dtype, q_shape, device)
-    if k_in is None or v_in is None or q_in is None or dtype not in _HEAD_TYPES or not _sound(
-            device, ((table, t_shape), (lens, (rows,)))) or ((q_start is not None or seen is not None) and not _sound(
-                device, ((q_start, (rows + 1,)), (seen, (rows,))))):
+    t_row, t_one = table.stride()
+    if k_in is None or v_in is None or q_in is None or device < 0 or dtype not in _HEAD_TYPES \
+            or table.dtype is not _INT or t_one != 1 or table.get_device() != device \
+            or not isinstance(lens, _Tensor) or lens.dtype is not _INT or lens.shape != (rows,) \
+            or lens.get_device() != device or lens.stride() != (1,) \
+            or ((q_start is not None or seen is not None) and not _sound(device, ((q_start, (rows + 1,)), (seen, (rows,))))):
         check_tensors(
             ("kv_cache", kv_cache, kv_dtype, kv_cache.shape), ("keys", keys, _HEAD_TYPES, k_shape),
             ("values", values, dtype, k_shape), ("query", query, dtype, q_shape),
@@ -148,7 +151,7 @@ def append_tokens(
         arguments = _pack(
             *q_in, k_at, v_at, k_token, k_head, v_token, v_head, *q_to, cache,
             cache + kv_part * kv_cache.element_size() if cache else 0, kv_block, kv_pos, kv_head, pages, table.data_ptr(),
-            table.stride(0), lens.data_ptr(), 0 if seen is None else seen.data_ptr(), at_first, first_stride,
+            t_row, lens.data_ptr(), 0 if seen is None else seen.data_ptr(), at_first, first_stride,
             0 if q_start is None else q_start.data_ptr(), at, stride, turning, axis, q_weighs, k_weighs, q_step, k_step,
             *scores_at, *places_at, ekv_hip.dtype_code(dtype), w_type, ekv_hip.dtype_code(kv_dtype), rows, width, tokens,
             max_query, q_heads, kv_heads, dim, block, pairs, count, 1 if adjacent else 0, 1 if advance else 0,

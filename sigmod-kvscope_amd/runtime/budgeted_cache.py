@@ -13,26 +13,42 @@ slots, so the table never changes.  A prompt that all rows share lies in the cac
         out, lse = cache.attend(query, scale)
         if cache.full:
             cache.trim()
+
+With ``rotation`` the cache norms and rotates what it is given, so that queries, keys and values come as the projection
+leaves them, and an eviction changes no position:
+
+    cache = BudgetedCache(rows, kv_heads, dim, budget=1024, rotation=dict(frequencies=rotary_frequencies(dim // 2)))
+    query = cache.append(keys, values, query=query)
+    out, lse = cache.attend(query, scale)
 """
 
 from __future__ import annotations
 
 import torch
 
+from runtime.append import append_tokens
 from runtime.eviction import evict_tokens
 from runtime.prefix_attention import prefix_attention
+
+_ROTATION = {"frequencies", "axes", "adjacent", "rotary_scale", "q_weight", "k_weight", "eps", "weight_offset"}
+_CACHE_TYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 
 
 class BudgetedCache:
     """``rows`` rows of at most ``budget + slack`` tokens behind a shared prefix of at most ``prefix`` tokens.  ``recent``
     and ``sinks``: the newest and the first tokens that an eviction spares; ``decay``: what a step leaves of the weight
-    accumulated before it; ``k_scale`` / ``v_scale``: an fp8 cache's scales."""
+    accumulated before it; ``k_scale`` / ``v_scale``: an fp8 cache's scales; ``rotation``: the arguments of ``append_tokens``
+    that norm and rotate (``frequencies``, ``axes``, ``adjacent``, ``rotary_scale``, ``q_weight``, ``k_weight``, ``eps``,
+    ``weight_offset``).  Keys and values then come as the model made them and are divided by the scales here; without it they
+    come rotated and already over the scales."""
 
     def __init__(self, rows: int, kv_heads: int, dim: int, budget: int, slack: int = 64, *, prefix: int = 0,
                  block: int = 16, dtype: torch.dtype = torch.bfloat16, recent: int = 32, sinks: int = 4,
-                 decay: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0, device="cuda"):
+                 decay: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0, rotation: dict | None = None, device="cuda"):
         if rows < 1 or budget < 1 or slack < 1 or prefix < 0 or block < 1:
             raise ValueError(f"{rows} rows of a budget of {budget} and {slack} tokens, a prefix of {prefix}, blocks of {block}")
+        if rotation is not None and not rotation.keys() <= _ROTATION:
+            raise ValueError(f"rotation has {sorted(rotation.keys() - _ROTATION)}, not among {sorted(_ROTATION)}")
         width, shared = -(-(budget + slack) // block), -(-prefix // block)
         pages = 1 + rows * width + shared
         self.capacity, self.budget, self.recent, self.sinks, self.decay = budget + slack, budget, recent, sinks, decay
@@ -51,6 +67,9 @@ class BudgetedCache:
         self.scores, self.positions = self._all_scores[:rows], self._all_positions[:rows]
         self._other_lens = torch.zeros_like(self.lens)
         self.longest = 0  # no row has more tokens (the device alone knows each row's)
+        self.rotation = rotation
+        # append_tokens writes what torch's indexing would, a dozen launches of it in one
+        self._one_pass = self.kv.is_cuda and dim % 16 == 0 and dim <= 256 and dtype in _CACHE_TYPES
 
     @property
     def full(self) -> bool:
@@ -68,21 +87,56 @@ class BudgetedCache:
             rows = rows.to(self.kv.dtype)
             raw[page, part, slot % self.block] = rows.view(torch.uint8) if raw is not self.kv else rows
 
-    def set_prefix(self, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """The prefix that every row shares: keys and values ``[tokens, kv_heads, dim]`` (already over an fp8 cache's scales)."""
+    def _new(self, *new: torch.Tensor) -> list[torch.Tensor]:
+        """Keys and values as append_tokens takes them: of the cache's type (or one it rounds from), at multiples of 16 bytes."""
+        kind = self.kv.dtype
+        if kind == torch.float8_e4m3fn:
+            kind = new[0].dtype if new[0].dtype in _CACHE_TYPES[:3] and new[0].dtype == new[1].dtype else torch.float32
+        ready = []
+        for rows in new:
+            rows = rows.to(kind)
+            token, head, one = rows.stride()
+            size = rows.element_size()
+            if one != 1 or rows.data_ptr() % 16 or (rows.shape[0] > 1 and token * size % 16) or (rows.shape[1] > 1 and head * size % 16):
+                rows = rows.clone(memory_format=torch.contiguous_format)
+            ready.append(rows)
+        return ready
+
+    def set_prefix(self, keys: torch.Tensor, values: torch.Tensor, positions: torch.Tensor | None = None) -> None:
+        """The prefix that every row shares: keys and values ``[tokens, kv_heads, dim]`` (without ``rotation`` already over an
+        fp8 cache's scales).  With ``rotation``: before the rows' tokens, whose positions follow the prefix's; ``positions``
+        int32 ``[tokens]`` or ``[axes, tokens]`` for other ones than 0, 1, 2 ..."""
         self._check(keys, values)
         n = keys.shape[0]
         if self.prefix_table is None or n > self.prefix_table.shape[1] * self.block:
             raise ValueError(f"no room for a prefix of {n} tokens")
+        if self.rotation is not None:
+            self.prefix_len.fill_(n)
+            start = torch.arange(2, dtype=torch.int32, device=self.kv.device) * n
+            append_tokens(self.kv, self.prefix_table, self.prefix_len, keys, values, q_start=start, max_query=max(1, n),
+                          positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(None))
+            return
+        if positions is not None:
+            raise ValueError("positions need a rotation")
         slot = torch.arange(n, device=self.kv.device)
         self._write(self.prefix_table[0, slot // self.block].long(), slot, keys, values)
         self.prefix_len.fill_(n)
 
-    def append(self, keys: torch.Tensor, values: torch.Tensor, q_start: torch.Tensor | None = None, max_query: int = 1) -> None:
+    def _turn(self, query) -> dict:
+        """The rotation's arguments, without the queries' weights where there are no queries."""
+        return self.rotation if query is not None else {k: v for k, v in self.rotation.items() if k != "q_weight"}
+
+    def append(self, keys: torch.Tensor, values: torch.Tensor, q_start: torch.Tensor | None = None, max_query: int = 1, *,
+               query: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor | None:
         """Each row's next tokens, ``[tokens, kv_heads, dim]``: row r's from ``q_start[r]`` to ``q_start[r + 1]`` (None: one a
         row), at most ``max_query``.  What passes it, or is no row's (padding before or behind the rows'), is not kept: the
-        device alone knows the counts, and no row outgrows its pages whatever they are."""
+        device alone knows the counts, and no row outgrows its pages whatever they are.
+
+        With ``rotation``: ``query [tokens, q_heads, dim]`` comes back normed and rotated; a token's position is the prefix's
+        length plus the count of its row's tokens before it, or ``positions`` int32 ``[tokens]`` or ``[axes, tokens]``."""
         self._check(keys, values)
+        if self.rotation is None and (query is not None or positions is not None):
+            raise ValueError("a query and positions need a rotation")
         rows, n, device = self.lens.shape[0], keys.shape[0], self.kv.device
         if q_start is None and n != rows:
             raise ValueError(f"{n} tokens of {rows} rows need q_start")
@@ -92,6 +146,19 @@ class BudgetedCache:
             raise ValueError(f"at most {max_query} tokens a row")
         if self.longest + max_query > self.capacity:
             raise ValueError(f"{max_query} more tokens pass the {self.capacity} of a row: trim first")
+        if self.rotation is not None or self._one_pass:
+            start = None if q_start is None else q_start.to(torch.int32).contiguous()
+            how = dict(saturate=False)
+            if self.rotation is not None:
+                how = dict(query=query, positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(query))
+                if self.prefix_table is not None:
+                    how["first"] = self.prefix_len.expand(rows)
+            else:
+                keys, values = self._new(keys, values)
+            query = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start, max_query=max_query,
+                                  seen=self.seen, scores=self.scores, slot_positions=self.positions, advance=True, **how)
+            self.longest += max_query
+            return query
         token = torch.arange(n, device=device)
         if q_start is None:
             row = into = token
@@ -113,6 +180,7 @@ class BudgetedCache:
         self.lens += counts
         self.seen += counts
         self.longest += max_query
+        return None
 
     def attend(self, query: torch.Tensor, scale: float, q_start: torch.Tensor | None = None, max_query: int = 1):
         """``(out, lse)`` of the newest tokens' queries ``[tokens, q_heads, dim]``; the own tokens' scores grow by the weight
