@@ -555,6 +555,7 @@ __global__ __launch_bounds__(256) void advance_kernel(Params p) {
 // -- host -----------------------------------------------------------------------------------------
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t kMostWaves = (1ll << 26) - 64;  // a launch has fewer than 2^32 threads
 
 template <class T, class C, bool PAGED, Norm NORM, Past PAST>
 int launch_pairs(const Params &p, hipStream_t stream, const char *who) {
@@ -586,11 +587,11 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   // us, 167 with two, 173 with one).
   p.parts = p.tokens * 4ll <= 16ll * cu_count() || (past == kAll && NORM == kNone) ? 4 : 2;
   while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
-  switch (past) {
-    case kNothing: return launch_pairs<T, C, PAGED, NORM, kNothing>(p, stream, who);
-    case kLoads: return launch_pairs<T, C, PAGED, NORM, kLoads>(p, stream, who);
-    default: return launch_pairs<T, C, PAGED, NORM, kAll>(p, stream, who);
-  }
+  while (p.parts > 1 && (int64_t)p.tokens * p.parts >= kMostWaves) p.parts /= 2;
+  if constexpr (sizeof(T) == 2)
+    if (past == kAll) return launch_pairs<T, C, PAGED, NORM, kAll>(p, stream, who);
+  return past == kLoads ? launch_pairs<T, C, PAGED, NORM, kLoads>(p, stream, who)
+                        : launch_pairs<T, C, PAGED, NORM, kNothing>(p, stream, who);
 }
 
 template <class T, class C, bool PAGED>
@@ -625,7 +626,7 @@ int fill(const Block *a, Params &p, const char *who) {
     return fail(EKV_EINVAL, "%s: tokens %d, heads %d / %d", who, a->tokens, a->q_heads, a->kv_heads);
   if (a->pairs > 0 && a->frequencies == nullptr) return fail(EKV_EINVAL, "%s: null pointer (frequencies)", who);
   if (a->pairs > 0 && a->positions != nullptr &&
-      (a->axis_count < 1 || (a->axis_count > 1 && a->positions_stride < a->tokens)))
+      (a->axis_count < 1 || a->positions_stride < 0))
     return fail(EKV_EINVAL, "%s: positions of %d axes, stride %lld", who, a->axis_count, (long long)a->positions_stride);
   if (!(a->eps >= 0.f)) return fail(EKV_EINVAL, "%s: eps %g", who, a->eps);
   const int e = bytes_of(a->dtype), we = bytes_of(a->weight_dtype);
@@ -680,7 +681,7 @@ extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
       !append::row_aligned(p.out[append::kKey]) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads and weights start at multiples of 16 bytes", who);
-  if (p.tokens >= 1 << 26) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
+  if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
     case EKV_F32: return append::launch<float, float, false>(p, s, "ekv_rotate_heads launch");
@@ -754,7 +755,7 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
     return fail(EKV_EINVAL, "%s: heads, weights and the cache's rows start at multiples of 16 bytes", who);
   if (p.table_stride < p.width)
     return fail(EKV_EINVAL, "%s: table rows of %d blocks, stride %lld", who, p.width, (long long)p.table_stride);
-  if (p.tokens >= 1 << 26) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
+  if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
   hipStream_t s = (hipStream_t)stream;
   const bool fp8 = a->kv_dtype == EKV_FP8_E4M3;
   int status;

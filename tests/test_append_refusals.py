@@ -37,10 +37,10 @@ def rotation(**over):
     (dict(pairs=12), "pairs"), (dict(pairs=40), "pairs"), (dict(tokens=-1), "tokens"), (dict(q_heads=-1), "heads"),
     (dict(kv_heads=(1 << 20) + 1), "heads"), (dict(frequencies=0), "null"), (dict(positions=0), "null"), (dict(query=0), "null"),
     (dict(q_out=0), "null"), (dict(key=0), "null"), (dict(k_out=0), "null"), (dict(axis_count=0), "axes"),
-    (dict(axis_count=2, positions_stride=2), "axes"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(axis_count=2, positions_stride=-1), "axes"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
     (dict(query=P + 8), "16 bytes"), (dict(k_out=P + 2), "16 bytes"), (dict(q_stride_head=68), "16 bytes"),
     (dict(k_stride_token=129), "16 bytes"), (dict(q_out_stride_token=4), "16 bytes"), (dict(q_weight=P + 4), "16 bytes"),
-    (dict(k_weight=P, k_weight_stride=20), "16 bytes"), (dict(tokens=1 << 26), "launch"),
+    (dict(k_weight=P, k_weight_stride=20), "16 bytes"), (dict(tokens=(1 << 26) - 64), "launch"),
 ])
 def test_rotation_arguments(over, match):
     a = rotation(**over)
@@ -70,7 +70,7 @@ def appending(**over):
     (dict(blocks=0), "empty cache"), (dict(new_keys=P + 8), "16 bytes"), (dict(new_values=P + 2), "16 bytes"),
     (dict(keys=P + 4), "16 bytes"), (dict(values=P + 8), "16 bytes"), (dict(kv_stride_pos=129), "16 bytes"),
     (dict(kv_stride_head=68), "16 bytes"), (dict(kv_stride_block=4097), "16 bytes"), (dict(v_stride_head=4), "16 bytes"),
-    (dict(k_weight=P + 8), "16 bytes"), (dict(table_stride=3), "stride"), (dict(rows=1 << 26, tokens=1 << 26), "launch"),
+    (dict(k_weight=P + 8), "16 bytes"), (dict(table_stride=3), "stride"), (dict(rows=1 << 26, tokens=(1 << 26)), "launch"),
     (dict(positions=P, axis_count=0), "axes"), (dict(eps=-1.0), "eps"), (dict(tokens=-1), "tokens"),
 ])
 def test_append_arguments(over, match):
@@ -150,6 +150,7 @@ def test_python_checks_come_before_the_device():
 def host(monkeypatch):
     """A library that notes (entry point, arguments, stream), and checks that let host tensors pass."""
     launches = []
+    monkeypatch.setattr(ekv_hip, "_raw_stream", None)
 
     class Library:
         def __getattr__(self, name):
@@ -223,6 +224,36 @@ def test_what_is_passed(host):
     assert (name, stream, a.query, a.q_heads, a.pairs, a.saturate, a.advance) == ("ekv_append_tokens", 5, None, 0, 0, 1, 1)
     assert (a.first, a.first_stride, a.values - a.keys, a.scores_stride_row) == (prefix.data_ptr(), 0, 2 * 2048, 80)
     assert a.new_values - a.new_keys == 256 and a.blocks == 4 and a.table_stride == 2
+
+
+def test_a_stream_is_what_a_call_allocates_on(host):
+    """With ``stream=`` every output is made while that stream is the current one, and the launch goes to it."""
+    current, made = [None], []
+
+    class Context:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            current.append(self.stream)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    empty = torch.empty
+
+    def noted(*args, **kwargs):
+        made.append(current[-1])
+        return empty(*args, **kwargs)
+
+    host.patch.setattr(torch.cuda, "stream", Context)
+    host.patch.setattr(torch, "empty", noted)
+    side = types.SimpleNamespace(cuda_stream=77)
+    x = torch.zeros(3, 2, 64)
+    rotate_heads(x, x, None, None, stream=side)
+    cache, table = torch.zeros(4, 2, 16, 2, 64), torch.zeros(3, 2, dtype=torch.int32)
+    append_tokens(cache, table, torch.ones(3, dtype=torch.int32), x, x, query=x, stream=side)
+    assert made == [side] * 3 and [stream for _, _, stream in host.launches] == [77, 77]
 
 
 def test_another_device_and_its_streams(monkeypatch):

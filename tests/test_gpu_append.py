@@ -7,6 +7,7 @@ import torch
 
 from append_cases import Tokens, check
 from runtime.append import append_tokens
+from runtime.rotary import rotary_frequencies
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16, FP8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
@@ -179,6 +180,32 @@ def test_offsets_past_32_bits():
     spread.copy_(args["query"])
     out = append_tokens(**{**args, "kv_cache": cache, "query": spread}, q_out=spread)
     check(batch, {**args, "kv_cache": cache[far.cuda()]}, out)
+
+
+@pytest.mark.parametrize("kv", [BF16, FP8], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("tokens", [9000, 14000, 30000])
+def test_sizes_around_the_caches(kv, tokens):
+    """Launches whose accesses differ by their size: the same bytes as the rows appended in pieces."""
+    heads, dim, block, rows = 8, 128, 16, 3
+    packed = torch.randn(tokens, 4 * heads, dim, device="cuda").to(BF16)
+    query, keys, values = packed[:, :2 * heads], packed[:, 2 * heads:3 * heads], packed[:, 3 * heads:]
+    counts = [tokens // 2, 1, tokens - tokens // 2 - 1]
+    start = torch.tensor([0, counts[0], counts[0] + 1, tokens], dtype=torch.int32, device="cuda")
+    width = -(-max(counts) // block)
+    table = torch.randperm(rows * width, device="cuda").to(torch.int32).view(rows, width)
+    lens = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    how = dict(frequencies=rotary_frequencies(dim // 2), k_scale=0.02, v_scale=0.02)
+    cache = torch.zeros(rows * width, 2, block, heads, dim, dtype=kv, device="cuda")
+    got = append_tokens(cache, table, lens, keys, values, q_start=start, max_query=max(counts), query=query, **how)
+    want, out = torch.zeros_like(cache), torch.empty_like(got)
+    for r in range(rows):
+        for a in range(0, counts[r], 1000):
+            b = min(counts[r], a + 1000)
+            part = slice(int(start[r]) + a, int(start[r]) + b)
+            out[part] = append_tokens(want, table[r:r + 1], torch.full((1,), b, dtype=torch.int32, device="cuda"), keys[part],
+                                      values[part], q_start=torch.tensor([0, b - a], dtype=torch.int32, device="cuda"),
+                                      max_query=b - a, query=query[part], **how)
+    assert torch.equal(got, out) and torch.equal(cache.view(torch.uint8), want.view(torch.uint8))
 
 
 def test_captured_steps():

@@ -177,6 +177,45 @@ def test_sections_on_the_device():
     assert torch.equal(same, want)  # text: every axis the same position
 
 
+@pytest.mark.parametrize("tokens,dim", [(2**25 + 3, 16), (2**24 + 5, 128)])
+def test_more_waves_than_a_launch_has_threads_for(tokens, dim):
+    """A token a wave where two or four would pass 2^32 threads: slices of the call's result are those of calls of their own."""
+    x = torch.empty(tokens, 1, dim, dtype=BF16, device="cuda")
+    for a in range(0, tokens, 2**22):
+        x[a:a + 2**22] = torch.randn(min(2**22, tokens - a), 1, dim, device="cuda")
+    at = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    f = rotary_frequencies(dim // 2)
+    got, _ = rotate_heads(x, None, at, f)
+    for a in (0, 2**22 - 9, 2**24 - 17, tokens - 1000):
+        part = slice(a, a + 1000)
+        want, _ = rotate_heads(x[part], None, at[part], f)
+        assert torch.equal(got[part], want)
+
+
+@pytest.mark.parametrize("pairs,dim,dtype", [(64, 128, BF16), (40, 80, F16), (64, 128, F32), (32, 128, BF16)])
+@pytest.mark.parametrize("tokens", [9000, 21000, 60000])
+def test_sizes_around_the_caches(pairs, dim, dtype, tokens):
+    """Launches of 60 MB to 2 GB, whose accesses differ: slices of the result are those of small calls."""
+    x = torch.randn(tokens, 16, dim, device="cuda").to(dtype)
+    at = torch.arange(tokens, dtype=torch.int32, device="cuda") + 1000
+    f, w = rotary_frequencies(pairs), torch.rand(dim, device="cuda").to(dtype)
+    for weight in (None, w):
+        query, key = rotate_heads(x[:, :12], x[:, 12:], at, f, q_weight=weight, k_weight=weight)
+        for a in (0, tokens // 2 + 1, tokens - 700):
+            part = slice(a, a + 700)
+            want = rotate_heads(x[part, :12], x[part, 12:], at[part], f, q_weight=weight, k_weight=weight)
+            assert torch.equal(query[part], want[0]) and torch.equal(key[part], want[1])
+
+
+def test_axes_of_one_row_of_positions():
+    """Positions that are one row seen as three."""
+    n = torch.arange(50, dtype=torch.int32, device="cuda")
+    x = torch.randn(50, 2, 64, device="cuda")
+    got, _ = rotate_heads(x, None, n.expand(3, 50), rotary_frequencies(32), axes=section_axes(8, 12, 12))
+    want, _ = rotate_heads(x, None, n, rotary_frequencies(32))
+    assert torch.equal(got, want)
+
+
 def test_no_tokens():
     x = torch.empty(0, 4, 64, device="cuda", dtype=BF16)
     query, key = rotate_heads(x, x, torch.empty(0, dtype=torch.int32, device="cuda"), rotary_frequencies(32))
