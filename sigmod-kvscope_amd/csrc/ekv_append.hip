@@ -376,7 +376,8 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         const float x = p.weight_f32 || sizeof(T) == 4 ? __builtin_bit_cast(float, w)
                         : std::is_same<T, __bf16>::value ? __builtin_bit_cast(float, w << 16)
                                                          : (float)__builtin_bit_cast(_Float16, (uint16_t)w);
-        s_weight[wave][kind][k * kWave + lane] = (kind == kQuery ? p.q_weight : p.k_weight) == nullptr ? 1.f : p.weight_offset + x;
+        const bool weighs = (kind == kQuery ? p.q_weight : p.k_weight) != nullptr;
+        s_weight[wave][kind][k * kWave + lane] = weighs ? p.weight_offset + x : 1.f;
       }
     }
 
@@ -392,7 +393,10 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
         double pos = (double)own;
         if (p.positions != nullptr) {  // the axes' positions are scalar
           int32_t mine = 0;
-          for (int x = 0; x < p.axis_count; ++x) mine = axis[k] == x ? p.positions[x * p.positions_stride + token] : mine;
+          for (int x = 0; x < p.axis_count; ++x) {
+            const int32_t there = __builtin_amdgcn_readfirstlane(p.positions[x * p.positions_stride + token]);
+            mine = axis[k] == x ? there : mine;
+          }
           pos = (double)mine;
         }
         const double turn = pos * frequency[k] * 0.15915494309189533577;  // 1 / 2 pi
@@ -669,6 +673,9 @@ bool weight_aligned(const char *at, int64_t stride) { return aligned16(at) && st
 }  // namespace ekv
 
 using namespace ekv;
+using append::kKey;
+using append::kQuery;
+using append::kValue;
 
 extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
   const char *who = "ekv_rotate_heads";
@@ -677,14 +684,15 @@ extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
   const int rc = append::fill(a, p, who);
   if (rc != EKV_OK) return rc;
   const int e = append::bytes_of(a->dtype);
-  p.in[append::kKey] = append::heads_of(a->key, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
-  p.out[append::kKey] = append::heads_of(a->k_out, a->k_out_stride_token, a->k_out_stride_head, a->tokens, a->kv_heads, e);
+  p.in[kKey] = append::heads_of(a->key, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.out[kKey] = append::heads_of(a->k_out, a->k_out_stride_token, a->k_out_stride_head, a->tokens, a->kv_heads, e);
   if (p.tokens == 0 || p.q_heads + p.kv_heads == 0) return EKV_OK;
-  if ((p.q_heads > 0 && (p.in[append::kQuery].at == nullptr || p.out[append::kQuery].at == nullptr)) ||
-      (p.kv_heads > 0 && (p.in[append::kKey].at == nullptr || p.out[append::kKey].at == nullptr)) || (p.pairs > 0 && p.positions == nullptr))
+  if ((p.q_heads > 0 && (p.in[kQuery].at == nullptr || p.out[kQuery].at == nullptr)) ||
+      (p.kv_heads > 0 && (p.in[kKey].at == nullptr || p.out[kKey].at == nullptr)) ||
+      (p.pairs > 0 && p.positions == nullptr))
     return fail(EKV_EINVAL, "%s: null pointer", who);
-  if (!append::row_aligned(p.in[append::kQuery]) || !append::row_aligned(p.out[append::kQuery]) || !append::row_aligned(p.in[append::kKey]) ||
-      !append::row_aligned(p.out[append::kKey]) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
+  if (!append::row_aligned(p.in[kQuery]) || !append::row_aligned(p.out[kQuery]) || !append::row_aligned(p.in[kKey]) ||
+      !append::row_aligned(p.out[kKey]) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads and weights start at multiples of 16 bytes", who);
   if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
@@ -715,8 +723,8 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   if (!(a->k_scale > 0.f) || !(a->v_scale > 0.f))
     return fail(EKV_EINVAL, "%s: scales %g and %g", who, a->k_scale, a->v_scale);
   const int e = append::bytes_of(a->dtype), ce = append::bytes_of(a->kv_dtype);
-  p.in[append::kKey] = append::heads_of(a->new_keys, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
-  p.in[append::kValue] = append::heads_of(a->new_values, a->v_stride_token, a->v_stride_head, a->tokens, a->kv_heads, e);
+  p.in[kKey] = append::heads_of(a->new_keys, a->k_stride_token, a->k_stride_head, a->tokens, a->kv_heads, e);
+  p.in[kValue] = append::heads_of(a->new_values, a->v_stride_token, a->v_stride_head, a->tokens, a->kv_heads, e);
   p.keys = (char *)a->keys;
   p.values = (char *)a->values;
   p.st_block = a->blocks > 1 ? a->kv_stride_block * ce : 0;
@@ -749,13 +757,13 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   p.v_inverse = (float)(1.0 / a->v_scale);
   if (p.tokens == 0) return EKV_OK;
   if (p.rows == 0) return fail(EKV_EINVAL, "%s: %d tokens of no row", who, p.tokens);
-  if (p.in[append::kKey].at == nullptr || p.in[append::kValue].at == nullptr || p.lens == nullptr ||
-      (p.q_heads > 0 && (p.in[append::kQuery].at == nullptr || p.out[append::kQuery].at == nullptr)) ||
+  if (p.in[kKey].at == nullptr || p.in[kValue].at == nullptr || p.lens == nullptr ||
+      (p.q_heads > 0 && (p.in[kQuery].at == nullptr || p.out[kQuery].at == nullptr)) ||
       (p.width > 0 && (p.keys == nullptr || p.values == nullptr || p.table == nullptr)))
     return fail(EKV_EINVAL, "%s: null pointer", who);
   if (p.blocks < 1 && p.width > 0) return fail(EKV_EINVAL, "%s: tables of an empty cache", who);
-  if (!append::row_aligned(p.in[append::kQuery]) || !append::row_aligned(p.out[append::kQuery]) || !append::row_aligned(p.in[append::kKey]) ||
-      !append::row_aligned(p.in[append::kValue]) || !append::aligned16(p.keys) || !append::aligned16(p.values) || p.st_block % 16 != 0 ||
+  if (!append::row_aligned(p.in[kQuery]) || !append::row_aligned(p.out[kQuery]) || !append::row_aligned(p.in[kKey]) ||
+      !append::row_aligned(p.in[kValue]) || !append::aligned16(p.keys) || !append::aligned16(p.values) || p.st_block % 16 != 0 ||
       p.st_pos % 16 != 0 || p.st_head % 16 != 0 || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads, weights and the cache's rows start at multiples of 16 bytes", who);
