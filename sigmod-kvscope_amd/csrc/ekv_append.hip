@@ -592,10 +592,13 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   const bool whole = sizeof(T) == 2 && p.pairs % 64 == 0 && (p.dim / 2 - p.pairs) % 64 == 0;
   const Past past = moved < 160ll << 20 ? kNothing : moved < 300ll << 20 ? kLoads : whole ? kAll : kNothing;
   // Waves of a token: four while that does not fill the chip, so that a pass of the heads is not behind another (a decode
-  // step's 128 tokens 4.1 us, 4.7 with two, 6.4 with one); two where there are tokens enough (16384 tokens' norms 60 us, 61
-  // with one, 66 with four); four again where the launch outlasts its caches and has no weights to load (38000 tokens 156
-  // us, 167 with two, 173 with one).
-  p.parts = p.tokens * 4ll <= 16ll * cu_count() || (past == kAll && NORM == kNone) ? 4 : 2;
+  // step's 128 tokens 4.1 us, 4.7 with two, 6.4 with one).  Where there are tokens enough a wave needs passes enough for what
+  // it does once, its token's place and angles: two waves from five passes on (16384 tokens' norms, five passes, 60 us, 61
+  // with one, 66 with four; 9536 tokens of 16 query and 2 KV heads into a cache, four passes, 21.8, 20.6 with one, 29.3 with
+  // four; of 8 and 1, three, 19.3, 16.7, 27.4), and four where the launch outlasts its caches, has no weights to load and six
+  // passes (38000 tokens 156 us, 167 with two, 173 with one).
+  const bool few = p.tokens * 4ll <= 16ll * cu_count();
+  p.parts = few || (past == kAll && NORM == kNone && passes > 5) ? 4 : passes >= 5 ? 2 : 1;
   while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
   while (p.parts > 1 && (int64_t)p.tokens * p.parts >= kMostWaves) p.parts /= 2;
   if constexpr (sizeof(T) == 2)
