@@ -13,11 +13,13 @@ import torch
 import ekv_hip
 from observe.allocation import check_tensors
 from runtime.prefix_attention import _cache_shape, _sound
-from runtime.rotary import _HEAD_TYPES, _HERE, _NONE, _row, _shape_of, _turns, _weights
+from runtime.rotary import _HEAD_TYPES, _HERE, _NO_WEIGHTS, _look, _output, _turns, _weights
 
 _pack = ekv_hip.packer(ekv_hip.Append)
 _INT, _FLOAT = torch.int32, torch.float32
+_FP8 = torch.float8_e4m3fn
 _Tensor = torch.Tensor
+_NONE = (0, 0, 0)
 
 
 def _slots(name: str, t, kind, rows: int, heads: int, least: int, device: int) -> tuple[int, int, int]:
@@ -82,79 +84,80 @@ def append_tokens(
     and limits as ``ekv_append_tokens`` documents them.  ``stream``: the call launches and allocates as under
     ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
     through the call."""
-    pages, block, kv_heads, dim = _cache_shape(kv_cache)
+    if not isinstance(kv_cache, _Tensor) or kv_cache.ndim != 5:
+        _cache_shape(kv_cache)  # refuses it
+    pages, _, block, kv_heads, dim = c_shape = kv_cache.shape
+    kv_block, kv_part, kv_pos, kv_head, kv_one = kv_cache.stride()
+    if c_shape[1] != 2 or kv_one != 1 or block < 1 or kv_heads < 1:
+        _cache_shape(kv_cache)
     if not isinstance(table, _Tensor) or table.ndim != 2:
         raise ValueError("the block table must be a [rows, width] tensor")
     rows, width = t_shape = table.shape
-    tokens, heads, k_dim = k_shape = _shape_of("keys", keys)
+    t_row, t_one = table.stride()
+    k_shape, dtype, k_device, k_at, k_token, k_head, sound = _look("keys", keys)
+    tokens, heads, k_dim = k_shape
     if heads != kv_heads or k_dim != dim:
         raise ValueError(f"keys must be a [tokens, {kv_heads}, {dim}] tensor, got {tuple(k_shape)}")
-    dtype, kv_dtype, q_heads, q_shape = keys.dtype, kv_cache.dtype, 0, None
-    if kv_dtype is not dtype and kv_dtype is not torch.float8_e4m3fn:
+    kv_dtype, device = kv_cache.dtype, kv_cache.get_device()
+    if kv_dtype is not dtype and kv_dtype is not _FP8:
         raise ValueError(f"keys of {dtype} for a cache of {kv_dtype}")
+    v_shape, v_type, v_device, v_at, v_token, v_head, v_sound = _look("values", values)
+    sound = sound and v_sound and v_shape == k_shape and v_type is dtype and k_device == v_device == device
+    q_shape, q_heads, q_at, q_token, q_head = None, 0, 0, 0, 0
     if query is not None:
-        q_tokens, q_heads, q_dim = q_shape = _shape_of("query", query)
+        q_shape, q_type, q_device, q_at, q_token, q_head, q_sound = _look("query", query)
+        q_tokens, q_heads, q_dim = q_shape
         if q_tokens != tokens or q_dim != dim:
             raise ValueError(f"query must be a [{tokens}, heads, {dim}] tensor, got {tuple(q_shape)}")
+        sound = sound and q_sound and q_type is dtype and q_device == device
     elif q_out is not None or q_weight is not None:
         raise ValueError("q_out and q_weight need a query")
     if frequencies is None and positions is not None:
         raise ValueError("positions need frequencies")
-    if width == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
-        table = table.new_empty(t_shape)
-    if tokens == 0:
-        if not isinstance(values, _Tensor) or values.shape != k_shape or values.dtype != dtype:
-            raise ValueError(f"values must be {dtype} of shape {tuple(k_shape)}")
-        keys, values = keys.new_empty(k_shape), values.new_empty(k_shape)
-        query = None if query is None else query.new_empty(q_shape)
-    device = kv_cache.get_device()
-    k_in, v_in = _row(keys, dtype, k_shape, device), _row(values, dtype, k_shape, device)
-    q_in = _NONE if query is None else _row(query, dtype, q_shape, device)
-    t_row, t_one = table.stride()
-    if k_in is None or v_in is None or q_in is None or device < 0 or dtype not in _HEAD_TYPES \
-            or table.dtype is not _INT or t_one != 1 or table.get_device() != device \
-            or not isinstance(lens, _Tensor) or lens.dtype is not _INT or lens.shape != (rows,) \
-            or lens.get_device() != device or lens.stride() != (1,) \
-            or ((q_start is not None or seen is not None) and not _sound(device, ((q_start, (rows + 1,)), (seen, (rows,))))):
+    if not sound or device < 0 or dtype not in _HEAD_TYPES or table.dtype is not _INT or t_one != 1 \
+            or table.get_device() != device or not isinstance(lens, _Tensor) or lens.dtype is not _INT or lens.shape != (rows,) \
+            or lens.get_device() != device or lens.stride() != (1,) or ((q_start is not None or seen is not None) and not _sound(
+                device, ((q_start, (rows + 1,)), (seen, (rows,))))):
+        if width == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
+            table = table.new_empty(t_shape)
+        if tokens == 0:
+            if v_shape != k_shape or v_type != dtype:
+                raise ValueError(f"values must be {dtype} of shape {tuple(k_shape)}, got {v_type} of {tuple(v_shape)}")
+            keys, values = keys.new_empty(k_shape), values.new_empty(k_shape)
+            query = None if query is None else query.new_empty(q_shape)
         check_tensors(
-            ("kv_cache", kv_cache, kv_dtype, kv_cache.shape), ("keys", keys, _HEAD_TYPES, k_shape),
+            ("kv_cache", kv_cache, kv_dtype, c_shape), ("keys", keys, _HEAD_TYPES, k_shape),
             ("values", values, dtype, k_shape), ("query", query, dtype, q_shape),
-            ("q_out", q_out, dtype, q_shape), ("table", table, _INT, t_shape), ("lens", lens, _INT, (rows,)), ("q_start", q_start, _INT, (rows + 1,)),
-            ("seen", seen, _INT, (rows,)))
-    turns = _turns(tokens, dim, positions, frequencies, axes, device)
-    weights = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
+            ("q_out", q_out, dtype, q_shape), ("table", table, _INT, t_shape), ("lens", lens, _INT, (rows,)),
+            ("q_start", q_start, _INT, (rows + 1,)), ("seen", seen, _INT, (rows,)))
+    at, stride, count, turning, axis, pairs = _turns(tokens, dim, positions, frequencies, axes, device)
+    q_weighs, k_weighs, q_step, k_step, w_type = _NO_WEIGHTS if q_weight is None and k_weight is None else \
+        _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
     at_first = first_stride = 0
     if first is not None:
         if not isinstance(first, _Tensor) or first.shape != (rows,) or first.dtype != _INT or first.get_device() != device:
             raise ValueError(f"first must be an int32 [{rows}] tensor on the cache's device")
         at_first, first_stride = first.data_ptr(), first.stride(0)
-    scores_at = _NONE if scores is None else _slots("scores", scores, _FLOAT, rows, kv_heads, width * block, device)
-    places_at = _NONE if slot_positions is None else \
+    s_at, s_row, s_head = _NONE if scores is None else _slots("scores", scores, _FLOAT, rows, kv_heads, width * block, device)
+    p_at, p_row, p_head = _NONE if slot_positions is None else \
         _slots("slot_positions", slot_positions, _INT, rows, kv_heads, width * block, device)
     context, handle = ekv_hip.beside(stream, kv_cache)
     with context or _HERE:
-        if query is None:
-            q_to = _NONE
-        elif q_out is None:
-            q_out = torch.empty(tokens, q_heads, dim, dtype=dtype, device=kv_cache.device)
-            q_to = q_out.data_ptr(), q_heads * dim, dim
-        else:
-            q_to = _row(q_out, dtype, q_shape, device)
-            if q_to is None:
-                check_tensors(("kv_cache", kv_cache, kv_dtype, kv_cache.shape), ("q_out", q_out, dtype, q_shape))
-        kv_block, kv_part, kv_pos, kv_head, _ = kv_cache.stride()
+        o_at = o_token = o_head = 0
+        if query is not None:
+            if q_out is None:
+                q_out = torch.empty(tokens, q_heads, dim, dtype=dtype, device=kv_cache.device)
+                o_at, o_token, o_head = q_out.data_ptr(), q_heads * dim, dim
+            else:
+                o_at, o_token, o_head = _output("q_out", q_out, dtype, q_shape, kv_cache)
         cache = kv_cache.data_ptr()
-        k_at, k_token, k_head = k_in
-        v_at, v_token, v_head = v_in
-        q_weighs, k_weighs, q_step, k_step, w_type = weights
-        at, stride, count, turning, axis, pairs = turns
         arguments = _pack(
-            *q_in, k_at, v_at, k_token, k_head, v_token, v_head, *q_to, cache,
+            q_at, q_token, q_head, k_at, v_at, k_token, k_head, v_token, v_head, o_at, o_token, o_head, cache,
             cache + kv_part * kv_cache.element_size() if cache else 0, kv_block, kv_pos, kv_head, pages, table.data_ptr(),
             t_row, lens.data_ptr(), 0 if seen is None else seen.data_ptr(), at_first, first_stride,
             0 if q_start is None else q_start.data_ptr(), at, stride, turning, axis, q_weighs, k_weighs, q_step, k_step,
-            *scores_at, *places_at, ekv_hip.dtype_code(dtype), w_type, ekv_hip.dtype_code(kv_dtype), rows, width, tokens,
-            max_query, q_heads, kv_heads, dim, block, pairs, count, 1 if adjacent else 0, 1 if advance else 0,
+            s_at, s_row, s_head, p_at, p_row, p_head, ekv_hip.dtype_code(dtype), w_type, ekv_hip.dtype_code(kv_dtype), rows,
+            width, tokens, max_query, q_heads, kv_heads, dim, block, pairs, count, 1 if adjacent else 0, 1 if advance else 0,
             1 if saturate else 0, rotary_scale, eps, weight_offset, k_scale, v_scale, 0)
         status = (ekv_hip._lib or ekv_hip.load()).ekv_append_tokens(arguments, handle)
     if status:

@@ -21,7 +21,6 @@ _INT = torch.int32
 _Tensor = torch.Tensor
 _STILL = (0, 0, 1, 0, 0, 0)  # no rotation
 _NO_WEIGHTS = (0, 0, 0, 0, 0)
-_NONE = (0, 0, 0)
 _HERE = contextlib.nullcontext()
 
 
@@ -49,20 +48,23 @@ def section_axes(*pairs: int, interleaved: bool = False, device="cuda") -> torch
     return torch.tensor(axis, dtype=_INT, device=device)
 
 
-def _shape_of(name: str, t) -> tuple[int, int, int]:
-    if not isinstance(t, _Tensor) or t.ndim != 3:
-        raise ValueError(f"{name} must be a [tokens, heads, dim] tensor")
-    return t.shape
+def _look(name: str, t) -> tuple:
+    """(shape, type, device, address, strides of the tokens and heads, whether rows are contiguous) of a ``[tokens, heads,
+    dim]`` tensor: the usual call's one look at it (``check_tensors`` finds the words for one that is not sound)."""
+    if isinstance(t, _Tensor):
+        shape = t.shape
+        if len(shape) == 3:
+            token, head, one = t.stride()
+            return shape, t.dtype, t.get_device(), t.data_ptr(), token, head, one == 1 or shape[0] == 0
+    raise ValueError(f"{name} must be a [tokens, heads, dim] tensor")
 
 
-def _row(t, dtype, shape, device: int):
-    """(address, strides of the tokens and heads) of a sound ``[tokens, heads, dim]`` tensor, else None: the usual call's
-    one look at it (``check_tensors`` finds the words for one that is not)."""
-    if isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == shape:
-        token, head, one = t.stride()
-        if one == 1:
-            return t.data_ptr(), token, head
-    return None
+def _output(name: str, t, dtype, shape, like) -> tuple[int, int, int]:
+    """(address, strides of the tokens and heads) of a given output, which is of ``like``'s device."""
+    o_shape, o_type, o_device, at, token, head, sound = _look(name, t)
+    if not sound or o_shape != shape or o_type is not dtype or o_device != like.get_device():
+        check_tensors(("the input", like, like.dtype, like.shape), (name, t, dtype, shape))
+    return at, token, head
 
 
 def _turns(tokens: int, dim: int, positions, frequencies, axes, device: int) -> tuple[int, ...]:
@@ -163,48 +165,46 @@ def rotate_heads(
     limits as ``ekv_rotate_heads`` documents them.  ``stream``: the call launches and allocates as under
     ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
     through the call."""
-    tokens, q_heads, dim = q_shape = _shape_of("query", query)
-    dtype, kv_heads, k_shape = query.dtype, 0, None
+    q_shape, dtype, device, q_at, q_token, q_head, sound = _look("query", query)
+    tokens, q_heads, dim = q_shape
+    k_shape, kv_heads, k_at, k_token, k_head = None, 0, 0, 0, 0
     if key is not None:
-        k_tokens, kv_heads, k_dim = k_shape = _shape_of("key", key)
+        k_shape, k_type, k_device, k_at, k_token, k_head, k_sound = _look("key", key)
+        k_tokens, kv_heads, k_dim = k_shape
         if k_tokens != tokens or k_dim != dim:
             raise ValueError(f"key must be a [{tokens}, heads, {dim}] tensor, got {tuple(k_shape)}")
+        sound = sound and k_sound and k_type is dtype and k_device == device
     elif k_out is not None or k_weight is not None:
         raise ValueError("k_out and k_weight need a key")
     if frequencies is not None and positions is None:
         raise ValueError("frequencies need positions")
-    if tokens == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
-        query, key = query.new_empty(q_shape), None if key is None else key.new_empty(k_shape)
-    device = query.get_device()
-    q_in, k_in = _row(query, dtype, q_shape, device), _NONE if key is None else _row(key, dtype, k_shape, device)
-    if device < 0 or dtype not in _HEAD_TYPES or q_in is None or k_in is None:
+    if not sound or device < 0 or dtype not in _HEAD_TYPES:
+        if tokens == 0:  # no rows to be contiguous: an empty tensor's strides may be anything
+            query, key = query.new_empty(q_shape), None if key is None else key.new_empty(k_shape)
         check_tensors(("query", query, _HEAD_TYPES, q_shape), ("key", key, dtype, k_shape), ("q_out", q_out, dtype, q_shape),
                       ("k_out", k_out, dtype, k_shape))
-    turns = _turns(tokens, dim, positions, frequencies, axes, device)
-    weights = _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
+    at, stride, count, turning, axis, pairs = _turns(tokens, dim, positions, frequencies, axes, device)
+    q_weighs, k_weighs, q_step, k_step, w_type = _NO_WEIGHTS if q_weight is None and k_weight is None else \
+        _weights(q_weight, q_heads, k_weight, kv_heads, dim, dtype, device)
     context, handle = ekv_hip.beside(stream, query)
     with context or _HERE:
         # an output made here is contiguous
         if q_out is None:
             q_out = torch.empty(tokens, q_heads, dim, dtype=dtype, device=query.device)
-            q_to = q_out.data_ptr(), q_heads * dim, dim
+            qo_at, qo_token, qo_head = q_out.data_ptr(), q_heads * dim, dim
         else:
-            q_to = _row(q_out, dtype, q_shape, device)
-        if key is None:
-            k_to = _NONE
-        elif k_out is None:
-            k_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=query.device)
-            k_to = k_out.data_ptr(), kv_heads * dim, dim
-        else:
-            k_to = _row(k_out, dtype, k_shape, device)
-        if q_to is None or k_to is None:
-            check_tensors(("query", query, dtype, q_shape), ("q_out", q_out, dtype, q_shape), ("k_out", k_out, dtype, k_shape))
-        q_weighs, k_weighs, q_step, k_step, w_type = weights
-        at, stride, count, turning, axis, pairs = turns
+            qo_at, qo_token, qo_head = _output("q_out", q_out, dtype, q_shape, query)
+        ko_at = ko_token = ko_head = 0
+        if key is not None:
+            if k_out is None:
+                k_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=query.device)
+                ko_at, ko_token, ko_head = k_out.data_ptr(), kv_heads * dim, dim
+            else:
+                ko_at, ko_token, ko_head = _output("k_out", k_out, dtype, k_shape, query)
         arguments = _pack(
-            *q_in, *k_in, *q_to, *k_to, at, stride, turning, axis, q_weighs, k_weighs, q_step, k_step,
-            ekv_hip.dtype_code(dtype), w_type, tokens, q_heads, kv_heads, dim, pairs, count, 1 if adjacent else 0, rotary_scale,
-            eps, weight_offset)
+            q_at, q_token, q_head, k_at, k_token, k_head, qo_at, qo_token, qo_head, ko_at, ko_token, ko_head, at,
+            stride, turning, axis, q_weighs, k_weighs, q_step, k_step, ekv_hip.dtype_code(dtype), w_type, tokens, q_heads,
+            kv_heads, dim, pairs, count, 1 if adjacent else 0, rotary_scale, eps, weight_offset)
         status = (ekv_hip._lib or ekv_hip.load()).ekv_rotate_heads(arguments, handle)
     if status:
         ekv_hip.check(status, "ekv_rotate_heads")

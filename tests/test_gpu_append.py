@@ -72,6 +72,14 @@ def test_many_rows(rows):
     run(Tokens(counts + 2, counts, q_heads=2, kv_heads=1, dim=32, block=4, advance=rows % 2 == 1, behind=4, seed=13))
 
 
+@pytest.mark.parametrize("rows", [1, 3, 1023, 1025, 2051, 5001])
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(2, 1, 32), (20, 4, 256)])
+def test_single_tokens_of_many_rows_advance(rows, q_heads, kv_heads, dim):
+    """Without q_start the counts grow in the launch itself: one, two or four waves a token, one to four tokens a workgroup."""
+    lens = np.random.default_rng(rows).integers(0, 9, size=rows)
+    run(Tokens(lens, None, q_heads=q_heads, kv_heads=kv_heads, dim=dim, block=4, advance=True, evicting=True, seed=29))
+
+
 def test_one_long_row():
     run(Tokens([3000], [2900], q_heads=4, kv_heads=2, dim=64, evicting=True, seed=14))
 
