@@ -74,6 +74,8 @@ struct Params {
   int bs_shift;
   bool adjacent, advance, saturate, weight_f32;
   int parts;                // waves of a token: 1, 2 or 4
+  int crowd;                // tokens of a wave of crowd_kernel
+  PageDivisor by_q_heads, by_kv_heads, by_pairs;
   int lanes_log;            // of a head: 2, 4, 8 or 16 lanes
   int q_passes, kv_passes;  // of 64 / lanes heads, that the queries and that the keys (and the values) of a token take
   float rotary_scale, eps, weight_offset, k_inverse, v_inverse, mean;  // mean: 1 / dim
@@ -204,6 +206,143 @@ __device__ __forceinline__ float head_sum(float v, int lanes) {
   return v;
 }
 
+// i / divisor, 0 <= i < 2^31
+__device__ __forceinline__ int quotient(int i, const PageDivisor &d) { return (int)(__umulhi((uint32_t)i << 1, d.mul) >> d.shift); }
+
+// -- the arithmetic of a head ---------------------------------------------------------------------
+//
+// Which products are fused with which sums is written out, so that a head's result is the same bits in every kernel.
+
+// 1 / the root mean square of the head whose elements the lanes hold, two units each (a lane that is not `mine` holds none).
+// All lanes of the wave are active.
+__device__ __forceinline__ float over_rms(const Params &p, const float (&x)[kUnit], const float (&y)[kUnit], bool mine, int lanes) {
+  float squares = 0.f;
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) squares = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], squares));
+  squares = head_sum(mine ? squares : 0.f, lanes);
+  float over = rsqrtf(__builtin_fmaf(squares, p.mean, p.eps));
+  if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
+    float small = 0.f;
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) {
+      const float u = x[e] * 0x1p-80f, v = y[e] * 0x1p-80f;
+      small = __builtin_fmaf(u, u, __builtin_fmaf(v, v, small));
+    }
+    small = head_sum(mine ? small : 0.f, lanes);
+    if (squares == __builtin_inff()) over = rsqrtf(small * p.mean) * 0x1p-80f;
+  }
+  return over;
+}
+
+// The weights of one head's own, of queries or keys (1 without): elements [a, a + 8) and [b, b + 8).
+template <class T>
+__device__ __forceinline__ void own_weights(const Params &p, int kind, int head, int a, int b, float (&wa)[kUnit],
+                                            float (&wb)[kUnit]) {
+  const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) wa[e] = wb[e] = 1.f;
+  if (weight == nullptr) return;
+  const char *row = weight + head * (kind == kQuery ? p.q_weight_stride : p.k_weight_stride);
+  if (p.weight_f32) {
+    load_weights<float>(row + a * 4, wa);
+    load_weights<float>(row + b * 4, wb);
+  } else {
+    load_weights<T>(row + a * sizeof(T), wa);
+    load_weights<T>(row + b * sizeof(T), wb);
+  }
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) {
+    wa[e] += p.weight_offset;
+    wb[e] += p.weight_offset;
+  }
+}
+
+// Weights that every head shares, of queries and of keys: asked for as they lie in memory (converting one at once would wait
+// for it at once), then kept in LDS (1 without).
+template <class T>
+struct SharedWeights {
+  static constexpr int kHeld = 2 * kMostPairs / kWave;  // of a lane, for each kind
+  uint32_t raw[2][kHeld];
+  __device__ __forceinline__ void load(const Params &p) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = k * kWave + lane_id();
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
+        raw[kind][k] = 0;
+        if (weight != nullptr && i < p.dim)
+          raw[kind][k] = p.weight_f32 ? as_global((const uint32_t *)weight)[i] : as_global((const uint16_t *)weight)[i];
+      }
+    }
+  }
+  __device__ __forceinline__ void keep(const Params &p, float (&to)[2][2 * kMostPairs]) const {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const uint32_t w = raw[kind][k];
+        const float x = p.weight_f32 || sizeof(T) == 4 ? __builtin_bit_cast(float, w)
+                        : std::is_same<T, __bf16>::value ? __builtin_bit_cast(float, w << 16)
+                                                         : (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+        const bool weighs = (kind == kQuery ? p.q_weight : p.k_weight) != nullptr;
+        to[kind][k * kWave + lane_id()] = weighs ? p.weight_offset + x : 1.f;
+      }
+    }
+  }
+};
+
+// The cosine and sine, times the rotary scale, of a position times a frequency.
+__device__ __forceinline__ void turn_of(const Params &p, double pos, double frequency, float &cosine, float &sine) {
+  const double angle = pos * frequency, whole = __builtin_rint(angle * 0.15915494309189533577);  // 1 / 2 pi
+  const float x = (float)__builtin_fma(angle, 0.15915494309189533577, -whole);
+  float s, c;
+  sincospif(2.f * x, &s, &c);
+  cosine = c * p.rotary_scale;
+  sine = s * p.rotary_scale;
+}
+
+// The lane's 8 pairs turned: x[e] with y[e], or adjacent elements of x and then of y.
+template <bool ADJACENT>
+__device__ __forceinline__ void rotate(float (&x)[kUnit], float (&y)[kUnit], const float (&cosine)[kUnit],
+                                       const float (&sine)[kUnit]) {
+  auto turn = [&](float &u, float &v, float c, float s) {
+    const float was = u;
+    u = __builtin_fmaf(was, c, -(v * s));
+    v = __builtin_fmaf(was, s, v * c);
+  };
+#pragma unroll
+  for (int e = 0; e < kUnit; ++e) {
+    if constexpr (!ADJACENT) turn(x[e], y[e], cosine[e], sine[e]);
+    else if (e < 4) turn(x[2 * e], x[2 * e + 1], cosine[e], sine[e]);
+    else turn(y[2 * e - 8], y[2 * e - 7], cosine[e], sine[e]);
+  }
+}
+
+// What a lane holds of a head.
+struct Share {
+  bool active;  // an idle lane reads what the first lane of its head does, and writes nothing
+  bool turns;   // its elements are rotated
+  int nth;      // the head of the pass
+  int a, b;     // its elements: [a, a + 8) and [b, b + 8)
+  int low, high;  // the pairs of its cosines: [low, low + 4) and [high, high + 4)
+};
+template <bool ADJACENT>
+__device__ __forceinline__ Share share_of(const Params &p) {
+  const int lane = lane_id(), lanes = 1 << p.lanes_log, turning = p.pairs / kUnit, rest = p.dim - 2 * p.pairs;
+  Share s;
+  s.nth = lane >> p.lanes_log;
+  s.active = (lane & (lanes - 1)) * 2 * kUnit < p.dim;
+  const int unit = s.active ? lane & (lanes - 1) : 0;
+  s.turns = unit < turning;
+  s.a = s.turns ? unit * kUnit : 2 * p.pairs + (unit - turning) * kUnit;
+  s.b = s.turns ? p.pairs + s.a : s.a + rest / 2;
+  // adjacent: [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
+  s.low = !s.turns ? 0 : ADJACENT ? s.a / 2 : s.a;
+  s.high = !s.turns ? 0 : ADJACENT ? s.b / 2 : s.a + 4;
+  return s;
+}
+
 // -- where a token belongs ------------------------------------------------------------------------
 
 struct Place {
@@ -312,14 +451,10 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
   const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
   const int token = (int)(item / p.parts), part = (int)(item % p.parts);
 
-  const int nth = lane >> p.lanes_log, turning = p.pairs / kUnit, rest = p.dim - 2 * p.pairs;
-  const bool active = (lane & (lanes - 1)) * 2 * kUnit < p.dim;
-  const int unit = active ? lane & (lanes - 1) : 0;  // an idle lane reads what lane 0 of its head does, and writes nothing
-  const bool turns = unit < turning;
-  // the lane's elements: [a, a + 8) and [b, b + 8)
-  const int a = turns ? unit * kUnit : 2 * p.pairs + (unit - turning) * kUnit;
-  const int b = turns ? p.pairs + a : a + rest / 2;
-  const bool paired = turning % 2 == 0 && p.dim % 32 == 0;  // fp8 caches: store_e4m3
+  const Share share = share_of<ADJACENT>(p);
+  const bool active = share.active, turns = share.turns;
+  const int nth = share.nth, a = share.a, b = share.b;
+  const bool paired = p.pairs / kUnit % 2 == 0 && p.dim % 32 == 0;  // fp8 caches: store_e4m3
 
   // The passes of the queries, then the keys, then the values; the wave takes every parts-th.  A pass has heads of one
   // kind, so that what depends on the kind is scalar.
@@ -351,35 +486,13 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
       frequency[k] = i < p.pairs ? p.frequencies[i] : 0.0;
       axis[k] = p.axes != nullptr && i < p.pairs ? p.axes[i] : 0;
     }
-    constexpr int kWeights = NORM == kShared ? 2 * kMostPairs / kWave : 0;  // of a lane, for each of queries and keys
-    uint32_t weights[2][kWeights + 1];  // as they lie in memory: converting one here would wait for it here
-#pragma unroll
-    for (int k = 0; k < kWeights; ++k) {
-      const int i = k * kWave + lane;
-#pragma unroll
-      for (int kind = 0; kind < 2; ++kind) {
-        const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
-        weights[kind][k] = 0;
-        if (weight != nullptr && i < p.dim)
-          weights[kind][k] = p.weight_f32 ? as_global((const uint32_t *)weight)[i] : as_global((const uint16_t *)weight)[i];
-      }
-    }
+    SharedWeights<T> weights;
+    if constexpr (NORM == kShared) weights.load(p);
     if (part < passes) fetch(part);
 
     Place at{true, 0, 0, 0, false, -1};
     if constexpr (PAGED) at = place_of(p, token, search);
-#pragma unroll
-    for (int k = 0; k < kWeights; ++k) {
-#pragma unroll
-      for (int kind = 0; kind < 2; ++kind) {
-        const uint32_t w = weights[kind][k];
-        const float x = p.weight_f32 || sizeof(T) == 4 ? __builtin_bit_cast(float, w)
-                        : std::is_same<T, __bf16>::value ? __builtin_bit_cast(float, w << 16)
-                                                         : (float)__builtin_bit_cast(_Float16, (uint16_t)w);
-        const bool weighs = (kind == kQuery ? p.q_weight : p.k_weight) != nullptr;
-        s_weight[wave][kind][k * kWave + lane] = weighs ? p.weight_offset + x : 1.f;
-      }
-    }
+    if constexpr (NORM == kShared) weights.keep(p, s_weight[wave]);
 
     // the token's cosines and sines
     float cosine[kUnit], sine[kUnit];
@@ -399,24 +512,17 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
           }
           pos = (double)mine;
         }
-        const double turn = pos * frequency[k] * 0.15915494309189533577;  // 1 / 2 pi
-        const float x = (float)(turn - __builtin_rint(turn));
-        float s, c;
-        sincospif(2.f * x, &s, &c);
-        s_cos[wave][i] = c * p.rotary_scale;
-        s_sin[wave][i] = s * p.rotary_scale;
+        turn_of(p, pos, frequency[k], s_cos[wave][i], s_sin[wave][i]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    // adjacent: [a, a + 8) are pairs a / 2 .. a / 2 + 3, [b, b + 8) those from b / 2 on
-    const int low = !turns ? 0 : ADJACENT ? a / 2 : a, high = !turns ? 0 : ADJACENT ? b / 2 : a + 4;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      cosine[e] = s_cos[wave][low + e];
-      sine[e] = s_sin[wave][low + e];
-      cosine[4 + e] = s_cos[wave][high + e];
-      sine[4 + e] = s_sin[wave][high + e];
+      cosine[e] = s_cos[wave][share.low + e];
+      sine[e] = s_sin[wave][share.low + e];
+      cosine[4 + e] = s_cos[wave][share.high + e];
+      sine[4 + e] = s_sin[wave][share.high + e];
     }
 
     int64_t in_page = 0;
@@ -451,23 +557,7 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
       widen(va, x);
       widen(vb, y);
       if (NORM != kNone && (!PAGED || kind != kValue)) {
-        const char *const weight = kind == kQuery ? p.q_weight : p.k_weight;
-        float squares = 0.f;
-#pragma unroll
-        for (int e = 0; e < kUnit; ++e) squares += x[e] * x[e] + y[e] * y[e];
-        squares = head_sum(mine ? squares : 0.f, lanes);
-        float over = rsqrtf(squares * p.mean + p.eps);
-        if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
-          float small = 0.f;
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e) {
-            const float u = x[e] * 0x1p-80f, v = y[e] * 0x1p-80f;
-            small += u * u + v * v;
-          }
-          small = head_sum(mine ? small : 0.f, lanes);
-          if (squares == __builtin_inff()) over = rsqrtf(small * p.mean) * 0x1p-80f;
-        }
-        if (weight == nullptr) over = 1.f;  // the other one's heads are normed, not these
+        const float over = (kind == kQuery ? p.q_weight : p.k_weight) == nullptr ? 1.f : over_rms(p, x, y, mine, lanes);
         float wa[kUnit], wb[kUnit];
         if constexpr (NORM == kShared) {
 #pragma unroll
@@ -476,23 +566,7 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
             wb[e] = s_weight[wave][kind][b + e];
           }
         } else {
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e) wa[e] = wb[e] = 1.f;
-          if (weight != nullptr) {
-            const char *row = weight + min(head, heads - 1) * (kind == kQuery ? p.q_weight_stride : p.k_weight_stride);
-            if (p.weight_f32) {
-              load_weights<float>(row + a * 4, wa);
-              load_weights<float>(row + b * 4, wb);
-            } else {
-              load_weights<T>(row + a * sizeof(T), wa);
-              load_weights<T>(row + b * sizeof(T), wb);
-            }
-#pragma unroll
-            for (int e = 0; e < kUnit; ++e) {
-              wa[e] += p.weight_offset;
-              wb[e] += p.weight_offset;
-            }
-          }
+          own_weights<T>(p, kind, min(head, heads - 1), a, b, wa, wb);
         }
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) {
@@ -500,25 +574,7 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
           y[e] *= over * wb[e];
         }
       }
-      if (turns && (!PAGED || kind != kValue)) {
-        if constexpr (ADJACENT) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u = x[2 * e], v = x[2 * e + 1], r = y[2 * e], s = y[2 * e + 1];
-            x[2 * e] = u * cosine[e] - v * sine[e];
-            x[2 * e + 1] = u * sine[e] + v * cosine[e];
-            y[2 * e] = r * cosine[4 + e] - s * sine[4 + e];
-            y[2 * e + 1] = r * sine[4 + e] + s * cosine[4 + e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e) {
-            const float u = x[e], v = y[e];
-            x[e] = u * cosine[e] - v * sine[e];
-            y[e] = u * sine[e] + v * cosine[e];
-          }
-        }
-      }
+      if (turns && (!PAGED || kind != kValue)) rotate<ADJACENT>(x, y, cosine, sine);
       if (!PAGED || kind == kQuery) {
         if (mine) {
           const Heads &out = p.out[kind];
@@ -554,6 +610,97 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
   }
 }
 
+// Heads without a cache, several tokens a wave: where a token's heads leave most of a pass idle, a pass takes the heads of one
+// kind of `crowd` tokens in a row.  Their angles are spread over all lanes, and each lane reads its token's for each pass.
+template <class T, Norm NORM, bool ADJACENT, Past PAST>
+__global__ __launch_bounds__(kWaves *kWave) void crowd_kernel(Params p) {
+  constexpr int kMostTurns = kWave * kUnit;  // of the wave's tokens: no more than a pass has heads, 8 pairs a lane
+  __shared__ __align__(16) float s_cos[kWaves][kMostTurns], s_sin[kWaves][kMostTurns];
+  __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2][2 * kMostPairs];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int lanes = 1 << p.lanes_log, per = kWave >> p.lanes_log;  // of a head; heads of a pass
+  const int64_t first = ((int64_t)blockIdx.x * kWaves + wave) * p.crowd;
+  if (first >= p.tokens) return;
+  const int n = (int)min((int64_t)p.crowd, p.tokens - first);
+  const Share share = share_of<ADJACENT>(p);
+  const int a = share.a, b = share.b;
+  const int q_passes = (n * p.q_heads + per - 1) / per, passes = q_passes + (n * p.kv_heads + per - 1) / per;
+  struct Item {
+    int t, head;  // of the wave's tokens, of its heads of the kind
+    bool there;
+  };
+  auto item_of = [&](int pass, int kind) {
+    const int heads = kind == kQuery ? p.q_heads : p.kv_heads;
+    const int i = (pass - (kind == kQuery ? 0 : q_passes)) * per + share.nth, last = n * heads - 1;
+    const int within = min(i, last), t = quotient(within, kind == kQuery ? p.by_q_heads : p.by_kv_heads);
+    return Item{t, within - t * heads, i <= last};
+  };
+  Unit<T> ua, ub;
+  auto fetch = [&](int pass) {
+    const int kind = pass < q_passes ? kQuery : kKey;
+    const Item item = item_of(pass, kind);
+    const char *x = p.in[kind].at + (first + item.t) * p.in[kind].token + item.head * p.in[kind].head;
+    ua = load_unit<T, PAST != kNothing>(x + a * sizeof(T));
+    ub = load_unit<T, PAST != kNothing>(x + b * sizeof(T));
+  };
+  SharedWeights<T> weights;
+  if constexpr (NORM == kShared) weights.load(p);
+  fetch(0);
+  if constexpr (NORM == kShared) weights.keep(p, s_weight[wave]);
+  for (int i = lane; i < n * p.pairs; i += kWave) {
+    const int t = quotient(i, p.by_pairs), pair = i - t * p.pairs, axis = p.axes != nullptr ? p.axes[pair] : 0;
+    double pos = 0.0;
+    if ((uint32_t)axis < (uint32_t)p.axis_count) pos = (double)p.positions[axis * p.positions_stride + first + t];
+    turn_of(p, pos, p.frequencies[pair], s_cos[wave][i], s_sin[wave][i]);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int pass = 0; pass < passes; ++pass) {
+    const int kind = pass < q_passes ? kQuery : kKey;
+    const Item item = item_of(pass, kind);
+    const bool mine = share.active && item.there;
+    float x[kUnit], y[kUnit];
+    widen(ua, x);
+    widen(ub, y);
+    if (pass + 1 < passes) fetch(pass + 1);
+    if constexpr (NORM != kNone) {
+      const float over = (kind == kQuery ? p.q_weight : p.k_weight) == nullptr ? 1.f : over_rms(p, x, y, mine, lanes);
+      float wa[kUnit], wb[kUnit];
+      if constexpr (NORM == kShared) {
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) {
+          wa[e] = s_weight[wave][kind][a + e];
+          wb[e] = s_weight[wave][kind][b + e];
+        }
+      } else {
+        own_weights<T>(p, kind, item.head, a, b, wa, wb);
+      }
+#pragma unroll
+      for (int e = 0; e < kUnit; ++e) {
+        x[e] *= over * wa[e];
+        y[e] *= over * wb[e];
+      }
+    }
+    if (share.turns) {
+      float cosine[kUnit], sine[kUnit];
+      const int at = item.t * p.pairs;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        cosine[e] = s_cos[wave][at + share.low + e];
+        sine[e] = s_sin[wave][at + share.low + e];
+        cosine[4 + e] = s_cos[wave][at + share.high + e];
+        sine[4 + e] = s_sin[wave][at + share.high + e];
+      }
+      rotate<ADJACENT>(x, y, cosine, sine);
+    }
+    if (mine) {
+      char *to = (char *)p.out[kind].at + (first + item.t) * p.out[kind].token + item.head * p.out[kind].head;
+      store_unit<T, PAST == kAll>(to + a * sizeof(T), narrow<T>(x));
+      store_unit<T, PAST == kAll>(to + b * sizeof(T), narrow<T>(y));
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void advance_kernel(Params p) {
   const int row = blockIdx.x * 256 + threadIdx.x;
   if (row >= p.rows) return;
@@ -569,6 +716,14 @@ constexpr int64_t kMostWaves = (1ll << 26) - 64;  // a launch has fewer than 2^3
 
 template <class T, class C, bool PAGED, Norm NORM, Past PAST>
 int launch_pairs(const Params &p, hipStream_t stream, const char *who) {
+  if constexpr (!PAGED) {
+    if (p.crowd > 1) {
+      const dim3 grid((unsigned)ceil_div(ceil_div(p.tokens, p.crowd), kWaves)), block(kWaves * kWave);
+      if (p.adjacent) hipLaunchKernelGGL((crowd_kernel<T, NORM, true, PAST>), grid, block, 0, stream, p);
+      else hipLaunchKernelGGL((crowd_kernel<T, NORM, false, PAST>), grid, block, 0, stream, p);
+      return check_hip(hipGetLastError(), who);
+    }
+  }
   const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.parts, kWaves)), block(kWaves * kWave);
   if (p.adjacent) hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, true, PAST>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((heads_kernel<T, C, PAGED, NORM, false, PAST>), grid, block, 0, stream, p);
@@ -601,6 +756,17 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   p.parts = few || (past == kAll && NORM == kNone && passes > 5) ? 4 : passes >= 5 ? 2 : 1;
   while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
   while (p.parts > 1 && (int64_t)p.tokens * p.parts >= kMostWaves) p.parts /= 2;
+  // Eight tokens a wave (four of the widest heads), where passes of one token would be more than five eighths idle and the
+  // waves stay four a compute unit: 32768 tokens of one query and one KV head of 96, normed, 14 us against 27 one by one, of
+  // 4 and 1 of 128 20 / 29, of 16 and 4 of 32 19 / 28; of 4 and 4 of 128, half idle, 31 / 24 without norms.
+  p.crowd = 1;
+  const int heads_of_pass = kWave >> p.lanes_log, crowd = heads_of_pass < 8 ? heads_of_pass : 8;
+  if (!PAGED && (p.q_heads + p.kv_heads) * 8ll <= 3ll * passes * heads_of_pass && p.tokens >= crowd * 4 * cu_count()) {
+    p.crowd = crowd;
+    if (p.q_heads > 0) p.by_q_heads = page_divisor(p.q_heads);
+    if (p.kv_heads > 0) p.by_kv_heads = page_divisor(p.kv_heads);
+    if (p.pairs > 0) p.by_pairs = page_divisor(p.pairs);
+  }
   if constexpr (sizeof(T) == 2)
     if (past == kAll) return launch_pairs<T, C, PAGED, NORM, kAll>(p, stream, who);
   return past == kLoads ? launch_pairs<T, C, PAGED, NORM, kLoads>(p, stream, who)

@@ -207,6 +207,31 @@ def test_sizes_around_the_caches(pairs, dim, dtype, tokens):
             assert torch.equal(query[part], want[0]) and torch.equal(key[part], want[1])
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim,pairs", [(1, 1, 96, 48), (3, 1, 128, 32), (2, 1, 64, 32), (1, 1, 256, 128), (5, 2, 32, 16),
+                                                        (1, 0, 80, 40), (4, 1, 128, 0), (1, 1, 16, 8), (3, 1, 240, 120)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("norm", [None, "shared", "heads"])
+def test_few_heads_of_many_tokens(q_heads, kv_heads, dim, pairs, dtype, norm):
+    """Where a token's heads are few a wave takes several tokens: the same bits as small calls, which take them one by one."""
+    tokens = 8 * 1024 + 13
+    for axes, adjacent in ((0, False), (3, True)):
+        args, check = case(tokens, q_heads, kv_heads, dim, pairs, dtype, 9, axes=axes if pairs else 0, adjacent=adjacent, norm=norm)
+        query, key = rotate_heads(**args)
+        for a in range(0, tokens, 2000):
+            part = slice(a, a + 2000)
+            where = {} if not pairs else {"positions": args["positions"][..., part].contiguous()}
+            want = rotate_heads(**{**args, **where, "query": args["query"][part], "key": None if key is None else args["key"][part]})
+            assert torch.equal(query[part], want[0]) and (key is None or torch.equal(key[part], want[1]))
+        got = rotate_heads(**args, q_out=args["query"], k_out=args["key"])
+        assert torch.equal(got[0], query) and (key is None or torch.equal(got[1], key))
+
+
+@pytest.mark.parametrize("dtype,norm", [(F32, "heads"), (F16, "shared"), (BF16, None)])
+def test_few_heads_against_the_definition(dtype, norm):
+    args, check = case(8 * 1024 + 3, 1, 1, 32, 16, dtype, 10, axes=2, norm=norm)
+    check(*rotate_heads(**args))
+
+
 def test_axes_of_one_row_of_positions():
     """Positions that are one row seen as three."""
     n = torch.arange(50, dtype=torch.int32, device="cuda")
