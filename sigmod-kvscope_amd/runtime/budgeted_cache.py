@@ -111,10 +111,10 @@ class BudgetedCache:
         if self.prefix_table is None or n > self.prefix_table.shape[1] * self.block:
             raise ValueError(f"no room for a prefix of {n} tokens")
         if self.rotation is not None:
-            self.prefix_len.fill_(n)
             start = torch.arange(2, dtype=torch.int32, device=self.kv.device) * n
-            append_tokens(self.kv, self.prefix_table, self.prefix_len, keys, values, q_start=start, max_query=max(1, n),
+            append_tokens(self.kv, self.prefix_table, start[1:], keys, values, q_start=start, max_query=max(1, n),
                           positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(None))
+            self.prefix_len.fill_(n)
             return
         if positions is not None:
             raise ValueError("positions need a rotation")

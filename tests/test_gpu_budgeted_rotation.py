@@ -185,3 +185,11 @@ def test_refusals():
     with pytest.raises(ValueError, match="device tensor"):
         cache.append(rows.bfloat16(), rows.bfloat16())
     assert cache.longest == 0
+
+
+def test_a_refused_prefix_leaves_none():
+    cache = BudgetedCache(2, HEADS, 32, budget=4, prefix=3, rotation=dict(frequencies=rotary_frequencies(16, device="cpu")), device="cpu")
+    rows = torch.zeros(3, HEADS, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="device tensor"):
+        cache.set_prefix(rows, rows)
+    assert cache.prefix_len.item() == 0
