@@ -665,6 +665,7 @@ typedef struct ekv_append {
  * table, and one whose table entry is no page of the cache, is not written (of the latter, scores and
  * slot_positions are).  A row keeps its first max_query tokens.  With advance, lens[r] then grows by the
  * tokens kept, but not past width * block_size, and seen[r] by as many as there were within max_query.
+ * lens, seen and first then share no memory.
  * Tokens of no row (before the first, behind the last, past max_query) write nothing and get q_out 0.
  * Types: new tokens and queries fp32, f16 or bf16; the cache the same, or fp8 e4m3; limits as
  * ekv_rotate_heads has them, and width * block_size below 2^31 - 4096.

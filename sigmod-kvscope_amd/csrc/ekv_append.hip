@@ -838,6 +838,11 @@ int fill(const Block *a, Params &p, const char *who) {
 bool row_aligned(const Heads &h) { return aligned16(h.at) && h.token % 16 == 0 && h.head % 16 == 0; }
 bool weight_aligned(const char *at, int64_t stride) { return aligned16(at) && stride % 16 == 0; }
 
+// Whether m counts from a and n from b have one in common.
+bool share(const int32_t *a, int64_t m, const int32_t *b, int64_t n) {
+  return a != nullptr && b != nullptr && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)(a + m);
+}
+
 }  // namespace append
 }  // namespace ekv
 
@@ -926,6 +931,8 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   p.v_inverse = (float)(1.0 / a->v_scale);
   if (p.tokens == 0) return EKV_OK;
   if (p.rows == 0) return fail(EKV_EINVAL, "%s: %d tokens of no row", who, p.tokens);
+  if (p.first != nullptr && p.first_stride < 0)
+    return fail(EKV_EINVAL, "%s: first of stride %lld", who, (long long)p.first_stride);
   if (p.in[kKey].at == nullptr || p.in[kValue].at == nullptr || p.lens == nullptr ||
       (p.q_heads > 0 && (p.in[kQuery].at == nullptr || p.out[kQuery].at == nullptr)) ||
       (p.width > 0 && (p.keys == nullptr || p.values == nullptr || p.table == nullptr)))
@@ -939,6 +946,11 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
   if (p.table_stride < p.width)
     return fail(EKV_EINVAL, "%s: table rows of %d blocks, stride %lld", who, p.width, (long long)p.table_stride);
   if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
+  if (p.advance) {  // a row's counts grow while other rows' are read, and each of them once
+    const int64_t n = p.rows, reach = p.first == nullptr ? 0 : 1 + (n - 1) * p.first_stride;
+    if (append::share(p.lens, n, p.seen, n) || append::share(p.first, reach, p.lens, n) || append::share(p.first, reach, p.seen, n))
+      return fail(EKV_EINVAL, "%s: lens, seen and first share memory", who);
+  }
   hipStream_t s = (hipStream_t)stream;
   const bool fp8 = a->kv_dtype == EKV_FP8_E4M3;
   int status;

@@ -309,3 +309,16 @@ def test_sections():
     for bad in ((0, 10.0), (4, 0.0)):
         with pytest.raises(ValueError, match="pairs"):
             rotary_frequencies(*bad, device="cpu")
+
+
+@pytest.mark.parametrize("over", [dict(seen=P), dict(seen=P + 8), dict(first=P + 4), dict(first=P - 16, first_stride=2), dict(seen=2 * P, first=2 * P)])
+def test_counts_that_share_memory_do_not_advance(over):
+    """lens and seen both grow by a row's tokens, while other rows' tokens may still read `first`."""
+    a = appending(lens=P, advance=1, **over)
+    with pytest.raises(ValueError, match="memory"):
+        ekv_hip.call("ekv_append_tokens", ctypes.addressof(a), 0)
+
+
+def test_first_of_a_negative_stride():
+    with pytest.raises(ValueError, match="stride"):
+        ekv_hip.call("ekv_append_tokens", ctypes.addressof(a := appending(first=2 * P, first_stride=-1)), 0)
