@@ -8,7 +8,7 @@
 //
 // Bound.  Every input is read once and every output written once, 3 or 4 flop an element: bandwidth, or a launch's
 // latency where the tokens are few.  Measured (32 query and 8 KV heads of 128, bf16): 38241 tokens of prompts, 940 MB, 155 us
-// (6.1 TB/s; a bare copy of the same pattern 155), the norms of 16384 tokens, 335 MB, 58 us (5.8 TB/s), 128 tokens of a
+// (6.1 TB/s; a bare copy of the same pattern 155), the norms of 16384 tokens, 335 MB, 57 us (5.9 TB/s), 128 tokens of a
 // decode step 4.1 us.
 //
 // Layout.  A head's pairs are cut into units of 8, a unit a lane: the 8 elements of the first halves and the 8 of the
@@ -757,8 +757,8 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
   while (p.parts > 1 && (int64_t)p.tokens * p.parts >= kMostWaves) p.parts /= 2;
   // Eight tokens a wave (four of the widest heads), where passes of one token would be more than five eighths idle and the
-  // waves stay four a compute unit: 32768 tokens of one query and one KV head of 96, normed, 14 us against 27 one by one, of
-  // 4 and 1 of 128 20 / 29, of 16 and 4 of 32 19 / 28; of 4 and 4 of 128, half idle, 31 / 24 without norms.
+  // waves stay four a compute unit: 32768 tokens of one query and one KV head of 96, normed, 13 us against 27 one by one, of
+  // 4 and 1 of 128 20 / 29, of 16 and 4 of 32 18 / 28; of 4 and 4 of 128, half idle, 31 / 24 without norms.
   p.crowd = 1;
   const int heads_of_pass = kWave >> p.lanes_log, crowd = heads_of_pass < 8 ? heads_of_pass : 8;
   if (!PAGED && (p.q_heads + p.kv_heads) * 8ll <= 3ll * passes * heads_of_pass && p.tokens >= crowd * 4 * cu_count()) {
