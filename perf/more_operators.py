@@ -246,12 +246,10 @@ def run(state):
     return _rotate_own(state) if own else _rotate_plain(state)
 
 
-_PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sigmod-kvscope_amd")
-
-
 def _package():
-    if _PACKAGE not in sys.path:  # a user's program finds the package once
-        sys.path.insert(0, _PACKAGE)
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sigmod-kvscope_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
 
 
 def _rotate_own(s):
