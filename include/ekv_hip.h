@@ -508,6 +508,7 @@ typedef struct ekv_attention {
   int32_t rows, width, prefix_groups, prefix_width, tokens, max_query;
   int32_t q_heads, kv_heads, head_dim, block_size;
   float scale, k_scale, v_scale, decay;
+  int32_t kept;                 /* lens count no more than so many of a row's query tokens (0: all of them) */
 } ekv_attention_t;
 
 /*
@@ -515,7 +516,9 @@ typedef struct ekv_attention {
  * the reference, which leaves attention to the serving engine.
  *
  * Query token i (of t) of row r sees every token of its group's prefix and the row's own slots
- * j <= lens[r] - t + i.  With s = scale * k_scale * <q, k>, head hq reading KV head hq / (q_heads / kv_heads):
+ * j <= lens[r] - t + i; with `kept`, j <= lens[r] - min(t, kept) + i, as ekv_append_tokens leaves the
+ * lengths with advance, `kept` being its max_query.
+ * With s = scale * k_scale * <q, k>, head hq reading KV head hq / (q_heads / kv_heads):
  *     lse = log sum exp(s)        out = v_scale * sum exp(s - lse) v
  * and a query that sees nothing has out 0 and lse -inf.  A table entry that is no page of the cache
  * (negative, or blocks and more) is as if its tokens were not there.  What the cache holds in slots that
@@ -665,7 +668,9 @@ typedef struct ekv_append {
  * table, and one whose table entry is no page of the cache, is not written (of the latter, scores and
  * slot_positions are).  A row keeps its first max_query tokens.  With advance, lens[r] then grows by the
  * tokens kept, but not past width * block_size, and seen[r] by as many as there were within max_query.
- * lens, seen and first then share no memory.
+ * lens, seen and first then share no memory.  Attention of the same q_start takes lengths grown so with
+ * max_query as its `kept`.  (Of a row that passes its table it would take the kept tokens for the last ones
+ * that the table has.)
  * Tokens of no row (before the first, behind the last, past max_query) write nothing and get q_out 0.
  * Types: new tokens and queries fp32, f16 or bf16; the cache the same, or fp8 e4m3; limits as
  * ekv_rotate_heads has them, and width * block_size below 2^31 - 4096.

@@ -266,7 +266,7 @@ __global__ __launch_bounds__((Narrow<T, D>::kThreads), (D == 256 ? 1 : 2)) void 
       s.table = p.table + (int64_t)s.row * p.table_stride;
       s.first = uniform(t.first);
       s.rows = uniform(min(t.count, p.max_query) * p.group);
-      s.see = uniform(len - t.count + 1);
+      s.see = uniform(own_see(p, len, t));
       s.slot = j - j0;
       const int u0 = (int)(at - row_at), u1 = (int)(min(stop, row_at + units) - row_at);
       s.begin = u0 * N::kKeys;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(W == 1 ? kThreads : W *kWave) void combine_kernel(c
   int own = 0, pre = 0;  // slots written for this query
   if (i_q >= 0 && i_q < min(t.count, p.max_query)) {
     const int len = row_length(p, row);
-    const int seen = min(len, len - t.count + 1 + i_q);
+    const int seen = min(len, own_see(p, len, t) + i_q);
     const int g = group_of(p, row);
     const int n = g >= 0 ? group_length(p, g) : 0;
     if (p.wide_own) {
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(THREADS) void fold_kernel(const Params p, int piece
   const int len = row_length(p, row);
   if (key >= len) return;
   const RowQueries t = row_queries(p, row);
-  const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
+  const int see = own_see(p, len, t), rows = min(t.count, p.max_query) * p.group;
   const float *logits = p.logits + ((int64_t)row * p.kv_heads + head) * p.logit_rows * p.logit_stride + key;
   float total[4] = {0.f, 0.f, 0.f, 0.f};
   for (int m = 0; m < rows; ++m) {
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void weigh_kernel(const Params p, int pie
   if (begin >= end) return;
   const int32_t *table = p.table + (int64_t)row * p.table_stride;
   const RowQueries t = row_queries(p, row);
-  const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
+  const int see = own_see(p, len, t), rows = min(t.count, p.max_query) * p.group;
   const int lane = lane_id(), g = lane / 16, n = lane % 16;
   const int mine = min(begin + lane, end - 1);
   const int page_mine = table[page_of(p, mine)];
@@ -714,6 +714,7 @@ int fill(const ekv_attention_t *a, Params &p) {
   if (a->q_start == nullptr && (a->tokens != a->rows || a->max_query != 1))
     return fail(EKV_EINVAL, "%s: %d tokens, at most %d a row, of %d rows need q_start", who, a->tokens, a->max_query,
                 a->rows);
+  if (a->kept < 0) return fail(EKV_EINVAL, "%s: %d kept tokens a row", who, a->kept);
   if ((int64_t)a->width * a->block_size >= kMostKeys || (int64_t)a->prefix_width * a->block_size >= kMostKeys)
     return fail(EKV_EINVAL, "%s: a table of %d or %d blocks of %d tokens passes 2^31 - 4096", who, a->width, a->prefix_width,
                 a->block_size);
@@ -762,6 +763,7 @@ int fill(const ekv_attention_t *a, Params &p) {
   p.scale2 = a->scale * a->k_scale * kLog2e;
   p.v_scale = a->v_scale;
   p.decay = a->decay;
+  p.kept = a->kept > 0 ? a->kept : INT32_MAX;
   plan(p, a->head_dim, a->kv_dtype);
   // a launch has fewer than 2^32 threads: 64 a wave or item of the narrow kernel and of the weights read again, 256 an
   // item of the wide one

@@ -76,6 +76,7 @@ struct Params {
   // its group.  wide_own alone: a row's tiles walk its prefix ahead of the own keys, on one axis.  direct: one chunk
   // holds everything a query sees, so the wide kernel writes the result.
   bool wide_own, wide_pre, direct;
+  int kept;    // lens count no more than so many of a row's query tokens
   bool whole;  // 16 slots from a multiple of 16 on lie in one page, at offsets below 2^31
 };
 
@@ -351,6 +352,10 @@ __device__ __forceinline__ RowQueries row_queries(const Params &p, int row) {
 }
 __device__ __forceinline__ int row_length(const Params &p, int row) {
   return min(max(p.lens[row], 0), p.width * p.block_size);  // the host keeps width * block_size below 2^31
+}
+// A row's query token i sees own slots below own_see + i.
+__device__ __forceinline__ int own_see(const Params &p, int len, const RowQueries &t) {
+  return len - min(t.count, p.kept) + 1;
 }
 // The token ranges and lengths of the prefix groups.
 __device__ __forceinline__ RowQueries group_queries(const Params &p, int g) {

@@ -153,7 +153,7 @@ __device__ __forceinline__ bool own_item(const Params &p, uint32_t index, Item &
     s.plen = group_length(p, g);
   }
   s.own = own_begin(s.plen);
-  s.see = len - t.count + 1;
+  s.see = own_see(p, len, t);
   const int last = (min(s.m0 + p.tile_own, s.rows) - 1) / p.group;
   const int64_t begin = (int64_t)s.slot * p.chunk_own;
   const int seen = min(len, s.see + last);
@@ -490,7 +490,7 @@ __global__ __launch_bounds__((kPerGroup<D> * kWave), (D == 256 ? 1 : 2)) void we
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = lane_id(), half = lane / 32, n = lane % 32;
   const RowQueries t = row_queries(p, row);
-  const int see = len - t.count + 1, rows = min(t.count, p.max_query) * p.group;
+  const int see = own_see(p, len, t), rows = min(t.count, p.max_query) * p.group;
   const int32_t *table = p.table + (int64_t)row * p.table_stride;
   const int at = begin + lane;
   int page = -1;

@@ -59,7 +59,7 @@ class Attention(ctypes.Structure):
         ("q_dtype", _i32), ("kv_dtype", _i32), ("rows", _i32), ("width", _i32), ("prefix_groups", _i32),
         ("prefix_width", _i32), ("tokens", _i32), ("max_query", _i32), ("q_heads", _i32), ("kv_heads", _i32),
         ("head_dim", _i32), ("block_size", _i32),
-        ("scale", _f32), ("k_scale", _f32), ("v_scale", _f32), ("decay", _f32),
+        ("scale", _f32), ("k_scale", _f32), ("v_scale", _f32), ("decay", _f32), ("kept", _i32),
     ]
 
 

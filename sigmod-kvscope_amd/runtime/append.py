@@ -70,7 +70,8 @@ def append_tokens(
     other row uses).  Row r's new tokens are ``q_start[r] .. q_start[r + 1]`` (None: one a row), at most ``max_query``,
     and the last of its ``lens[r]`` tokens, as ``prefix_attention`` takes them afterwards; with ``advance`` they come
     behind the ``lens[r]`` that it has, and the call adds them to ``lens`` (and ``seen``; neither shares memory with the
-    other or with ``first``).  A token whose slot is outside
+    other or with ``first``; ``prefix_attention`` takes them with this ``max_query`` as its
+    ``kept``).  A token whose slot is outside
     the row's table, or behind an entry that is no page, is not written.  Tokens of no row write nothing, and their
     queries come back 0.
 

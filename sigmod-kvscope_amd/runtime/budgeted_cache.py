@@ -67,6 +67,7 @@ class BudgetedCache:
         self.scores, self.positions = self._all_scores[:rows], self._all_positions[:rows]
         self._other_lens = torch.zeros_like(self.lens)
         self.longest = 0  # no row has more tokens (the device alone knows each row's)
+        self._kept = 0  # the most tokens of a row that the last append kept
         self.rotation = rotation
         # append_tokens writes what torch's indexing would, a dozen launches of it in one
         self._one_pass = self.kv.is_cuda and dim % 16 == 0 and dim <= 256 and dtype in _CACHE_TYPES
@@ -158,6 +159,7 @@ class BudgetedCache:
             query = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start, max_query=max_query,
                                   seen=self.seen, scores=self.scores, slot_positions=self.positions, advance=True, **how)
             self.longest += max_query
+            self._kept = max_query
             return query
         token = torch.arange(n, device=device)
         if q_start is None:
@@ -180,16 +182,19 @@ class BudgetedCache:
         self.lens += counts
         self.seen += counts
         self.longest += max_query
+        self._kept = max_query
         return None
 
     def attend(self, query: torch.Tensor, scale: float, q_start: torch.Tensor | None = None, max_query: int = 1):
-        """``(out, lse)`` of the newest tokens' queries ``[tokens, q_heads, dim]``; the own tokens' scores grow by the weight
-        they received."""
+        """``(out, lse)`` of the newest tokens' queries ``[tokens, q_heads, dim]``, with the ``q_start`` that they were
+        appended with (what the append did not keep gets 0 and -inf); the own tokens' scores grow by the weight they
+        received."""
         shared = self.prefix_table is not None
+        kept = self._kept if max_query <= self._kept else 0  # more queries than the last append can have kept: several appends'
         return prefix_attention(
             query, self.kv, self.table, self.lens, scale, q_start=q_start, max_query=max_query,
             prefix_table=self.prefix_table, prefix_lens=self.prefix_len if shared else None, k_scale=self.k_scale,
-            v_scale=self.v_scale, scores=self.scores, decay=self.decay)
+            v_scale=self.v_scale, scores=self.scores, decay=self.decay, kept=kept)
 
     def trim(self) -> None:
         """Back to the budget: the tokens that received least are gone."""

@@ -53,7 +53,7 @@ def _sound(device: int, ints, *rows) -> bool:
 
 
 def _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table, prefix_lens, prefix_rows,
-               k_scale, v_scale, scores, decay, out, lse):
+               k_scale, v_scale, scores, decay, kept, out, lse):
     pages, block, kv_heads, dim = _cache_shape(kv_cache)
     if not isinstance(query, torch.Tensor) or query.ndim != 3 or query.shape[2] != dim:
         raise ValueError(f"query must be a [tokens, heads, {dim}] tensor")
@@ -121,7 +121,7 @@ def _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_t
         at_prefix_lens, at_prefix_rows, at_scores, score_row, score_head, out.data_ptr(), o_token, o_head,
         lse.data_ptr(), ekv_hip.dtype_code(dtype), ekv_hip.dtype_code(kv_cache.dtype), rows, width,
         groups, prefix_width, tokens, max_query, q_heads, kv_heads, dim, block, scale, k_scale, v_scale,
-        decay), out, lse, device
+        decay, kept), out, lse, device
 
 
 def prefix_attention(
@@ -140,6 +140,7 @@ def prefix_attention(
     v_scale: float = 1.0,
     scores: torch.Tensor | None = None,
     decay: float = 1.0,
+    kept: int = 0,
     out: torch.Tensor | None = None,
     lse: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
@@ -152,7 +153,9 @@ def prefix_attention(
     included (a ``DecodeView``'s buffers serve).  Row r's query tokens are ``q_start[r] .. q_start[r + 1]``
     (None: one a row) and the last of its own tokens; query i of t sees slots up to ``len - t + i``.
     ``max_query`` bounds a row's query tokens; what passes it, or is no row's, gets 0 and -inf, as a query
-    that sees nothing does.
+    that sees nothing does.  ``kept``: the lengths count no more than so many of a row's query tokens (0: all of
+    them), as ``append_tokens`` of that ``max_query`` leaves them with ``advance``; query i then sees slots up to
+    ``len - min(t, kept) + i``.
 
     ``prefix_table`` int32 ``[groups, pages]`` and ``prefix_lens`` int32 ``[groups]``: shared prefixes, seen
     whole by every query of rows ``prefix_rows[g] .. prefix_rows[g + 1]`` (ascending; None: one group of
@@ -168,7 +171,7 @@ def prefix_attention(
     is taken through the call."""
     with ekv_hip.on_stream(stream, query):
         arguments, out, lse, device = _arguments(query, kv_cache, table, lens, scale, q_start, max_query, prefix_table,
-                                                 prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, out, lse)
+                                                 prefix_lens, prefix_rows, k_scale, v_scale, scores, decay, kept, out, lse)
         lib = ekv_hip._lib or ekv_hip.load()
         need = lib.ekv_prefix_attention_workspace(arguments)
         if workspace is None:
