@@ -214,13 +214,30 @@ __device__ __forceinline__ int quotient(int i, const PageDivisor &d) { return (i
 // Which products are fused with which sums is written out, so that a head's result is the same bits in every kernel.
 
 // 1 / the root mean square of the head whose elements the lanes hold, two units each (a lane that is not `mine` holds none).
+// Elements whose squares vanish beside an eps next to 0 come back 2^100 times larger, and the result is theirs.
 // All lanes of the wave are active.
-__device__ __forceinline__ float over_rms(const Params &p, const float (&x)[kUnit], const float (&y)[kUnit], bool mine, int lanes) {
+__device__ __forceinline__ float over_rms(const Params &p, float (&x)[kUnit], float (&y)[kUnit], bool mine, int lanes) {
   float squares = 0.f;
 #pragma unroll
   for (int e = 0; e < kUnit; ++e) squares = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], squares));
   squares = head_sum(mine ? squares : 0.f, lanes);
-  float over = rsqrtf(__builtin_fmaf(squares, p.mean, p.eps));
+  const float mean = __builtin_fmaf(squares, p.mean, p.eps);
+  float over = rsqrtf(mean);
+  // From 2^-100 on, squares below float32's least are nothing beside the others or eps; below it again, of elements whose
+  // scaling is exact: float32's least becomes 2^-49, and what has a mean below 2^-100 stays below 2^54.
+  const bool vanish = mean < 0x1p-100f;
+  if (__any(mine && vanish)) {
+    const float up = vanish ? 0x1p100f : 1.f;
+    float large = 0.f;
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) {
+      x[e] *= up;
+      y[e] *= up;
+      large = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], large));
+    }
+    large = head_sum(mine ? large : 0.f, lanes);
+    if (vanish) over = rsqrtf(__builtin_fmaf(large, p.mean, p.eps * 0x1p100f * 0x1p100f));
+  }
   if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
     float small = 0.f;
 #pragma unroll
