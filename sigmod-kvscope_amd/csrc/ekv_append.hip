@@ -214,7 +214,7 @@ __device__ __forceinline__ int quotient(int i, const PageDivisor &d) { return (i
 // Which products are fused with which sums is written out, so that a head's result is the same bits in every kernel.
 
 // 1 / the root mean square of the head whose elements the lanes hold, two units each (a lane that is not `mine` holds none).
-// Elements whose squares vanish beside an eps next to 0 come back 2^100 times larger, and the result is theirs.
+// Elements whose squares vanish beside an eps next to 0, or pass float32, come back scaled, and the result is theirs.
 // All lanes of the wave are active.
 __device__ __forceinline__ float over_rms(const Params &p, float (&x)[kUnit], float (&y)[kUnit], bool mine, int lanes) {
   float squares = 0.f;
@@ -238,7 +238,10 @@ __device__ __forceinline__ float over_rms(const Params &p, float (&x)[kUnit], fl
     large = head_sum(mine ? large : 0.f, lanes);
     if (vanish) over = rsqrtf(__builtin_fmaf(large, p.mean, p.eps * 0x1p100f * 0x1p100f));
   }
-  if (__any(squares == __builtin_inff())) {  // squares past float32: again, of elements 2^80 times smaller
+  // Squares past float32: again, of elements 2^80 times smaller.  The norm's inverse is then down to 2^-128, where float32
+  // has no bits left for its product with a weight: the elements take it, all but 2^-80 of it.
+  const bool past = squares == __builtin_inff();
+  if (__any(mine && past)) {
     float small = 0.f;
 #pragma unroll
     for (int e = 0; e < kUnit; ++e) {
@@ -246,7 +249,13 @@ __device__ __forceinline__ float over_rms(const Params &p, float (&x)[kUnit], fl
       small = __builtin_fmaf(u, u, __builtin_fmaf(v, v, small));
     }
     small = head_sum(mine ? small : 0.f, lanes);
-    if (squares == __builtin_inff()) over = rsqrtf(small * p.mean) * 0x1p-80f;
+    const float root = past ? rsqrtf(__builtin_fmaf(small, p.mean, p.eps * 0x1p-80f * 0x1p-80f)) : 1.f;
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) {
+      x[e] *= root;
+      y[e] *= root;
+    }
+    if (past) over = 0x1p-80f;
   }
   return over;
 }

@@ -1,4 +1,4 @@
-"""Norms of heads whose squares leave float32: small elements with an eps of 0 or next to it."""
+"""Norms of heads whose squares leave float32: small elements with an eps of 0 or next to it, large ones with small weights."""
 
 import numpy as np
 import pytest
@@ -91,3 +91,16 @@ def test_keys_on_their_way_into_a_cache(dtype):
     close(query, want, dtype)
     close(cache[:, 0, 0], want, dtype)
     assert torch.equal(cache[:, 1, 0], x)
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("weight", [1.0, 1e-2, 1e-4, 1e-8])
+@pytest.mark.parametrize("tokens,count", [(12, 3), (8200, 1)])
+def test_large_elements_with_small_weights(dtype, weight, tokens, count):
+    x = heads(tokens, count, [1.0, 2.0**64, 2.0**90, 2.0**110, 2.0**124], dtype, 3).clamp(-3e38, 3e38)
+    w = weight * (1 + 0.3 * torch.rand(DIM, generator=seeded(5), device="cuda"))
+    got, _ = rotate_heads(x, None, None, None, q_weight=w, eps=1e-6)
+    close(got, normed(x, w, 1e-6), dtype)
+    mixed = x.clone()  # small elements beside large ones
+    mixed[..., ::2] *= 2.0**-60
+    got, _ = rotate_heads(mixed, None, None, None, q_weight=w, eps=1e-6)
+    close(got, normed(mixed, w, 1e-6), dtype)
