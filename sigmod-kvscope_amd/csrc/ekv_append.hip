@@ -223,39 +223,21 @@ __device__ __forceinline__ float over_rms(const Params &p, float (&x)[kUnit], fl
   squares = head_sum(mine ? squares : 0.f, lanes);
   const float mean = __builtin_fmaf(squares, p.mean, p.eps);
   float over = rsqrtf(mean);
-  // From 2^-100 on, squares below float32's least are nothing beside the others or eps; below it again, of elements whose
-  // scaling is exact: float32's least becomes 2^-49, and what has a mean below 2^-100 stays below 2^54.
-  const bool vanish = mean < 0x1p-100f;
-  if (__any(mine && vanish)) {
-    const float up = vanish ? 0x1p100f : 1.f;
-    float large = 0.f;
+  // From 2^-100 on, squares below float32's least are nothing beside the others or eps.  A mean below it, or squares past
+  // float32: again, of scaled elements.  2^100 is exact, float32's least becomes 2^-49 and what has a mean below 2^-100 stays
+  // below 2^54.  2^-70 takes the largest to 2^58, and bits of elements below 2^-56 alone, beside one of 2^60 or more.
+  const bool vanish = mean < 0x1p-100f, past = squares == __builtin_inff();
+  if (__any(mine && (vanish || past))) {
+    const float by = vanish ? 0x1p100f : past ? 0x1p-70f : 1.f;
+    squares = 0.f;
 #pragma unroll
     for (int e = 0; e < kUnit; ++e) {
-      x[e] *= up;
-      y[e] *= up;
-      large = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], large));
+      x[e] *= by;
+      y[e] *= by;
+      squares = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], squares));
     }
-    large = head_sum(mine ? large : 0.f, lanes);
-    if (vanish) over = rsqrtf(__builtin_fmaf(large, p.mean, p.eps * 0x1p100f * 0x1p100f));
-  }
-  // Squares past float32: again, of elements 2^80 times smaller.  The norm's inverse is then down to 2^-128, where float32
-  // has no bits left for its product with a weight: the elements take it, all but 2^-80 of it.
-  const bool past = squares == __builtin_inff();
-  if (__any(mine && past)) {
-    float small = 0.f;
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) {
-      const float u = x[e] * 0x1p-80f, v = y[e] * 0x1p-80f;
-      small = __builtin_fmaf(u, u, __builtin_fmaf(v, v, small));
-    }
-    small = head_sum(mine ? small : 0.f, lanes);
-    const float root = past ? rsqrtf(__builtin_fmaf(small, p.mean, p.eps * 0x1p-80f * 0x1p-80f)) : 1.f;
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) {
-      x[e] *= root;
-      y[e] *= root;
-    }
-    if (past) over = 0x1p-80f;
+    squares = head_sum(mine ? squares : 0.f, lanes);
+    over = rsqrtf(__builtin_fmaf(squares, p.mean, p.eps * by * by));
   }
   return over;
 }
@@ -468,8 +450,11 @@ __device__ __forceinline__ void advance_row(const Params &p, int row, int t) {
 
 // T: the inputs' type.  C: the cache's (FP8 or T).  PAGED: with a cache and values; else keys go to k_out.  NORM: what
 // weights there are.  ADJACENT: the order of the pairs.  PAST: what goes past the caches.
+// Waves a SIMD: those of 16-bit heads with their own weights are asked for (one fewer, by two registers, took 68.5 us where
+// 16384 tokens of 32 query and 8 KV heads of 128 into an fp8 cache take 65, and 41.5 where crowd_kernel takes 36 for 65536
+// tokens of 4 and 1 heads); the others come out at 5 to 8 by themselves.
 template <class T, class C, bool PAGED, Norm NORM, bool ADJACENT, Past PAST>
-__global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
+__global__ __launch_bounds__(kWaves *kWave, (sizeof(T) == 2 && NORM == kOfHeads ? 6 : 1)) void heads_kernel(Params p) {
   __shared__ __align__(16) float s_cos[kWaves][kMostPairs], s_sin[kWaves][kMostPairs];
   __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2][2 * kMostPairs];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
@@ -639,7 +624,7 @@ __global__ __launch_bounds__(kWaves *kWave) void heads_kernel(Params p) {
 // Heads without a cache, several tokens a wave: where a token's heads leave most of a pass idle, a pass takes the heads of one
 // kind of `crowd` tokens in a row.  Their angles are spread over all lanes, and each lane reads its token's for each pass.
 template <class T, Norm NORM, bool ADJACENT, Past PAST>
-__global__ __launch_bounds__(kWaves *kWave) void crowd_kernel(Params p) {
+__global__ __launch_bounds__(kWaves *kWave, (sizeof(T) == 2 && NORM == kOfHeads ? 8 : 1)) void crowd_kernel(Params p) {
   constexpr int kMostTurns = kWave * kUnit;  // of the wave's tokens: no more than a pass has heads, 8 pairs a lane
   __shared__ __align__(16) float s_cos[kWaves][kMostTurns], s_sin[kWaves][kMostTurns];
   __shared__ __align__(16) float s_weight[NORM == kShared ? kWaves : 1][2][2 * kMostPairs];
