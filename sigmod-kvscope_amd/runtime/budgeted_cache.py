@@ -156,8 +156,9 @@ class BudgetedCache:
                     how["first"] = self.prefix_len.expand(rows)
             else:
                 keys, values = self._new(keys, values)
-            query = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start, max_query=max_query,
-                                  seen=self.seen, scores=self.scores, slot_positions=self.positions, advance=True, **how)
+            query = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start,
+                                  max_query=1 if start is None else max_query, seen=self.seen, scores=self.scores,
+                                  slot_positions=self.positions, advance=True, **how)
             self.longest += max_query
             self._kept = max_query
             return query
