@@ -616,7 +616,8 @@ typedef struct ekv_rotation {
  * norms and rotations are float32, its angles float64 until they are less than a turn; the result is
  * rounded once, to the inputs' type.
  * Types: fp32, f16 or bf16; weights of the same type or fp32.  head_dim a multiple of 16, at most 256; pairs
- * a multiple of 8 (0: norms alone); rows of every tensor start at multiples of 16 bytes.
+ * a multiple of 8 (0: norms alone); rows of every tensor start at multiples of 16 bytes; no two heads of an
+ * output share memory.
  */
 int ekv_rotate_heads(const ekv_rotation_t *a, void *stream);
 

@@ -849,6 +849,20 @@ int fill(const Block *a, Params &p, const char *who) {
 bool row_aligned(const Heads &h) { return aligned16(h.at) && h.token % 16 == 0 && h.head % 16 == 0; }
 bool weight_aligned(const char *at, int64_t stride) { return aligned16(at) && stride % 16 == 0; }
 
+// Whether no two of the rows [tokens, heads] of `bytes` bytes share memory.
+bool apart(const Heads &h, int64_t tokens, int64_t heads, int64_t bytes) {
+  typedef unsigned __int128 Wide;  // products of strides and counts
+  const Wide token = h.token < 0 ? -(Wide)h.token : (Wide)h.token, head = h.head < 0 ? -(Wide)h.head : (Wide)h.head;
+  if (tokens < 1 || heads < 1) return true;
+  if ((tokens > 1 && token < (Wide)bytes) || (heads > 1 && head < (Wide)bytes)) return false;
+  if (tokens < 2 || heads < 2 || token >= head * (Wide)(heads - 1) + bytes || head >= token * (Wide)(tokens - 1) + bytes) return true;
+  for (int64_t j = 1; j < heads; ++j) {  // neither axis lies within the other's steps: the tokens nearest to j heads on
+    const Wide n = head * (Wide)j / token, off = head * (Wide)j % token;
+    if ((n < (Wide)tokens && off < (Wide)bytes) || (n + 1 < (Wide)tokens && token - off < (Wide)bytes)) return false;
+  }
+  return true;
+}
+
 // Whether m counts from a and n from b have one in common.
 bool share(const int32_t *a, int64_t m, const int32_t *b, int64_t n) {
   return a != nullptr && b != nullptr && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)(a + m);
@@ -880,6 +894,9 @@ extern "C" int ekv_rotate_heads(const ekv_rotation_t *a, void *stream) {
       !append::row_aligned(p.out[kKey]) || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads and weights start at multiples of 16 bytes", who);
+  if (!append::apart(p.out[kQuery], p.tokens, p.q_heads, (int64_t)p.dim * e) ||
+      !append::apart(p.out[kKey], p.tokens, p.kv_heads, (int64_t)p.dim * e))
+    return fail(EKV_EINVAL, "%s: heads of an output share memory", who);
   if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
@@ -954,6 +971,8 @@ extern "C" int ekv_append_tokens(const ekv_append_t *a, void *stream) {
       p.st_pos % 16 != 0 || p.st_head % 16 != 0 || !append::weight_aligned(p.q_weight, p.q_weight_stride) ||
       !append::weight_aligned(p.k_weight, p.k_weight_stride))
     return fail(EKV_EINVAL, "%s: heads, weights and the cache's rows start at multiples of 16 bytes", who);
+  if (!append::apart(p.out[kQuery], p.tokens, p.q_heads, (int64_t)p.dim * e))
+    return fail(EKV_EINVAL, "%s: heads of an output share memory", who);
   if (p.table_stride < p.width)
     return fail(EKV_EINVAL, "%s: table rows of %d blocks, stride %lld", who, p.width, (long long)p.table_stride);
   if (p.tokens >= append::kMostWaves) return fail(EKV_EINVAL, "%s: %d tokens pass the threads of a launch", who, p.tokens);

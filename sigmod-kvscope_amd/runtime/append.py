@@ -82,10 +82,10 @@ def append_tokens(
     ``saturate``, as NaN without.
 
     ``scores`` float32 and ``slot_positions`` int32 ``[rows, kv_heads, slots]``: 0 and the token's index (without
-    ``first``) at each new slot, for every KV head.  ``q_out`` may be ``query`` itself and overlaps nothing else.  Types
-    and limits as ``ekv_append_tokens`` documents them.  ``stream``: the call launches and allocates as under
-    ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
-    through the call."""
+    ``first``) at each new slot, for every KV head.  ``q_out`` may be ``query`` itself; its heads overlap
+    nothing else, nor each other.  Types and limits as ``ekv_append_tokens`` documents them.  ``stream``: the call launches
+    and allocates as under ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No
+    gradient is taken through the call."""
     if not isinstance(kv_cache, _Tensor) or kv_cache.ndim != 5:
         _cache_shape(kv_cache)  # refuses it
     pages, _, block, kv_heads, dim = c_shape = kv_cache.shape

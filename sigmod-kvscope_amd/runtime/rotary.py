@@ -161,10 +161,10 @@ def rotate_heads(
     divided by its root mean square (``eps`` added to the mean square) and multiplied by ``weight_offset`` plus its
     weights.  None: that tensor is not normed.
 
-    ``q_out`` and ``k_out`` may be ``query`` and ``key`` themselves and overlap nothing else.  Types, head dims and
-    limits as ``ekv_rotate_heads`` documents them.  ``stream``: the call launches and allocates as under
-    ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is taken
-    through the call."""
+    ``q_out`` and ``k_out`` may be ``query`` and ``key`` themselves; their heads overlap nothing else, nor each other.
+    Types, head dims and limits as ``ekv_rotate_heads`` documents them.  ``stream``: the call launches and allocates as
+    under ``torch.cuda.stream(stream)``; the caller orders it after the work that makes its inputs.  No gradient is
+    taken through the call."""
     q_shape, dtype, device, q_at, q_token, q_head, sound = _look("query", query)
     tokens, q_heads, dim = q_shape
     k_shape, kv_heads, k_at, k_token, k_head = None, 0, 0, 0, 0
