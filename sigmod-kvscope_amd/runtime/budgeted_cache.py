@@ -40,7 +40,9 @@ class BudgetedCache:
     accumulated before it; ``k_scale`` / ``v_scale``: an fp8 cache's scales; ``rotation``: the arguments of ``append_tokens``
     that norm and rotate (``frequencies``, ``axes``, ``adjacent``, ``rotary_scale``, ``q_weight``, ``k_weight``, ``eps``,
     ``weight_offset``).  Keys and values then come as the model made them and are divided by the scales here; without it they
-    come rotated and already over the scales."""
+    come rotated and already over the scales.  Either way they may be of any type: they are rounded to the cache's first.  An
+    fp8 cache takes float32 and 16-bit ones as they are (a rotation's all of one type, else through float32) and holds what
+    passes +-448 as that with a rotation, as NaN without."""
 
     def __init__(self, rows: int, kv_heads: int, dim: int, budget: int, slack: int = 64, *, prefix: int = 0,
                  block: int = 16, dtype: torch.dtype = torch.bfloat16, recent: int = 32, sinks: int = 4,
@@ -88,18 +90,24 @@ class BudgetedCache:
             rows = rows.to(self.kv.dtype)
             raw[page, part, slot % self.block] = rows.view(torch.uint8) if raw is not self.kv else rows
 
-    def _new(self, *new: torch.Tensor) -> list[torch.Tensor]:
-        """Keys and values as append_tokens takes them: of the cache's type (or one it rounds from), at multiples of 16 bytes."""
+    def _new(self, *new: torch.Tensor | None) -> list[torch.Tensor | None]:
+        """Keys, values and queries as append_tokens takes them: of the cache's type (or one it rounds from), at multiples of
+        16 bytes."""
         kind = self.kv.dtype
         if kind == torch.float8_e4m3fn:
-            kind = new[0].dtype if new[0].dtype in _CACHE_TYPES[:3] and new[0].dtype == new[1].dtype else torch.float32
+            kind = new[0].dtype
+            for rows in new:
+                if kind not in _CACHE_TYPES[:3] or (rows is not None and rows.dtype is not kind):
+                    kind = torch.float32
         ready = []
+        size = 4 if kind is torch.float32 else 2
         for rows in new:
-            rows = rows.to(kind)
-            token, head, one = rows.stride()
-            size = rows.element_size()
-            if one != 1 or rows.data_ptr() % 16 or (rows.shape[0] > 1 and token * size % 16) or (rows.shape[1] > 1 and head * size % 16):
-                rows = rows.clone(memory_format=torch.contiguous_format)
+            if rows is not None:
+                if rows.dtype is not kind:
+                    rows = rows.to(kind)
+                token, head, one = rows.stride()
+                if one != 1 or (rows.data_ptr() | token * size | head * size) & 15:
+                    rows = rows.clone(memory_format=torch.contiguous_format)
             ready.append(rows)
         return ready
 
@@ -113,8 +121,9 @@ class BudgetedCache:
             raise ValueError(f"no room for a prefix of {n} tokens")
         if self.rotation is not None:
             start = torch.arange(2, dtype=torch.int32, device=self.kv.device) * n
+            keys, values = self._new(keys, values)
             append_tokens(self.kv, self.prefix_table, start[1:], keys, values, q_start=start, max_query=max(1, n),
-                          positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(None))
+                          positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(None, keys.dtype))
             self.prefix_len.fill_(n)
             return
         if positions is not None:
@@ -123,9 +132,12 @@ class BudgetedCache:
         self._write(self.prefix_table[0, slot // self.block].long(), slot, keys, values)
         self.prefix_len.fill_(n)
 
-    def _turn(self, query) -> dict:
-        """The rotation's arguments, without the queries' weights where there are no queries."""
-        return self.rotation if query is not None else {k: v for k, v in self.rotation.items() if k != "q_weight"}
+    def _turn(self, query, kind: torch.dtype) -> dict:
+        """The rotation's arguments for heads of type ``kind``, without the queries' weights where there are no queries."""
+        how = self.rotation if query is not None else {k: v for k, v in self.rotation.items() if k != "q_weight"}
+        if kind == torch.float32:  # what came of other types meets weights of other types here too
+            how = {k: v.float() if k.endswith("_weight") and v is not None else v for k, v in how.items()}
+        return how
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, q_start: torch.Tensor | None = None, max_query: int = 1, *,
                query: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -133,11 +145,14 @@ class BudgetedCache:
         row), at most ``max_query``.  What passes it, or is no row's (padding before or behind the rows'), is not kept: the
         device alone knows the counts, and no row outgrows its pages whatever they are.
 
-        With ``rotation``: ``query [tokens, q_heads, dim]`` comes back normed and rotated; a token's position is the prefix's
-        length plus the count of its row's tokens before it, or ``positions`` int32 ``[tokens]`` or ``[axes, tokens]``."""
+        With ``rotation``: ``query [tokens, q_heads, dim]`` comes back normed and rotated, of the cache's type (an fp8 cache's
+        queries of their own); a token's position is the prefix's length plus the count of its row's tokens before it, or
+        ``positions`` int32 ``[tokens]`` or ``[axes, tokens]``."""
         self._check(keys, values)
         if self.rotation is None and (query is not None or positions is not None):
             raise ValueError("a query and positions need a rotation")
+        if query is not None and query.ndim != 3:
+            raise ValueError(f"query must be [tokens, heads, {keys.shape[2]}], got {tuple(query.shape)}")
         rows, n, device = self.lens.shape[0], keys.shape[0], self.kv.device
         if q_start is None and n != rows:
             raise ValueError(f"{n} tokens of {rows} rows need q_start")
@@ -150,18 +165,20 @@ class BudgetedCache:
         if self.rotation is not None or self._one_pass:
             start = None if q_start is None else q_start.to(torch.int32).contiguous()
             how = dict(saturate=False)
+            keys, values, heads = self._new(keys, values, query)
             if self.rotation is not None:
-                how = dict(query=query, positions=positions, k_scale=self.k_scale, v_scale=self.v_scale, **self._turn(query))
+                how = dict(query=heads, positions=positions, k_scale=self.k_scale, v_scale=self.v_scale,
+                           **self._turn(query, keys.dtype))
                 if self.prefix_table is not None:
                     how["first"] = self.prefix_len.expand(rows)
-            else:
-                keys, values = self._new(keys, values)
-            query = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start,
+            heads = append_tokens(self.kv, self.table, self.lens, keys, values, q_start=start,
                                   max_query=1 if start is None else max_query, seen=self.seen, scores=self.scores,
                                   slot_positions=self.positions, advance=True, **how)
             self.longest += max_query
             self._kept = max_query
-            return query
+            if heads is not None and heads.dtype is not query.dtype and self.kv.dtype == torch.float8_e4m3fn:
+                heads = heads.to(query.dtype)
+            return heads
         token = torch.arange(n, device=device)
         if q_start is None:
             row = into = token
