@@ -747,11 +747,15 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   p.q_passes = (int)ceil_div(p.q_heads, kWave >> p.lanes_log);
   p.kv_passes = (int)ceil_div(p.kv_heads, kWave >> p.lanes_log);
   const int passes = p.q_passes + (PAGED ? 2 : 1) * p.kv_passes;
-  // What goes past the 256 MB Infinity Cache (cache pages always do), by what the launch moves; 32 query and 8 KV heads of
-  // 128 in bf16, alone and followed by a kernel that reads the rotated queries, us: prompts of 117 MB 22 / 36 with the loads
-  // in the caches, 24 / 39 with neither loads nor queries in them; of 235 MB 49 / 75, 41 / 63 without the loads, 45 / 70
-  // without both; of 470 MB 92 / 142, 90 / 138 and 87 / 137; of 940 MB 172 / 277, 182 / 283 and 163 / 268.  Pieces that do not
-  // fill lines of 128 bytes are read twice past the caches: 500 MB of heads of 80 95 / 162, 105 / 173 and 112 / 180.
+  // What goes past the 256 MB Infinity Cache, by what the launch moves (cache pages do in any launch, but for fp8 units of 8
+  // bytes).  Measured, us, alone / with a kernel behind that reads the rotated queries, as nothing, the loads, loads and
+  // queries go past; MiB.  32 query and 8 KV heads of 128 in bf16: 120 25.5 / 45.0, 24.4 / 41.3, 25.2 / 43.8; 220 46.9 / 77.9,
+  // 40.9 / 69.6, 41.4 / 74.8; 280 56.9 / 99.6, 54.4 / 86.8, 51.7 / 92.6; 340 68 / 116, 67 / 109, 62 / 111; 500 98 / 165,
+  // 97 / 161, 90 / 159; into a cache 900 172 / 277, 182 / 283, 163 / 268.  Pieces that do not fill lines of 128 bytes are read
+  // twice past the caches, which the next kernel's reads make good for in smaller launches alone: heads of 80 180 41.2 / 65.9,
+  // 41.1 / 64.1, 46.6 / 74.1; 280 59.5 / 100, 63.8 / 96, 70.0 / 110; 340 71 / 118, 77 / 118, 84 / 132; 500 101 / 168, 110 / 179,
+  // 121 / 190; of 96 the same.  fp32 heads of 128, nothing and loads: 180 42.3 / 67.5, 39.7 / 63.6; 280 59.5 / 100, 60.0 / 93;
+  // 340 71 / 119, 74 / 116; 500 100 / 170, 104 / 174.
   const int64_t cache_bytes = std::is_same<C, attn::FP8>::value ? 1 : sizeof(T);
   const int64_t moved = p.tokens * (int64_t)p.dim *
                         ((2ll * p.q_heads + 2 * p.kv_heads) * sizeof(T) + (PAGED ? 2 * p.kv_heads * cache_bytes : 0));
@@ -762,7 +766,7 @@ int launch_norm(Params p, hipStream_t stream, const char *who) {
   // it does once, its token's place and angles: two waves from five passes on (16384 tokens' norms, five passes, 60 us, 61
   // with one, 66 with four; 9536 tokens of 16 query and 2 KV heads into a cache, four passes, 21.8, 20.6 with one, 29.3 with
   // four; of 8 and 1, three, 19.3, 16.7, 27.4), and four where the launch outlasts its caches, has no weights to load and six
-  // passes (38000 tokens 156 us, 167 with two, 173 with one).
+  // passes (38000 tokens of 32 query and 8 KV heads 156 us, 167 with two, 173 with one; no other shape was measured).
   const bool few = p.tokens * 4ll <= 16ll * cu_count();
   p.parts = few || (past == kAll && NORM == kNone && passes > 5) ? 4 : passes >= 5 ? 2 : 1;
   while (p.parts > 1 && p.parts / 2 >= passes) p.parts /= 2;
